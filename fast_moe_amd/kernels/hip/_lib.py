@@ -28,6 +28,7 @@ EXPORTED_SYMBOLS = (
     "fmoe_silu_mul", "fmoe_transpose_last2", "fmoe_jagged_transpose", "fmoe_segment_colsum",
     "fmoe_swiglu_bwd", "fmoe_combine_bwd", "fmoe_gather_rows", "fmoe_invert_index",
     "fmoe_gate_l1_bwd", "fmoe_gate_softmax_pays", "fmoe_gate_softmax", "fmoe_gate_route_pays", "fmoe_weight_grad_pays", "fmoe_weight_grad", "fmoe_route_topk_static", "fmoe_hbm_probe",
+    "fmoe_few_tokens_workspace_bytes", "fmoe_few_tokens",
 )
 ROUTE_STATIC_MAX_POSITIONS, ROUTE_STATIC_MAX_EXPERTS = 1 << 20, 512
 
@@ -54,6 +55,22 @@ class GemmDesc(ctypes.Structure):
         ("aux_stride_row", c_int64),
         ("a_stride_k", c_int64),
         ("a2", c_void_p), ("k2", c_int32), ("scale_pow2", c_int32), ("out2", c_void_p),
+    ]
+
+
+class FewDesc(ctypes.Structure):
+    """struct fmoe_few_desc, field for field."""
+    _fields_ = [
+        ("T", c_int32), ("E", c_int32), ("k", c_int32), ("D", c_int32), ("H", c_int32), ("O", c_int32),
+        ("dtype", c_int32), ("weight_dtype", c_int32), ("renorm", c_int32),
+        ("x", c_void_p), ("x_stride_row", c_int64), ("gate_weight", c_void_p), ("gate_stride_row", c_int64),
+        ("gate_bias", c_void_p), ("token_mask", c_void_p),
+        ("w", c_void_p), ("wp", c_void_p), ("w_stride_e", c_int64), ("w_stride_n", c_int64),
+        ("wo", c_void_p), ("wo_stride_e", c_int64), ("wo_stride_n", c_int64),
+        ("w_scale", c_void_p), ("wp_scale", c_void_p), ("wo_scale", c_void_p),
+        ("bias", c_void_p), ("bias_p", c_void_p), ("bias_stride_e", c_int64),
+        ("bias_out", c_void_p), ("bias_out_stride_e", c_int64),
+        ("out", c_void_p), ("out_stride_row", c_int64),
     ]
 
 
@@ -142,6 +159,10 @@ def load() -> ctypes.CDLL:
     lib.fmoe_gate_l1_bwd.argtypes = [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.fmoe_hbm_probe.restype = c_int
     lib.fmoe_hbm_probe.argtypes = [c_void_p, c_int64, c_int, c_int, c_void_p]
+    lib.fmoe_few_tokens_workspace_bytes.restype = c_size_t
+    lib.fmoe_few_tokens_workspace_bytes.argtypes = [POINTER(FewDesc)]
+    lib.fmoe_few_tokens.restype = c_int
+    lib.fmoe_few_tokens.argtypes = [POINTER(FewDesc), c_void_p, c_size_t, c_void_p]
     _lib = lib
     return lib
 

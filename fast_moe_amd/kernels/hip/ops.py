@@ -4,6 +4,7 @@ memory and streams only; every computation below happens in libfastmoe_hip.so.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Dict, Optional, Tuple
@@ -11,7 +12,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import EPI_GATED, EPI_NONE, EPI_SILU, EPI_SWIGLU, FMOE_BF16, FMOE_E4M3, FMOE_F32, GemmDesc
+from ._lib import EPI_GATED, EPI_NONE, EPI_SILU, EPI_SWIGLU, FMOE_BF16, FMOE_E4M3, FMOE_F32, FewDesc, GemmDesc
 
 _DTYPE_CODE = {torch.float32: FMOE_F32, torch.bfloat16: FMOE_BF16}
 FP8_DTYPE = torch.float8_e4m3fn
@@ -820,3 +821,98 @@ def gate_l1_bwd(scores: torch.Tensor, topk_idx: torch.Tensor, d_gates: torch.Ten
                                       topk_idx.data_ptr(), d_gates.data_ptr(), d_scores.data_ptr(), _stream(scores))
     _lib.check(rc, "fmoe_gate_l1_bwd")
     return d_scores
+
+
+# ----------------------------------------------------- a whole layer, few tokens
+FEW_TOKENS, FEW_EXPERTS, FEW_K = 64, 256, 16       # limits of fmoe_few_tokens
+
+
+def _on_device(t: torch.Tensor):
+    """t's device as the current one while kernels are launched on a stream of it (nothing where it is already)."""
+    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def few_tokens(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias: Optional[torch.Tensor], weight: torch.Tensor,
+               bias: Optional[torch.Tensor], weight_p: Optional[torch.Tensor], bias_p: Optional[torch.Tensor],
+               weight_out: torch.Tensor, bias_out: Optional[torch.Tensor], k: int, renorm: bool = True,
+               token_mask: Optional[torch.Tensor] = None, scales=(None, None, None)) -> torch.Tensor:
+    """A whole MoE layer for a few tokens, see fmoe_few_tokens.  ``weight`` / ``weight_p`` [E, D, H] and ``weight_out``
+    [E, H, O] are views of storage with the contraction contiguous (``stride(1) == 1``), of x's dtype or, with ``scales``
+    (multipliers [E, H], [E, H], [E, O] in fp32), e4m3."""
+    name = "fused_moe_few_tokens"
+    dev = _need_cuda(name, x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out, token_mask, *scales)
+    if x.dtype not in _DTYPE_CODE:
+        raise NotImplementedError(f"{name}: the HIP kernels take bf16 or fp32 tokens, got {x.dtype}")
+    fp8 = scales[0] is not None
+    if fp8 and x.dtype != torch.bfloat16:
+        raise NotImplementedError(f"{name}: e4m3 weights go with bf16 tokens, got {x.dtype}")
+    if x.ndim != 2 or gate_weight.ndim != 2 or weight.ndim != 3 or weight_out.ndim != 3:
+        raise ValueError(f"{name}: expected x [T, D], gate_weight [E, D], weight [E, D, H], weight_out [E, H, O]")
+    T, D = x.shape
+    E, H, O = gate_weight.shape[0], weight.shape[2], weight_out.shape[2]
+    if T > FEW_TOKENS:
+        raise ValueError(f"{name}: takes up to {FEW_TOKENS} tokens, got {T}; larger batches are what the jagged operators are for")
+    if (gate_weight.shape[1] != D or tuple(weight.shape) != (E, D, H) or tuple(weight_out.shape) != (E, H, O)
+            or (weight_p is not None and weight_p.shape != weight.shape)):
+        raise ValueError(f"{name}: shapes do not fit: x {tuple(x.shape)}, gate_weight {tuple(gate_weight.shape)}, weight "
+                         f"{tuple(weight.shape)}, weight_p {None if weight_p is None else tuple(weight_p.shape)}, weight_out {tuple(weight_out.shape)}")
+    if min(D, H, O) < 1 or not 1 <= k <= min(E, FEW_K) or E > FEW_EXPERTS:
+        raise ValueError(f"{name}: need widths >= 1, 1 <= k <= E, k <= {FEW_K}, E <= {FEW_EXPERTS}, got {D=}, {H=}, {O=}, {k=}, {E=}")
+    w_dtype = FP8_DTYPE if fp8 else x.dtype
+    for what, t, want in (("gate_weight", gate_weight, x.dtype), ("weight", weight, w_dtype), ("weight_p", weight_p, w_dtype),
+                          ("weight_out", weight_out, w_dtype)):
+        if t is not None and t.dtype != want:
+            raise ValueError(f"{name}: {what} must be {want}, got {t.dtype}")
+    for what, t in (("weight", weight), ("weight_p", weight_p), ("weight_out", weight_out)):
+        if t is not None and t.shape[1] > 1 and (t.stride(1) != 1 or (t.shape[2] > 1 and t.stride(2) < t.shape[1]) or t.stride(0) < 0):
+            raise ValueError(f"{name}: {what} must be a view of storage with the contraction contiguous, as the layers keep it "
+                             f"([E, D_out, D_in].permute(0, 2, 1)); got strides {t.stride()}")
+    if weight_p is not None and weight_p.stride() != weight.stride():
+        raise ValueError(f"{name}: weight and weight_p must have the same strides, got {weight.stride()} and {weight_p.stride()}")
+    for what, t, n in (("gate_bias", gate_bias, (E,)), ("bias", bias, (E, H)), ("bias_p", bias_p, (E, H)), ("bias_out", bias_out, (E, O))):
+        if t is not None and (t.dtype != x.dtype or tuple(t.shape) != n):
+            raise ValueError(f"{name}: {what} must be {x.dtype} {n}, got {t.dtype} {tuple(t.shape)}")
+    if bias_p is not None and weight_p is None:
+        raise ValueError(f"{name}: bias_p goes with weight_p")
+    if fp8:
+        for what, t, n in (("weight", scales[0], (E, H)), ("weight_p", scales[1], (E, H)), ("weight_out", scales[2], (E, O))):
+            if what == "weight_p" and weight_p is None:
+                continue
+            if t is None or t.dtype != torch.float32 or tuple(t.shape) != n:
+                raise ValueError(f"{name}: the scales of {what} must be fp32 {n}")
+        scales = tuple(None if t is None else t.contiguous() for t in scales)
+    if token_mask is not None and (token_mask.dtype != torch.bool or tuple(token_mask.shape) != (T,)):
+        raise ValueError(f"{name}: token_mask must be bool [{T}], got {token_mask.dtype} {tuple(token_mask.shape)}")
+    out = torch.empty((T, O), dtype=x.dtype, device=dev)
+    if T == 0:
+        return out
+    x, gate_weight = _plain_rows(x), _plain_rows(gate_weight)
+    gate_bias = None if gate_bias is None else gate_bias.contiguous()
+    token_mask = None if token_mask is None else token_mask.contiguous()
+    bias, bias_p, bias_out = (None if t is None else _plain_rows(t) for t in (bias, bias_p, bias_out))
+    if bias is not None and bias_p is not None and bias.stride(0) != bias_p.stride(0):
+        bias, bias_p = bias.contiguous(), bias_p.contiguous()
+    d = FewDesc()
+    d.T, d.E, d.k, d.D, d.H, d.O = T, E, k, D, H, O
+    d.dtype, d.weight_dtype, d.renorm = _DTYPE_CODE[x.dtype], FMOE_E4M3 if fp8 else _DTYPE_CODE[x.dtype], int(bool(renorm))
+    d.x, d.x_stride_row = x.data_ptr(), max(x.stride(0), D)
+    d.gate_weight, d.gate_stride_row, d.gate_bias = gate_weight.data_ptr(), max(gate_weight.stride(0), D), _ptr(gate_bias)
+    d.token_mask = _ptr(token_mask)
+    d.w, d.wp, d.w_stride_e, d.w_stride_n = weight.data_ptr(), _ptr(weight_p), weight.stride(0), max(weight.stride(2), D)
+    d.wo, d.wo_stride_e, d.wo_stride_n = weight_out.data_ptr(), weight_out.stride(0), max(weight_out.stride(2), H)
+    d.w_scale, d.wp_scale, d.wo_scale = (_ptr(t) for t in scales)
+    d.bias, d.bias_p = _ptr(bias), _ptr(bias_p)
+    d.bias_stride_e = bias.stride(0) if bias is not None else bias_p.stride(0) if bias_p is not None else 0
+    d.bias_out, d.bias_out_stride_e = _ptr(bias_out), 0 if bias_out is None else bias_out.stride(0)
+    d.out, d.out_stride_row = out.data_ptr(), O
+    lib = _lib.load()
+    ws = torch.empty((lib.fmoe_few_tokens_workspace_bytes(ctypes.byref(d)),), dtype=torch.uint8, device=dev)
+    with _on_device(x):
+        rc = lib.fmoe_few_tokens(ctypes.byref(d), ws.data_ptr(), ws.numel(), _stream(x))
+    _lib.check(rc, "fmoe_few_tokens")
+    return out
+
+
+def _plain_rows(t: torch.Tensor) -> torch.Tensor:
+    """A 2-D t with contiguous rows that do not overlap."""
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()

@@ -234,3 +234,33 @@ def fused_jagged_bmm_swiglu_combine(
     reverse_index = ops.invert_index(index)
     return silu_jagged_bmm_combine(0, offsets, hidden, weight_out, bias_out, token_index, reverse_index,
                                    gates, gates_index, has_silu=False, kernel=kernel)
+
+
+def fused_moe_few_tokens(
+    x: torch.Tensor,
+    gate_weight: torch.Tensor,
+    gate_bias: Optional[torch.Tensor],
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor],
+    weight_p: Optional[torch.Tensor],
+    bias_p: Optional[torch.Tensor],
+    weight_out: torch.Tensor,
+    bias_out: Optional[torch.Tensor],
+    k: int,
+    renorm: bool = True,
+    token_mask: Optional[torch.Tensor] = None,
+    kernel: KernelType = KernelType.HIP,
+) -> torch.Tensor:
+    """A whole MoE layer for up to 64 tokens (a decode step) in two launches, [T, D] -> [T, O]: router
+    ``softmax(x gate_weight^T + gate_bias)``, the ``k`` largest of every token (``renorm``: divided by their sum), and
+    ``sum_j g_j * (act(x W[e_j] + bias[e_j]) W_out[e_j] + bias_out[e_j])`` with ``act(a) = silu(a)``, or
+    ``silu(a) * (x W_p[e_j] + bias_p[e_j])`` when ``weight_p`` is given.
+
+    No counterpart in the reference.  What FastMoELayer.forward and fused_jagged_bmm_swiglu_combine compute, for the batch
+    sizes where the time is that of the launches and of reading the chosen experts' weights; logits are not rounded to
+    the tokens' type here, so that a near tie may fall the other way.  gate_weight is [E, D] (``nn.Linear.weight``), the expert weights
+    [E, D_in, D_out] views of [E, D_out, D_in] storage, everything in x's dtype (bf16 or fp32).  ``token_mask`` (bool [T]):
+    rows where it is False read no expert and come out as zeros (the padding of a captured decode batch).  Forward only."""
+    require_hip_kernel(kernel, "fused_moe_few_tokens")
+    ops._forward_only("fused_moe_few_tokens", x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out)
+    return ops.few_tokens(x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out, k, renorm, token_mask)

@@ -235,3 +235,28 @@ def index_select_jagged_bmm(
     return ops.grouped_gemm(offsets, qa, qw, total_rows=index.numel(), row_index=index,
                             index_div=index.shape[-1], bias=bias, scales_pow2=ops.scales_are_pow2(sa, sw), a_scale=sa,
                             b_scale=sw, epilogue=EPI_NONE)
+
+
+def fused_moe_few_tokens(
+    x: torch.Tensor,
+    gate_weight: torch.Tensor,
+    gate_bias: Optional[torch.Tensor],
+    fp8_weight: Tuple[torch.Tensor, torch.Tensor],
+    bias: Optional[torch.Tensor],
+    fp8_weight_p: Optional[Tuple[torch.Tensor, torch.Tensor]],
+    bias_p: Optional[torch.Tensor],
+    fp8_weight_out: Tuple[torch.Tensor, torch.Tensor],
+    bias_out: Optional[torch.Tensor],
+    k: int,
+    renorm: bool = True,
+    token_mask: Optional[torch.Tensor] = None,
+    kernel: KernelType = KernelType.HIP,
+) -> torch.Tensor:
+    """``kernels.moe.fused_moe_few_tokens`` on e4m3 expert weights: pairs as ``quantize_expert_weights`` returns them, any
+    positive scales.  The tokens (bf16) and the hidden rows are not quantised: a few tokens are bound by reading the
+    weights, which e4m3 halves, and gain nothing from e4m3 products."""
+    require_hip_kernel(kernel, "fused_moe_few_tokens")
+    ops._forward_only("fused_moe_few_tokens", x, gate_weight, gate_bias, bias, bias_p, bias_out)
+    qp, sp = fp8_weight_p if fp8_weight_p is not None else (None, None)
+    return ops.few_tokens(x, gate_weight, gate_bias, fp8_weight[0], bias, qp, bias_p, fp8_weight_out[0], bias_out, k, renorm, token_mask,
+                          (fp8_weight[1], sp, fp8_weight_out[1]))

@@ -156,6 +156,51 @@ typedef struct fmoe_gate {
 } fmoe_gate;
 int fmoe_gate_route_pays(int dtype, int64_t T, int D, int E, int K);
 
+/* ------------------------------------------------- a whole layer, few tokens */
+
+/*
+ * A whole mixture-of-experts layer for up to 64 tokens (a decode step) in two launches: router, the k experts of every token, and
+ * their weighted sum; no counterpart in the reference, which runs the operators one by one (modules/fast_moe_module.py:188-225).
+ *   l[t]    = x[t] . gate_weight^T + gate_bias                     fp32, not rounded
+ *   experts = the k largest of l[t] in descending order (equal ones: the lower id first; NaN counts as the largest),
+ *   g[t, j] = exp(l_j) / sum over the selected (renorm != 0: the L1-normalised softmax) or over all experts
+ *   a       = x[t] . w[e]^T + bias[e],   h = silu(a), or silu(a) * (x[t] . wp[e]^T + bias_p[e]) with wp
+ *   out[t]  = sum_j g[t, j] * (h . wo[e]^T + bias_out[e])          fp32 sums, rounded once
+ * g * h is rounded to dtype in between (bf16: half a step of 2^-8).  A token whose token_mask byte is 0 reads no expert and gets a row of zeros.
+ * dtype (tokens, gate, biases, output): FMOE_BF16 or FMOE_F32; weight_dtype: the same, or FMOE_E4M3 with bf16 tokens, which are not
+ * quantised (products in bf16, divided by the multiplier scales).  k contiguous in every weight.  Rows of whole 16-byte chunks at 16-byte
+ * boundaries are read 16 bytes at a time, others element by element (an order of magnitude slower).  The same inputs give the same bits.
+ */
+typedef struct fmoe_few_desc {
+    int32_t T, E, k;            /* T <= 64, E <= 256, k <= 16                          */
+    int32_t D, H, O;            /* widths of the tokens, the hidden rows, the output   */
+    int32_t dtype, weight_dtype;
+    int32_t renorm;
+    const void* x;              /* [T, D]                                              */
+    int64_t x_stride_row;
+    const void* gate_weight;    /* [E, D]                                              */
+    int64_t gate_stride_row;
+    const void* gate_bias;      /* [E] or NULL                                         */
+    const uint8_t* token_mask;  /* [T] or NULL                                         */
+    const void* w;              /* [E, H, D]                                           */
+    const void* wp;             /* [E, H, D] under w's strides, or NULL                */
+    int64_t w_stride_e, w_stride_n;
+    const void* wo;             /* [E, O, H]                                           */
+    int64_t wo_stride_e, wo_stride_n;
+    const float* w_scale;       /* [E, H] multipliers (FMOE_E4M3)                      */
+    const float* wp_scale;
+    const float* wo_scale;      /* [E, O]                                              */
+    const void* bias;           /* [E, H] rows at bias_stride_e, or NULL               */
+    const void* bias_p;
+    int64_t bias_stride_e;
+    const void* bias_out;       /* [E, O] rows at bias_out_stride_e, or NULL           */
+    int64_t bias_out_stride_e;
+    void* out;                  /* [T, O]                                              */
+    int64_t out_stride_row;
+} fmoe_few_desc;
+size_t fmoe_few_tokens_workspace_bytes(const fmoe_few_desc* desc /* host pointer */);
+int fmoe_few_tokens(const fmoe_few_desc* desc /* host pointer */, void* workspace, size_t workspace_bytes, fmoe_stream_t stream);
+
 /* ---------------------------------------------------------- FP8 quantisation */
 
 /*
