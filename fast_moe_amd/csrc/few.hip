@@ -18,19 +18,14 @@
 namespace fmoe {
 namespace {
 
-constexpr int kFewMostTokens = 64, kFewMostExperts = 256, kFewMostK = 16;
-constexpr int kUpWaves = 8, kDownWaves = 16;
+constexpr int kFewMostTokens = 64, kFewMostExperts = 256, kFewMostK = 16, kFewMostWidth = 1 << 16, kFewMostStride = 1 << 20;
+constexpr int kWaves = 16;             // of a block: one to a CU, so that the router is computed once per CU
 constexpr int kRouterRow = 64 + 4;      // floats of a token's sums over 64 experts (the 4: other banks for the next token)
 
 struct FewParams {
     fmoe_few_desc d;
-    // the workspace: routing as few_up's first block leaves it, and the hidden rows [T * k][H]
-    int32_t* count;         // experts with a token
-    int32_t* act;           // [E] their ids, ascending
-    uint64_t* mask;         // [E] their tokens
-    int32_t* sel;           // [T * k] rank of the expert, -1: none
-    float* gate;            // [T * k]
-    void* h;
+    void* lists;            // who goes where (FewLists)
+    void* h;                // hidden rows [T * k][H]
 };
 
 enum { kWF32 = 0, kWBF16 = 1, kWE4M3 = 2 };
@@ -59,6 +54,21 @@ __device__ __forceinline__ u32x4 chunk(const uint8_t* row, int k, int n) {
     }
     return v;
 }
+// Rows behind a base address that is the same in all lanes, each at a byte offset of its own (below 2^31: few_check).  Whole chunks come through a
+// buffer descriptor: an offset beyond its range reads as zeros, which makes the end of a row one select in the place of a branch around every load.
+template <int ES, bool VEC>
+struct Rows {
+    const uint8_t* base;
+    __amdgpu_buffer_rsrc_t buffer;
+    __device__ __forceinline__ void at(const void* p) {
+        base = (const uint8_t*)p;
+        if constexpr (VEC) buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0x7ffffff0, 0x00027000);
+    }
+    __device__ __forceinline__ u32x4 chunk(uint32_t row, int k, int n) const {
+        if constexpr (VEC) return __builtin_amdgcn_raw_buffer_load_b128(buffer, k < n ? (int)(row + (uint32_t)k * ES) : -1, 0, 0);
+        else return fmoe::chunk<ES, false>(base + row, k, n);
+    }
+};
 
 // Eight e4m3 values as bf16, which holds them exactly.
 __device__ __forceinline__ bf16x8 e4m3_to_bf16(uint32_t lo, uint32_t hi) {
@@ -87,6 +97,9 @@ __device__ __forceinline__ void mma(f32x4& acc, const u32x4& w, const u32x4* x) 
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3_to_bf16(w[2], w[3]), __builtin_bit_cast(bf16x8, x[1]), acc, 0, 0, 0);
     }
 }
+
+// (what the compiler cannot know to be the same in all lanes of a wave)
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 template <bool F32>
 __device__ __forceinline__ float element(const void* p, int64_t i) {
@@ -152,52 +165,54 @@ __device__ __forceinline__ FewLists few_lists(uint8_t* p, int T, int E, int k) {
     l.counts = (int*)take(8);
     return l;
 }
-__host__ __device__ constexpr int few_router_floats() { return kUpWaves * 16 * kRouterRow; }
-__host__ __device__ constexpr int few_up_floats(int mats, int nt) { return kUpWaves * mats * nt * 256; }
+// Sums that meet: of 8 shares of the router, or of 16 waves' two accumulators
+constexpr int kRedBytes = kWaves / 2 * 16 * kRouterRow * 4;
+static_assert(kRedBytes >= kWaves * 2 * kWave * 16, "the waves' accumulators lie in the router's buffer");
 
-// Logits of tokens t0 .. t0 + 15 into LDS [16][E]: 64 experts at a time, the waves share the contraction in pieces of 128 bytes per row
-// (whole cache lines) and their sums are added in wave order.
+// Logits of tokens t0 .. t0 + 15 into LDS [16][E], 64 experts at a time: the waves' halves have 32 each and share the contraction in pieces of
+// 128 bytes per row (whole cache lines); their sums are added in wave order.
 template <bool F32, bool VEC>
 __device__ __forceinline__ void router_logits(const fmoe_few_desc& d, int t0, float* red, float* logits) {
-    constexpr int WT = F32 ? kWF32 : kWBF16, CE = Wt<WT>::CE, ES = Wt<WT>::ES, STEP = 4 * CE, U = 4;
-    const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, quarter = lane >> 4;
+    constexpr int WT = F32 ? kWF32 : kWBF16, CE = Wt<WT>::CE, ES = Wt<WT>::ES, STEP = 4 * CE, U = 4, SHARES = kWaves / 2;
+    const int lane = lane_id(), wave = uniform(threadIdx.x / kWave), share = wave % SHARES, half = wave / SHARES, r16 = lane & 15, quarter = lane >> 4;
     const int t = t0 + r16 < d.T ? t0 + r16 : d.T - 1;
-    const uint8_t* const xrow = (const uint8_t*)d.x + (int64_t)t * d.x_stride_row * ES;
+    const uint32_t xrow = (uint32_t)(t * (int)d.x_stride_row * ES);
+    Rows<ES, VEC> x, g;
+    x.at(d.x);
+    g.at(d.gate_weight);
     const int steps = (d.D + STEP - 1) / STEP;
     for (int e0 = 0; e0 < d.E; e0 += 64) {
-        const int tiles = min(4, (d.E - e0 + 15) / 16);
-        const uint8_t* wrow[4];
+        const int first = e0 + 32 * half, tiles = first < d.E ? min(2, (d.E - first + 15) / 16) : 0;
+        uint32_t wrow[2];
 #pragma unroll
-        for (int f = 0; f < 4; ++f)
-            wrow[f] = (const uint8_t*)d.gate_weight + (int64_t)min(e0 + 16 * f + r16, d.E - 1) * d.gate_stride_row * ES;
-        f32x4 acc[4];
+        for (int f = 0; f < 2; ++f) wrow[f] = (uint32_t)(min(first + 16 * f + r16, d.E - 1) * (int)d.gate_stride_row * ES);
+        f32x4 acc[2];
 #pragma unroll
-        for (int f = 0; f < 4; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s0 = 2 * wave; s0 < steps; s0 += 2 * kUpWaves * (U / 2)) {
-            u32x4 xv[U], wv[U][4];
+        for (int f = 0; f < 2; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s0 = 2 * share; tiles && s0 < steps; s0 += SHARES * U) {
+            u32x4 xv[U], wv[U][2];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int k = (s0 + (u / 2) * 2 * kUpWaves + (u & 1)) * STEP + quarter * CE;
-                xv[u] = chunk<ES, VEC>(xrow, k, d.D);
+                const int k = (s0 + (u / 2) * 2 * SHARES + (u & 1)) * STEP + quarter * CE;
+                xv[u] = x.chunk(xrow, k, d.D);
 #pragma unroll
-                for (int f = 0; f < 4; ++f)
-                    if (f < tiles) wv[u][f] = chunk<ES, VEC>(wrow[f], k, d.D);
+                for (int f = 0; f < 2; ++f) wv[u][f] = g.chunk(wrow[f], k, f < tiles ? d.D : 0);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int f = 0; f < 4; ++f)
-                    if (f < tiles) mma<WT>(acc[f], wv[u][f], &xv[u]);
+                for (int f = 0; f < 2; ++f) mma<WT>(acc[f], wv[u][f], &xv[u]);
         }
 #pragma unroll
-        for (int f = 0; f < 4; ++f) *reinterpret_cast<f32x4*>(red + (wave * 16 + r16) * kRouterRow + 16 * f + 4 * quarter) = acc[f];
+        for (int f = 0; f < 2; ++f)
+            *reinterpret_cast<f32x4*>(red + (share * 16 + r16) * kRouterRow + 32 * half + 16 * f + 4 * quarter) = acc[f];
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * 64; i += kUpWaves * kWave) {
+        for (int i = threadIdx.x; i < 16 * 64; i += kWaves * kWave) {
             const int row = i >> 6, e = e0 + (i & 63);
             if (e < d.E) {
                 float s = red[row * kRouterRow + (i & 63)];
 #pragma unroll
-                for (int w = 1; w < kUpWaves; ++w) s += red[(w * 16 + row) * kRouterRow + (i & 63)];
+                for (int w = 1; w < SHARES; ++w) s += red[(w * 16 + row) * kRouterRow + (i & 63)];
                 if (d.gate_bias) s += element<F32>(d.gate_bias, e);
                 logits[row * d.E + e] = s;
             }
@@ -272,7 +287,7 @@ __device__ __forceinline__ void select_token(const fmoe_few_desc& d, int t, cons
 template <int NT>
 __device__ __forceinline__ void build_lists(const fmoe_few_desc& d, const FewLists& l) {
     const int lane = lane_id();
-    for (int i = threadIdx.x; i < d.T * d.k; i += kUpWaves * kWave)
+    for (int i = threadIdx.x; i < d.T * d.k; i += kWaves * kWave)
         if (l.sel[i] >= 0) atomicOr(&l.mask[l.sel[i]], 1ull << (i / d.k));
     __syncthreads();
     if (threadIdx.x < kWave) {
@@ -299,7 +314,7 @@ __device__ __forceinline__ void build_lists(const fmoe_few_desc& d, const FewLis
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < d.T * d.k; i += kUpWaves * kWave)
+    for (int i = threadIdx.x; i < d.T * d.k; i += kWaves * kWave)
         if (l.sel[i] >= 0) {
             const int e = l.sel[i];
             l.slots[l.base[l.rank[e]] + __popcll(l.mask[e] & ((1ull << (i / d.k)) - 1))] = (int16_t)i;
@@ -308,245 +323,297 @@ __device__ __forceinline__ void build_lists(const fmoe_few_desc& d, const FewLis
 }
 
 template <int WT, bool VEC, int NT, bool GATED>
-__global__ __launch_bounds__(kUpWaves* kWave) __attribute__((amdgpu_waves_per_eu(4))) void few_up_kernel(FewParams p) {
+__global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int share_bits) {
     constexpr bool F32 = WT == kWF32;
     constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, MATS = GATED ? 2 : 1;
-    constexpr int U = NT == 1 ? 4 : 2;      // steps whose loads are in flight
+    constexpr int U = VEC && NT * XC * MATS <= 2 ? 4 : 2;      // steps whose loads are in flight
+    constexpr int ROUND = NT == 1 ? MATS : 1;           // matrices whose sums are in LDS at a time
     extern __shared__ uint8_t lds[];
     const fmoe_few_desc& d = p.d;
-    const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, quarter = lane >> 4;
+    const int lane = lane_id(), wave = uniform(threadIdx.x / kWave), r16 = lane & 15, quarter = lane >> 4;
     float* const red = (float*)lds;
-    constexpr int kRed = (few_router_floats() > few_up_floats(MATS, NT) ? few_router_floats() : few_up_floats(MATS, NT)) * 4;
-    float* const logits = (float*)(lds + kRed);
-    const FewLists l = few_lists(lds + kRed + few_align(16 * d.E * 4), d.T, d.E, d.k);
-    for (int e = threadIdx.x; e < d.E; e += kUpWaves * kWave) l.mask[e] = 0;
+    float* const logits = (float*)(lds + kRedBytes);
+    uint8_t* const listed = lds + kRedBytes + few_align(16 * d.E * 4);
+    const FewLists l = few_lists(listed, d.T, d.E, d.k);
+    for (int e = threadIdx.x; e < d.E; e += kWaves * kWave) l.mask[e] = 0;
     for (int t0 = 0; t0 < d.T; t0 += 16) {
         router_logits<F32, VEC>(d, t0, red, logits);
-        for (int t = wave; t < 16 && t0 + t < d.T; t += kUpWaves) select_token(d, t0 + t, logits + t * d.E, l);
+        for (int t = wave; t < 16 && t0 + t < d.T; t += kWaves) select_token(d, t0 + t, logits + t * d.E, l);
         __syncthreads();
     }
     build_lists<NT>(d, l);
-    const int active = l.counts[0];
-    if (blockIdx.x == 0) {
-        for (int i = threadIdx.x; i < d.T * d.k; i += kUpWaves * kWave) {
-            p.sel[i] = l.sel[i] >= 0 ? l.rank[l.sel[i]] : -1;
-            p.gate[i] = l.gate[i];
-        }
-        for (int a = threadIdx.x; a < active; a += kUpWaves * kWave) {
-            p.act[a] = l.act[a];
-            p.mask[a] = l.mask[l.act[a]];
-        }
-        if (threadIdx.x == 0) *p.count = active;
-    }
-    const int tiles = (d.H + 15) / 16, items = l.counts[1] * tiles, steps = (d.D + STEP - 1) / STEP;
-    for (int it = blockIdx.x; it < items; it += gridDim.x) {
-        const int entry = l.item[it / tiles], a = entry & 0x3fff, first = (entry >> 14) * 16 * NT, h0 = it % tiles * 16;
-        const int e = l.act[a], n = min(16 * NT, (int)__popcll(l.mask[e]) - first);
-        const int16_t* const slots = l.slots + l.base[a] + first;
-        const int row = min(h0 + r16, d.H - 1);
-        const uint8_t* wrow[MATS];
-        wrow[0] = (const uint8_t*)d.w + ((int64_t)e * d.w_stride_e + (int64_t)row * d.w_stride_n) * ES;
-        if constexpr (GATED) wrow[1] = (const uint8_t*)d.wp + ((int64_t)e * d.w_stride_e + (int64_t)row * d.w_stride_n) * ES;
-        const uint8_t* xrow[NT];
-        int xn[NT];
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < few_lists_bytes(d.T, d.E, d.k) / 16; i += kWaves * kWave)
+            reinterpret_cast<u32x4*>(p.lists)[i] = reinterpret_cast<const u32x4*>(listed)[i];
+    // Groups of `shares` waves have an item each and share its contraction in pieces of two steps.
+    const int shares = 1 << share_bits, group = wave >> share_bits, share = wave & (shares - 1), groups = kWaves >> share_bits;
+    const int tiles = (d.H + 15) / 16, items = uniform(l.counts[1]) * tiles, steps = (d.D + STEP - 1) / STEP;
+    struct Item {
+        int e, n, h0;
+        const int16_t* slots;
+    };
+    Item at;
+    Rows<ES, VEC> w[MATS];
+    Rows<XES, VEC> x;
+    x.at(d.x);
+    uint32_t wrow = 0, xrow[NT];
+    bool live[NT];
+    auto take = [&](int it) {
+        const bool any = it < items;
+        const int entry = any ? uniform(l.item[it / tiles]) : 0, a = entry & 0x3fff, first = (entry >> 14) * 16 * NT;
+        at.h0 = any ? it % tiles * 16 : 0;
+        at.e = any ? uniform(l.act[a]) : 0;
+        at.n = any ? uniform(min(16 * NT, (int)__popcll(l.mask[at.e]) - first)) : 0;
+        at.slots = l.slots + (any ? uniform(l.base[a]) + first : 0);
+        const int64_t from = ((int64_t)at.e * d.w_stride_e + (int64_t)at.h0 * d.w_stride_n) * ES;
+        wrow = (uint32_t)(min(r16, d.H - 1 - at.h0) * (int)d.w_stride_n * ES);
+        w[0].at((const uint8_t*)d.w + from);
+        if constexpr (GATED) w[1].at((const uint8_t*)d.wp + from);
 #pragma unroll
         for (int f = 0; f < NT; ++f) {
-            const bool in = 16 * f + r16 < n;
-            xn[f] = in ? d.D : 0;
-            xrow[f] = (const uint8_t*)d.x + (in ? (int64_t)(slots[16 * f + r16] / d.k) * d.x_stride_row * XES : 0);
+            live[f] = 16 * f + r16 < at.n;
+            xrow[f] = live[f] ? (uint32_t)(at.slots[16 * f + r16] / d.k * (int)d.x_stride_row * XES) : 0u;
         }
-        f32x4 acc[MATS][NT];
+    };
+    u32x4 wv[U][MATS], xv[U][NT][XC];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (s0 + (u / 2) * 2 * shares + (u & 1)) * STEP + quarter * CE;
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) wv[u][m] = w[m].chunk(wrow, k, at.n ? d.D : 0);
+#pragma unroll
+            for (int f = 0; f < NT; ++f)
+#pragma unroll
+                for (int c = 0; c < XC; ++c) xv[u][f][c] = x.chunk(xrow[f], k + c * (16 / XES), live[f] ? d.D : 0);
+        }
+    };
+    f32x4 acc[MATS][NT];
+    auto clear = [&] {
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
             for (int f = 0; f < NT; ++f) acc[m][f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s0 = 2 * wave; s0 < steps; s0 += kUpWaves * U) {
-            u32x4 wv[U][MATS], xv[U][NT][XC];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = (s0 + (u / 2) * 2 * kUpWaves + (u & 1)) * STEP + quarter * CE;
-#pragma unroll
-                for (int m = 0; m < MATS; ++m) wv[u][m] = chunk<ES, VEC>(wrow[m], k, d.D);
-#pragma unroll
-                for (int f = 0; f < NT; ++f)
-#pragma unroll
-                    for (int c = 0; c < XC; ++c) xv[u][f][c] = chunk<XES, VEC>(xrow[f], k + c * (16 / XES), xn[f]);
-            }
+    };
+    const int step = gridDim.x * groups;
+    int base = blockIdx.x * groups;         // (the same in all waves: the groups of a block go through the barriers together)
+    take(base + group);
+    load(2 * share);
+    clear();
+    while (base < items) {
+        for (int s0 = 0;;) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int f = 0; f < NT; ++f)
-                    if (f == 0 || 16 * f < n) {
+                    if (f == 0 || 16 * f < at.n) {
 #pragma unroll
                         for (int m = 0; m < MATS; ++m) mma<WT>(acc[m][f], wv[u][m], xv[u][f]);
                     }
+            s0 += U * shares;
+            if (s0 >= steps) break;
+            load(s0 + 2 * share);
+        }
+        // the next item's loads are on their way while this one's sums meet
+        const Item done = at;
+        base += step;
+        if (base < items) {
+            take(base + group);
+            load(2 * share);
+        }
+        f32x4 sum[MATS][NT];
+#pragma unroll
+        for (int m0 = 0; m0 < MATS; m0 += ROUND) {
+            if (m0 > 0) __syncthreads();
+#pragma unroll
+            for (int m = 0; m < ROUND; ++m)
+#pragma unroll
+                for (int f = 0; f < NT; ++f) reinterpret_cast<f32x4*>(red)[((wave * ROUND + m) * NT + f) * kWave + lane] = acc[m0 + m][f];
+            __syncthreads();
+#pragma unroll
+            for (int f = 0; f < NT; ++f)
+                if ((f & (shares - 1)) == share && 16 * f < done.n)
+#pragma unroll
+                    for (int m = 0; m < ROUND; ++m) {
+                        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int w = 0; w < shares; ++w) {
+                            const f32x4 part = reinterpret_cast<f32x4*>(red)[(((group * shares + w) * ROUND + m) * NT + f) * kWave + lane];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] += part[i];
+                        }
+                        sum[m0 + m][f] = v;
+                    }
         }
 #pragma unroll
-        for (int m = 0; m < MATS; ++m)
-#pragma unroll
-            for (int f = 0; f < NT; ++f) reinterpret_cast<f32x4*>(red)[((wave * MATS + m) * NT + f) * kWave + lane] = acc[m][f];
-        __syncthreads();
-        if (wave < NT && 16 * wave + r16 < n) {
-            f32x4 sum[MATS];
-#pragma unroll
-            for (int m = 0; m < MATS; ++m) {
-                sum[m] = reinterpret_cast<f32x4*>(red)[(m * NT + wave) * kWave + lane];
-#pragma unroll
-                for (int w = 1; w < kUpWaves; ++w) {
-                    const f32x4 v = reinterpret_cast<f32x4*>(red)[((w * MATS + m) * NT + wave) * kWave + lane];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[m][i] += v[i];
-                }
-            }
-            const int slot = slots[16 * wave + r16];
+        for (int f = 0; f < NT; ++f) {
+            if ((f & (shares - 1)) != share || 16 * f + r16 >= done.n) continue;
+            const int slot = done.slots[16 * f + r16];
             const float g = l.gate[slot];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int col = h0 + 4 * quarter + i;
+                const int col = done.h0 + 4 * quarter + i;
                 if (col >= d.H) break;
-                float v = sum[0][i];
-                if constexpr (WT == kWE4M3) v /= d.w_scale[(int64_t)e * d.H + col];
-                if (d.bias) v += element<F32>(d.bias, (int64_t)e * d.bias_stride_e + col);
+                float v = sum[0][f][i];
+                if constexpr (WT == kWE4M3) v /= d.w_scale[(int64_t)done.e * d.H + col];
+                if (d.bias) v += element<F32>(d.bias, (int64_t)done.e * d.bias_stride_e + col);
                 v = silu_f32(v);
                 if constexpr (GATED) {
-                    float u = sum[1][i];
-                    if constexpr (WT == kWE4M3) u /= d.wp_scale[(int64_t)e * d.H + col];
-                    if (d.bias_p) u += element<F32>(d.bias_p, (int64_t)e * d.bias_stride_e + col);
+                    float u = sum[1][f][i];
+                    if constexpr (WT == kWE4M3) u /= d.wp_scale[(int64_t)done.e * d.H + col];
+                    if (d.bias_p) u += element<F32>(d.bias_p, (int64_t)done.e * d.bias_stride_e + col);
                     v *= u;
                 }
                 // bf16: the one rounding between the two products, of the gated value (half a step of bf16, as of the layer's own hidden rows)
                 put_element<F32>(p.h, (int64_t)slot * d.H + col, g * v);
             }
         }
+        clear();
         __syncthreads();
     }
 }
 
-template <int WT, bool VEC, int NT>
-__global__ __launch_bounds__(kDownWaves* kWave) void few_down_kernel(FewParams p) {
+// PARTS: a tile has 16 / PARTS output columns, and the MFMAs' rows (and columns: up to 16 / PARTS tokens) hold that many stretches of the
+// contraction side by side, of whose products the diagonal blocks count: more, smaller tiles where 16 columns each would leave CUs without one.
+template <int WT, bool VEC, int NT, int PARTS>
+__global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
     constexpr bool F32 = WT == kWF32;
-    constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, U = NT == 4 ? 2 : 4;
+    constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, U = VEC && NT * XC <= 2 ? 4 : 2, COLS = 16 / PARTS;
     extern __shared__ uint8_t lds[];
     const fmoe_few_desc& d = p.d;
-    const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, quarter = lane >> 4;
-    f32x4* const red = (f32x4*)lds;                                 // [waves][lanes]
-    int16_t* const slot_of = (int16_t*)(lds + kDownWaves * kWave * 16);        // [active][16 * NT] slot of a token at an expert, -1: none
-    const int active = *p.count;
-    for (int i = threadIdx.x; i < active * 16 * NT; i += kDownWaves * kWave) slot_of[i] = -1;
+    const int lane = lane_id(), wave = threadIdx.x / kWave, waves = blockDim.x / kWave, r16 = lane & 15, quarter = lane >> 4;
+    float* const sums = (float*)lds;                                        // [waves][T][16]
+    uint8_t* const listed = lds + (size_t)waves * d.T * 64;
+    const FewLists l = few_lists(listed, d.T, d.E, d.k);
+    for (int i = threadIdx.x; i < few_lists_bytes(d.T, d.E, d.k) / 16; i += blockDim.x)
+        reinterpret_cast<u32x4*>(listed)[i] = reinterpret_cast<const u32x4*>(p.lists)[i];
+    for (int i = threadIdx.x; i < waves * d.T * 4; i += blockDim.x) reinterpret_cast<f32x4*>(sums)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     __syncthreads();
-    for (int i = threadIdx.x; i < d.T * d.k; i += kDownWaves * kWave) {
-        const int a = p.sel[i];
-        if (a >= 0) slot_of[a * 16 * NT + i / d.k] = (int16_t)i;
-    }
-    __syncthreads();
-    const int n0 = blockIdx.x * 16, row = min(n0 + r16, d.O - 1);
-    const int steps = (d.H + STEP - 1) / STEP, pieces = (steps + 1) / 2, total = active * pieces;
-    f32x4 acc[NT];
-#pragma unroll
-    for (int f = 0; f < NT; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int q0 = wave; q0 < total; q0 += kDownWaves * (U / 2)) {
-        u32x4 wv[U], xv[U][NT][XC];
-        uint64_t mask[U / 2];
-        f32x4 inv[U / 2];
+    const int part = r16 / COLS, n0 = blockIdx.x * COLS, row = min(n0 + r16 % COLS, d.O - 1);
+    const int steps = (d.H + STEP - 1) / STEP, pieces = (steps + 1) / 2, total = l.counts[1] * pieces;
+    // every stretch (a wave's, or a part of its) takes as many pieces of two steps, experts after one another
+    const int per = (total + waves * PARTS - 1) / (waves * PARTS), from = (wave * PARTS + part) * per;
+    const int until = min(total, from + per);
+    struct Entry {
+        int index, e, n;
+        const int16_t* slots;
+    };
+    auto entry_of = [&](int index) {
+        const int item = l.item[index], a = item & 0x3fff, first = (item >> 14) * 16 * NT;
+        Entry en;
+        en.index = index;
+        en.e = l.act[a];
+        en.n = min(16 * NT, (int)__popcll(l.mask[en.e]) - first);
+        en.slots = l.slots + l.base[a] + first;
+        return en;
+    };
+    Entry next = {-1, 0, 0, l.slots}, cur = next;       // the expert whose loads are on their way, and whose products add up
+    int next_of[U / 2];
+    const uint8_t *wrow = nullptr, *xrow[NT] = {};
+    u32x4 wv[U], xv[U][NT][XC];
+    int q = from, index = total ? from / pieces : 0, piece = from - index * pieces;
+    auto load = [&] {
 #pragma unroll
         for (int u = 0; u < U / 2; ++u) {
-            const int q = q0 + u * kDownWaves;
-            mask[u] = 0;
-            if (q >= total) continue;
-            const int a = q / pieces, piece = q - a * pieces;
-            const int e = p.act[a];
-            mask[u] = p.mask[a];
-            const uint8_t* const wrow = (const uint8_t*)d.wo + ((int64_t)e * d.wo_stride_e + (int64_t)row * d.wo_stride_n) * ES;
-            if constexpr (WT == kWE4M3) {
+            const bool any = q < until;
+            next_of[u] = any ? index : next.index;
+            if (any && index != next.index) {
+                next = entry_of(index);
+                wrow = (const uint8_t*)d.wo + ((int64_t)next.e * d.wo_stride_e + (int64_t)row * d.wo_stride_n) * ES;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) inv[u][i] = 1.0f / d.wo_scale[(int64_t)e * d.O + min(n0 + 4 * quarter + i, d.O - 1)];
+                for (int f = 0; f < NT; ++f) {
+                    const int c = 16 * f + r16 % COLS;
+                    xrow[f] = c < next.n ? (const uint8_t*)p.h + (int64_t)next.slots[c] * d.H * XES : nullptr;
+                }
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const int k = (2 * piece + s) * STEP + quarter * CE;
-                wv[2 * u + s] = chunk<ES, VEC>(wrow, k, d.H);
+                wv[2 * u + s] = chunk<ES, VEC>(wrow, k, any ? d.H : 0);
 #pragma unroll
-                for (int f = 0; f < NT; ++f) {
-                    const int slot = slot_of[a * 16 * NT + 16 * f + r16];
-                    const uint8_t* const hrow = (const uint8_t*)p.h + (slot < 0 ? 0 : (int64_t)slot * d.H * XES);
+                for (int f = 0; f < NT; ++f)
 #pragma unroll
-                    for (int c = 0; c < XC; ++c) xv[2 * u + s][f][c] = chunk<XES, VEC>(hrow, k + c * (16 / XES), slot < 0 ? 0 : d.H);
-                }
+                    for (int c = 0; c < XC; ++c) xv[2 * u + s][f][c] = chunk<XES, VEC>(xrow[f], k + c * (16 / XES), any && xrow[f] ? d.H : 0);
+            }
+            ++q;
+            if (++piece == pieces) {
+                piece = 0;
+                ++index;
             }
         }
+    };
+    f32x4 acc[NT];
 #pragma unroll
-        for (int u = 0; u < U / 2; ++u)
+    for (int f = 0; f < NT; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // An expert's products go to its own tokens' sums, and only there (a column without a token holds zeros, which an infinity among the weights
+    // turns into NaN).
+    auto flush = [&] {
+        if (cur.index >= 0) {
+            f32x4 inv = {1.0f, 1.0f, 1.0f, 1.0f};
+            if constexpr (WT == kWE4M3) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) inv[i] = 1.0f / d.wo_scale[(int64_t)cur.e * d.O + min(n0 + (4 * quarter + i) % COLS, d.O - 1)];
+            }
 #pragma unroll
             for (int f = 0; f < NT; ++f) {
-                const uint32_t here = (uint32_t)(mask[u] >> (16 * f)) & 0xffff;
-                if (!here) continue;
-                f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma<WT>(part, wv[2 * u], xv[2 * u][f]);
-                mma<WT>(part, wv[2 * u + 1], xv[2 * u + 1][f]);
-                // (a token that is not the expert's has zeros in its column, which an infinity among the weights would make a NaN)
-                const bool routed = here >> r16 & 1;
+                const int c = 16 * f + r16 % COLS;
+                if (c < cur.n && quarter * 4 / COLS == part) {
+                    f32x4* const to = reinterpret_cast<f32x4*>(sums + ((size_t)wave * d.T + cur.slots[c] / d.k) * 16 + 4 * quarter);
+                    f32x4 v = *to;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (WT == kWE4M3) part[i] *= inv[u][i];
-                    acc[f][i] += routed ? part[i] : 0.0f;
+                    for (int i = 0; i < 4; ++i) v[i] += acc[f][i] * inv[i];
+                    *to = v;
                 }
-            }
-    }
-#pragma unroll
-    for (int f = 0; f < NT; ++f) {
-        if (f > 0) __syncthreads();
-        red[wave * kWave + lane] = acc[f];
-        __syncthreads();
-        const int t = 16 * f + r16;
-        if (wave == 0 && t < d.T) {
-            f32x4 sum = red[lane];
-#pragma unroll
-            for (int w = 1; w < kDownWaves; ++w) {
-                const f32x4 v = red[w * kWave + lane];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += v[i];
-            }
-            if (d.bias_out)
-                for (int j = 0; j < d.k; ++j) {
-                    const int a = p.sel[t * d.k + j];
-                    if (a < 0) continue;
-                    const float g = p.gate[t * d.k + j];
-                    for (int i = 0; i < 4; ++i) {
-                        const int col = n0 + 4 * quarter + i;
-                        if (col < d.O) sum[i] += g * element<F32>(d.bias_out, (int64_t)p.act[a] * d.bias_out_stride_e + col);
-                    }
-                }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int col = n0 + 4 * quarter + i;
-                if (col < d.O) put_element<F32>(d.out, (int64_t)t * d.out_stride_row + col, sum[i]);
             }
         }
+#pragma unroll
+        for (int f = 0; f < NT; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    load();
+    for (int done = 0; done < per; done += U / 2) {
+#pragma unroll
+        for (int u = 0; u < U / 2; ++u) {
+            if (__any(next_of[u] != cur.index)) {
+                flush();
+                if (next_of[u] >= 0) cur = entry_of(next_of[u]);
+            }
+#pragma unroll
+            for (int f = 0; f < NT; ++f)
+                if (f == 0 || 16 * f < cur.n) {
+                    mma<WT>(acc[f], wv[2 * u], xv[2 * u][f]);
+                    mma<WT>(acc[f], wv[2 * u + 1], xv[2 * u + 1][f]);
+                }
+        }
+        if (done + U / 2 < per) load();
+    }
+    flush();
+    __syncthreads();
+    for (int i = threadIdx.x; i < d.T * COLS; i += blockDim.x) {
+        const int t = i / COLS, c = i % COLS, col = n0 + c;
+        if (col >= d.O) continue;
+        float v = 0.0f;
+        for (int w = 0; w < waves; ++w)
+#pragma unroll
+            for (int q2 = 0; q2 < PARTS; ++q2) v += sums[((size_t)w * d.T + t) * 16 + q2 * COLS + c];
+        if (d.bias_out)
+            for (int j = 0; j < d.k; ++j) {
+                const int e = l.sel[t * d.k + j];
+                if (e >= 0) v += l.gate[t * d.k + j] * element<F32>(d.bias_out, (int64_t)e * d.bias_out_stride_e + col);
+            }
+        put_element<F32>(d.out, (int64_t)t * d.out_stride_row + col, v);
     }
 }
 
-struct FewLayout {
-    size_t act, mask, sel, gate, h, end;
-};
-FewLayout few_layout(const fmoe_few_desc& d) {
-    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    FewLayout l;
-    l.mask = 256;                                                   // (the count first)
-    l.act = up(l.mask + (size_t)d.E * 8);
-    l.sel = up(l.act + (size_t)d.E * 4);
-    l.gate = up(l.sel + (size_t)d.T * d.k * 4);
-    l.h = up(l.gate + (size_t)d.T * d.k * 4);
-    l.end = up(l.h + (size_t)d.T * d.k * d.H * (d.dtype == FMOE_F32 ? 4 : 2));
-    return l;
-}
+// The workspace: the lists as few_up's first block leaves them, and the hidden rows.
+size_t few_hidden_at(const fmoe_few_desc& d) { return ((size_t)few_lists_bytes(d.T, d.E, d.k) + 255) & ~(size_t)255; }
+size_t few_bytes(const fmoe_few_desc& d) { return few_hidden_at(d) + (size_t)d.T * d.k * d.H * (d.dtype == FMOE_F32 ? 4 : 2); }
 
 int few_check(const fmoe_few_desc* d) {
     FMOE_REQUIRE(d, "fmoe_few_tokens: desc is NULL");
     FMOE_REQUIRE(d->T >= 0 && d->T <= kFewMostTokens, "fmoe_few_tokens: up to %d tokens, got T=%d", kFewMostTokens, d->T);
     FMOE_REQUIRE(d->E >= 1 && d->E <= kFewMostExperts && d->k >= 1 && d->k <= kFewMostK && d->k <= d->E,
                  "fmoe_few_tokens: need 1 <= k <= E, k <= %d, E <= %d, got k=%d E=%d", kFewMostK, kFewMostExperts, d->k, d->E);
-    FMOE_REQUIRE(d->D >= 1 && d->H >= 1 && d->O >= 1 && d->D <= (1 << 24) && d->H <= (1 << 24) && d->O <= (1 << 24),
-                 "fmoe_few_tokens: widths of 1 to 2^24 expected");
+    FMOE_REQUIRE(d->D >= 1 && d->H >= 1 && d->O >= 1 && d->D <= kFewMostWidth && d->H <= kFewMostWidth && d->O <= kFewMostWidth,
+                 "fmoe_few_tokens: widths of 1 to %d expected", kFewMostWidth);
     FMOE_REQUIRE(d->dtype == FMOE_F32 || d->dtype == FMOE_BF16, "fmoe_few_tokens: tokens must be bf16 or fp32");
     FMOE_REQUIRE(d->weight_dtype == d->dtype || (d->weight_dtype == FMOE_E4M3 && d->dtype == FMOE_BF16),
                  "fmoe_few_tokens: weights must have the tokens' type, or be e4m3 with bf16 tokens");
@@ -557,6 +624,10 @@ int few_check(const fmoe_few_desc* d) {
     FMOE_REQUIRE(d->x_stride_row >= (d->T > 1 ? d->D : 0) && d->gate_stride_row >= (d->E > 1 ? d->D : 0) && d->out_stride_row >= (d->T > 1 ? d->O : 0) &&
                      d->w_stride_n >= (d->H > 1 ? d->D : 0) && d->wo_stride_n >= (d->O > 1 ? d->H : 0) && d->w_stride_e >= 0 && d->wo_stride_e >= 0,
                  "fmoe_few_tokens: rows overlap");
+    // (offsets of rows from their tile's first are 31 bits of bytes)
+    FMOE_REQUIRE(d->x_stride_row <= kFewMostStride && d->gate_stride_row <= kFewMostStride && d->w_stride_n <= kFewMostStride &&
+                     d->wo_stride_n <= kFewMostStride,
+                 "fmoe_few_tokens: row strides of up to %d elements expected", kFewMostStride);
     return FMOE_OK;
 }
 
@@ -567,19 +638,18 @@ using namespace fmoe;
 
 extern "C" size_t fmoe_few_tokens_workspace_bytes(const fmoe_few_desc* d) {
     if (few_check(d) != FMOE_OK || d->T == 0) return 0;
-    return few_layout(*d).end;
+    return few_bytes(*d);
 }
 
 extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_t workspace_bytes, fmoe_stream_t stream_) {
     const int rc = few_check(desc);
     if (rc != FMOE_OK || desc->T == 0) return rc;
     const fmoe_few_desc& d = *desc;
-    const FewLayout at = few_layout(d);
-    if (!workspace || workspace_bytes < at.end)
-        return fail(FMOE_ERR_WORKSPACE, "fmoe_few_tokens: workspace of %zu bytes, %zu needed", workspace_bytes, at.end);
+    const size_t need = few_bytes(d);
+    if (!workspace || workspace_bytes < need)
+        return fail(FMOE_ERR_WORKSPACE, "fmoe_few_tokens: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     FMOE_REQUIRE(aligned16(workspace), "fmoe_few_tokens: the workspace must be 16-byte aligned");
-    uint8_t* const ws = (uint8_t*)workspace;
-    FewParams p{d, (int32_t*)ws, (int32_t*)(ws + at.act), (uint64_t*)(ws + at.mask), (int32_t*)(ws + at.sel), (float*)(ws + at.gate), ws + at.h};
+    const FewParams p{d, workspace, (uint8_t*)workspace + few_hidden_at(d)};
     const int es = d.dtype == FMOE_F32 ? 4 : 2, wes = d.weight_dtype == FMOE_E4M3 ? 1 : es;
     // whole 16-byte chunks at 16-byte boundaries wherever rows are read
     auto whole = [](const void* q, int64_t elements, int size) { return aligned16(q) && elements * size % 16 == 0; };
@@ -589,24 +659,29 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     const bool gated = d.wp != nullptr;
     const int most_active = d.T * d.k < d.E ? d.T * d.k : d.E;
     hipStream_t stream = (hipStream_t)stream_;
-    auto up = [&](auto kern, int mats, int nt) {
-        const int floats = few_router_floats() > few_up_floats(mats, nt) ? few_router_floats() : few_up_floats(mats, nt);
-        const int64_t items = (int64_t)most_active * ((d.H + 15) / 16) * (nt == 2 && d.T > 32 ? 2 : 1);
-        const unsigned grid = (unsigned)(items < 512 ? items : 512);
-        kern<<<grid, kUpWaves * kWave, floats * 4 + few_align(16 * d.E * 4) + few_lists_bytes(d.T, d.E, d.k), stream>>>(p);
+    const int lists = few_lists_bytes(d.T, d.E, d.k), step = wes == 1 ? 64 : 64 / wes;
+    // waves to an item: four steps each where the rows are that long
+    int share_bits = 0;
+    while (share_bits < 4 && (4 << share_bits) * step < d.D) ++share_bits;
+    auto up = [&](auto kern, int nt) {
+        const int64_t items = (int64_t)most_active * ((d.H + 15) / 16) * (nt == 2 && d.T > 32 ? 2 : 1), blocks = (items + (kWaves >> share_bits) - 1) / (kWaves >> share_bits);
+        kern<<<(unsigned)(blocks < 256 ? blocks : 256), kWaves * kWave, kRedBytes + few_align(16 * d.E * 4) + lists, stream>>>(p, share_bits);
     };
-    auto down = [&](auto kern, int nt) {
-        kern<<<(unsigned)((d.O + 15) / 16), kDownWaves * kWave, kDownWaves * kWave * 16 + few_align(most_active * 16 * nt * 2), stream>>>(p);
+    auto down = [&](auto kern, int parts) {
+        const int cols = 16 / parts, waves = d.T > 32 ? kWaves / 2 : kWaves;        // (their sums for 64 tokens in 64 KB of LDS)
+        kern<<<(unsigned)((d.O + cols - 1) / cols), waves * kWave, waves * d.T * 64 + lists, stream>>>(p);
     };
-#define FMOE_FEW_UP(WT, VEC, NT) (gated ? up(few_up_kernel<WT, VEC, NT, true>, 2, NT) : up(few_up_kernel<WT, VEC, NT, false>, 1, NT))
+    const int parts = d.O >= 16 * 256 || d.T > 8 ? 1 : d.O >= 8 * 256 || d.T > 4 ? 2 : 4;
+#define FMOE_FEW_UP(WT, VEC, NT) (gated ? up(few_up_kernel<WT, VEC, NT, true>, NT) : up(few_up_kernel<WT, VEC, NT, false>, NT))
 #define FMOE_FEW(WT, VEC)                                                   \
     do {                                                                    \
         if (d.T <= 16) FMOE_FEW_UP(WT, VEC, 1); else FMOE_FEW_UP(WT, VEC, 2); \
         const int launched = check_launch("fmoe_few_tokens");               \
         if (launched != FMOE_OK) return launched;                           \
-        if (d.T <= 16) down(few_down_kernel<WT, VEC, 1>, 1);                \
-        else if (d.T <= 32) down(few_down_kernel<WT, VEC, 2>, 2);           \
-        else down(few_down_kernel<WT, VEC, 4>, 4);                          \
+        if (d.T > 16) down(few_down_kernel<WT, VEC, 2, 1>, 1);              \
+        else if (parts == 1) down(few_down_kernel<WT, VEC, 1, 1>, 1);       \
+        else if (parts == 2) down(few_down_kernel<WT, VEC, 1, 2>, 2);       \
+        else down(few_down_kernel<WT, VEC, 1, 4>, 4);                       \
     } while (0)
     if (d.weight_dtype == FMOE_F32) {
         if (vec) FMOE_FEW(kWF32, true); else FMOE_FEW(kWF32, false);
