@@ -20,12 +20,15 @@ namespace {
 
 constexpr int kFewMostTokens = 64, kFewMostExperts = 256, kFewMostK = 16, kFewMostWidth = 1 << 16, kFewMostStride = 1 << 20;
 constexpr int kWaves = 16;             // of a block: one to a CU, so that the router is computed once per CU
+constexpr int kLogitWaves = 8;
 constexpr int kRouterRow = 64 + 4;      // floats of a token's sums over 64 experts (the 4: other banks for the next token)
 
 struct FewParams {
     fmoe_few_desc d;
     void* lists;            // who goes where (FewLists)
     void* h;                // hidden rows [T * k][H]
+    const float* logits;    // [stretches][T][E]
+    int stretches;          // of the router's own launch, 0: the router is few_up's
 };
 
 enum { kWF32 = 0, kWBF16 = 1, kWE4M3 = 2 };
@@ -221,8 +224,47 @@ __device__ __forceinline__ void router_logits(const fmoe_few_desc& d, int t0, fl
     }
 }
 
-// The k experts of one token by one wave: descending logit, equal ones by ascending id.
-__device__ __forceinline__ void select_token(const fmoe_few_desc& d, int t, const float* logits, const FewLists& l) {
+// The router in a launch of its own: 16 experts and 16 tokens a block, a stretch of the contraction (blockIdx.z), sums [stretch][T][E].
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(kLogitWaves* kWave) void few_logits_kernel(fmoe_few_desc d, float* part) {
+    constexpr int WT = F32 ? kWF32 : kWBF16, CE = Wt<WT>::CE, ES = Wt<WT>::ES, STEP = 4 * CE, U = 4;
+    __shared__ f32x4 red[kLogitWaves][kWave];
+    const int lane = lane_id(), wave = uniform(threadIdx.x / kWave), r16 = lane & 15, quarter = lane >> 4, e0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
+    const int steps = (d.D + STEP - 1) / STEP, all = kLogitWaves * gridDim.z, share = blockIdx.z * kLogitWaves + wave;
+    const uint32_t xrow = (uint32_t)(min(t0 + r16, d.T - 1) * (int)d.x_stride_row * ES), wrow = (uint32_t)(min(e0 + r16, d.E - 1) * (int)d.gate_stride_row * ES);
+    Rows<ES, VEC> x, g;
+    x.at(d.x);
+    g.at(d.gate_weight);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 2 * share; s0 < steps; s0 += U * all) {
+        u32x4 xv[U], wv[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (s0 + (u / 2) * 2 * all + (u & 1)) * STEP + quarter * CE;
+            xv[u] = x.chunk(xrow, k, d.D);
+            wv[u] = g.chunk(wrow, k, d.D);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) mma<WT>(acc, wv[u], &xv[u]);
+    }
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && t0 + r16 < d.T) {
+#pragma unroll
+        for (int w = 1; w < kLogitWaves; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] += red[w][lane][i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = e0 + 4 * quarter + i;
+            if (e < d.E) part[((int64_t)blockIdx.z * d.T + t0 + r16) * d.E + e] = acc[i] + (d.gate_bias && blockIdx.z == 0 ? element<F32>(d.gate_bias, e) : 0.0f);
+        }
+    }
+}
+
+// The k experts of one token by one wave, from its logits: descending, equal ones by ascending id.
+template <typename Logit>
+__device__ __forceinline__ void select_token(const fmoe_few_desc& d, int t, Logit&& logit, const FewLists& l) {
     const int lane = lane_id();
     if (d.token_mask && !d.token_mask[t]) {
         if (lane < d.k) {
@@ -237,7 +279,7 @@ __device__ __forceinline__ void select_token(const fmoe_few_desc& d, int t, cons
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int e = i * kWave + lane;
-        v[i] = e < d.E ? logits[e] : 0.0f;
+        v[i] = e < d.E ? logit(e) : 0.0f;
         key[i] = e < d.E ? order_key(v[i]) : 0u;
     }
     float top = 0.0f, mine = -__builtin_inff();
@@ -326,20 +368,31 @@ template <int WT, bool VEC, int NT, bool GATED>
 __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int share_bits) {
     constexpr bool F32 = WT == kWF32;
     constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, MATS = GATED ? 2 : 1;
-    constexpr int U = VEC && NT * XC * MATS <= 2 ? 4 : 2;      // steps whose loads are in flight
+    constexpr int AHEAD = !VEC || NT * XC * MATS > 2 ? 2 : 3;    // batches of loads in flight
     constexpr int ROUND = NT == 1 ? MATS : 1;           // matrices whose sums are in LDS at a time
     extern __shared__ uint8_t lds[];
     const fmoe_few_desc& d = p.d;
     const int lane = lane_id(), wave = uniform(threadIdx.x / kWave), r16 = lane & 15, quarter = lane >> 4;
     float* const red = (float*)lds;
     float* const logits = (float*)(lds + kRedBytes);
-    uint8_t* const listed = lds + kRedBytes + few_align(16 * d.E * 4);
+    uint8_t* const listed = lds + kRedBytes + (p.stretches ? 0 : few_align(16 * d.E * 4));
     const FewLists l = few_lists(listed, d.T, d.E, d.k);
     for (int e = threadIdx.x; e < d.E; e += kWaves * kWave) l.mask[e] = 0;
-    for (int t0 = 0; t0 < d.T; t0 += 16) {
-        router_logits<F32, VEC>(d, t0, red, logits);
-        for (int t = wave; t < 16 && t0 + t < d.T; t += kWaves) select_token(d, t0 + t, logits + t * d.E, l);
+    if (p.stretches) {          // few_logits has run
         __syncthreads();
+        for (int t = wave; t < d.T; t += kWaves)
+            select_token(d, t, [&](int e) {
+                float v = p.logits[(int64_t)t * d.E + e];
+                for (int z = 1; z < p.stretches; ++z) v += p.logits[((int64_t)z * d.T + t) * d.E + e];
+                return v;
+            }, l);
+        __syncthreads();
+    } else {
+        for (int t0 = 0; t0 < d.T; t0 += 16) {
+            router_logits<F32, VEC>(d, t0, red, logits);
+            for (int t = wave; t < 16 && t0 + t < d.T; t += kWaves) select_token(d, t0 + t, [&](int e) { return logits[t * d.E + e]; }, l);
+            __syncthreads();
+        }
     }
     build_lists<NT>(d, l);
     if (blockIdx.x == 0)
@@ -348,44 +401,61 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
     // Groups of `shares` waves have an item each and share its contraction in pieces of two steps.
     const int shares = 1 << share_bits, group = wave >> share_bits, share = wave & (shares - 1), groups = kWaves >> share_bits;
     const int tiles = (d.H + 15) / 16, items = uniform(l.counts[1]) * tiles, steps = (d.D + STEP - 1) / STEP;
+    const int batches = (steps + 2 * shares - 1) / (2 * shares);       // of two steps a wave
     struct Item {
         int e, n, h0;
         const int16_t* slots;
     };
-    Item at;
+    auto item = [&](int it) {
+        Item at = {0, 0, 0, l.slots};
+        if (it < items) {
+            const int entry = uniform(l.item[it / tiles]), a = entry & 0x3fff, first = (entry >> 14) * 16 * NT;
+            at.h0 = it % tiles * 16;
+            at.e = uniform(l.act[a]);
+            at.n = uniform(min(16 * NT, (int)__popcll(l.mask[at.e]) - first));
+            at.slots = l.slots + uniform(l.base[a]) + first;
+        }
+        return at;
+    };
+    const int step = gridDim.x * groups;
+    int base = blockIdx.x * groups;         // (the same in all waves: the groups of a block go through the barriers together)
+    // What is loaded runs AHEAD batches before what is multiplied, over the ends of items.
     Rows<ES, VEC> w[MATS];
     Rows<XES, VEC> x;
     x.at(d.x);
     uint32_t wrow = 0, xrow[NT];
-    bool live[NT];
-    auto take = [&](int it) {
-        const bool any = it < items;
-        const int entry = any ? uniform(l.item[it / tiles]) : 0, a = entry & 0x3fff, first = (entry >> 14) * 16 * NT;
-        at.h0 = any ? it % tiles * 16 : 0;
-        at.e = any ? uniform(l.act[a]) : 0;
-        at.n = any ? uniform(min(16 * NT, (int)__popcll(l.mask[at.e]) - first)) : 0;
-        at.slots = l.slots + (any ? uniform(l.base[a]) + first : 0);
+    int wcols = 0, xcols[NT], load_it = base + group, load_s = 0;
+    auto take = [&] {
+        const Item at = item(load_it);
         const int64_t from = ((int64_t)at.e * d.w_stride_e + (int64_t)at.h0 * d.w_stride_n) * ES;
         wrow = (uint32_t)(min(r16, d.H - 1 - at.h0) * (int)d.w_stride_n * ES);
+        wcols = at.n ? d.D : 0;
         w[0].at((const uint8_t*)d.w + from);
         if constexpr (GATED) w[1].at((const uint8_t*)d.wp + from);
 #pragma unroll
         for (int f = 0; f < NT; ++f) {
-            live[f] = 16 * f + r16 < at.n;
-            xrow[f] = live[f] ? (uint32_t)(at.slots[16 * f + r16] / d.k * (int)d.x_stride_row * XES) : 0u;
+            const bool live = 16 * f + r16 < at.n;
+            xrow[f] = live ? (uint32_t)(at.slots[16 * f + r16] / d.k * (int)d.x_stride_row * XES) : 0u;
+            xcols[f] = live ? d.D : 0;
         }
     };
-    u32x4 wv[U][MATS], xv[U][NT][XC];
-    auto load = [&](int s0) {
+    u32x4 wv[AHEAD][2][MATS], xv[AHEAD][2][NT][XC];
+    auto load = [&](u32x4 (&wb)[2][MATS], u32x4 (&xb)[2][NT][XC]) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = (s0 + (u / 2) * 2 * shares + (u & 1)) * STEP + quarter * CE;
+        for (int u = 0; u < 2; ++u) {
+            const int k = (load_s + 2 * share + u) * STEP + quarter * CE;
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) wv[u][m] = w[m].chunk(wrow, k, at.n ? d.D : 0);
+            for (int m = 0; m < MATS; ++m) wb[u][m] = w[m].chunk(wrow, k, wcols);
 #pragma unroll
             for (int f = 0; f < NT; ++f)
 #pragma unroll
-                for (int c = 0; c < XC; ++c) xv[u][f][c] = x.chunk(xrow[f], k + c * (16 / XES), live[f] ? d.D : 0);
+                for (int c = 0; c < XC; ++c) xb[u][f][c] = x.chunk(xrow[f], k + c * (16 / XES), xcols[f]);
+        }
+        load_s += 2 * shares;
+        if (load_s >= steps) {
+            load_s = 0;
+            load_it += step;
+            take();
         }
     };
     f32x4 acc[MATS][NT];
@@ -395,32 +465,12 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 #pragma unroll
             for (int f = 0; f < NT; ++f) acc[m][f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     };
-    const int step = gridDim.x * groups;
-    int base = blockIdx.x * groups;         // (the same in all waves: the groups of a block go through the barriers together)
-    take(base + group);
-    load(2 * share);
+    take();
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) load(wv[i], xv[i]);
     clear();
-    while (base < items) {
-        for (int s0 = 0;;) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int f = 0; f < NT; ++f)
-                    if (f == 0 || 16 * f < at.n) {
-#pragma unroll
-                        for (int m = 0; m < MATS; ++m) mma<WT>(acc[m][f], wv[u][m], xv[u][f]);
-                    }
-            s0 += U * shares;
-            if (s0 >= steps) break;
-            load(s0 + 2 * share);
-        }
-        // the next item's loads are on their way while this one's sums meet
-        const Item done = at;
-        base += step;
-        if (base < items) {
-            take(base + group);
-            load(2 * share);
-        }
+    Item done = item(base + group);
+    auto finish = [&] {
         f32x4 sum[MATS][NT];
 #pragma unroll
         for (int m0 = 0; m0 < MATS; m0 += ROUND) {
@@ -468,7 +518,28 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
             }
         }
         clear();
+        base += step;
+        done = item(base + group);
         __syncthreads();
+    };
+    for (int left = batches; base < items;) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (base >= items) break;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int f = 0; f < NT; ++f)
+                    if (f == 0 || 16 * f < done.n) {
+#pragma unroll
+                        for (int m = 0; m < MATS; ++m) mma<WT>(acc[m][f], wv[i][u][m], xv[i][u][f]);
+                    }
+            load(wv[i], xv[i]);
+            if (--left == 0) {
+                finish();
+                left = batches;
+            }
+        }
     }
 }
 
@@ -477,7 +548,8 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 template <int WT, bool VEC, int NT, int PARTS>
 __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
     constexpr bool F32 = WT == kWF32;
-    constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, U = VEC && NT * XC <= 2 ? 4 : 2, COLS = 16 / PARTS;
+    constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, COLS = 16 / PARTS;
+    constexpr int AHEAD = !VEC ? 1 : NT * XC == 1 ? 4 : NT * XC == 2 ? 3 : 2;      // pieces whose loads are in flight
     extern __shared__ uint8_t lds[];
     const fmoe_few_desc& d = p.d;
     const int lane = lane_id(), wave = threadIdx.x / kWave, waves = blockDim.x / kWave, r16 = lane & 15, quarter = lane >> 4;
@@ -507,38 +579,35 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
         return en;
     };
     Entry next = {-1, 0, 0, l.slots}, cur = next;       // the expert whose loads are on their way, and whose products add up
-    int next_of[U / 2];
+    int next_of[AHEAD];
     const uint8_t *wrow = nullptr, *xrow[NT] = {};
-    u32x4 wv[U], xv[U][NT][XC];
+    u32x4 wv[AHEAD][2], xv[AHEAD][2][NT][XC];
     int q = from, index = total ? from / pieces : 0, piece = from - index * pieces;
-    auto load = [&] {
+    auto load = [&](int& of, u32x4 (&wb)[2], u32x4 (&xb)[2][NT][XC]) {
+        const bool any = q < until;
+        of = any ? index : next.index;
+        if (any && index != next.index) {
+            next = entry_of(index);
+            wrow = (const uint8_t*)d.wo + ((int64_t)next.e * d.wo_stride_e + (int64_t)row * d.wo_stride_n) * ES;
 #pragma unroll
-        for (int u = 0; u < U / 2; ++u) {
-            const bool any = q < until;
-            next_of[u] = any ? index : next.index;
-            if (any && index != next.index) {
-                next = entry_of(index);
-                wrow = (const uint8_t*)d.wo + ((int64_t)next.e * d.wo_stride_e + (int64_t)row * d.wo_stride_n) * ES;
-#pragma unroll
-                for (int f = 0; f < NT; ++f) {
-                    const int c = 16 * f + r16 % COLS;
-                    xrow[f] = c < next.n ? (const uint8_t*)p.h + (int64_t)next.slots[c] * d.H * XES : nullptr;
-                }
+            for (int f = 0; f < NT; ++f) {
+                const int c = 16 * f + r16 % COLS;
+                xrow[f] = c < next.n ? (const uint8_t*)p.h + (int64_t)next.slots[c] * d.H * XES : nullptr;
             }
+        }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int k = (2 * piece + s) * STEP + quarter * CE;
-                wv[2 * u + s] = chunk<ES, VEC>(wrow, k, any ? d.H : 0);
+        for (int s = 0; s < 2; ++s) {
+            const int k = (2 * piece + s) * STEP + quarter * CE;
+            wb[s] = chunk<ES, VEC>(wrow, k, any ? d.H : 0);
 #pragma unroll
-                for (int f = 0; f < NT; ++f)
+            for (int f = 0; f < NT; ++f)
 #pragma unroll
-                    for (int c = 0; c < XC; ++c) xv[2 * u + s][f][c] = chunk<XES, VEC>(xrow[f], k + c * (16 / XES), any && xrow[f] ? d.H : 0);
-            }
-            ++q;
-            if (++piece == pieces) {
-                piece = 0;
-                ++index;
-            }
+                for (int c = 0; c < XC; ++c) xb[s][f][c] = chunk<XES, VEC>(xrow[f], k + c * (16 / XES), any && xrow[f] ? d.H : 0);
+        }
+        ++q;
+        if (++piece == pieces) {
+            piece = 0;
+            ++index;
         }
     };
     f32x4 acc[NT];
@@ -568,22 +637,23 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
 #pragma unroll
         for (int f = 0; f < NT; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     };
-    load();
-    for (int done = 0; done < per; done += U / 2) {
 #pragma unroll
-        for (int u = 0; u < U / 2; ++u) {
-            if (__any(next_of[u] != cur.index)) {
+    for (int i = 0; i < AHEAD; ++i) load(next_of[i], wv[i], xv[i]);
+    for (int done = 0; done < per; done += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {       // (behind a stretch's last piece come zeros)
+            if (__any(next_of[i] != cur.index)) {
                 flush();
-                if (next_of[u] >= 0) cur = entry_of(next_of[u]);
+                if (next_of[i] >= 0) cur = entry_of(next_of[i]);
             }
 #pragma unroll
             for (int f = 0; f < NT; ++f)
                 if (f == 0 || 16 * f < cur.n) {
-                    mma<WT>(acc[f], wv[2 * u], xv[2 * u][f]);
-                    mma<WT>(acc[f], wv[2 * u + 1], xv[2 * u + 1][f]);
+                    mma<WT>(acc[f], wv[i][0], xv[i][0][f]);
+                    mma<WT>(acc[f], wv[i][1], xv[i][1][f]);
                 }
+            load(next_of[i], wv[i], xv[i]);
         }
-        if (done + U / 2 < per) load();
     }
     flush();
     __syncthreads();
@@ -605,7 +675,13 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
 
 // The workspace: the lists as few_up's first block leaves them, and the hidden rows.
 size_t few_hidden_at(const fmoe_few_desc& d) { return ((size_t)few_lists_bytes(d.T, d.E, d.k) + 255) & ~(size_t)255; }
-size_t few_bytes(const fmoe_few_desc& d) { return few_hidden_at(d) + (size_t)d.T * d.k * d.H * (d.dtype == FMOE_F32 ? 4 : 2); }
+size_t few_logits_at(const fmoe_few_desc& d) { return (few_hidden_at(d) + (size_t)d.T * d.k * d.H * (d.dtype == FMOE_F32 ? 4 : 2) + 255) & ~(size_t)255; }
+// Stretches of the router's own launch, 0 where few_up computes the router.
+int few_stretches(const fmoe_few_desc& d) {
+    if ((int64_t)d.E * d.D * (d.dtype == FMOE_F32 ? 4 : 2) * ((d.T + 15) / 16) <= 32 * 1024) return 0;
+    return d.T <= 16 ? 4 : 1;
+}
+size_t few_bytes(const fmoe_few_desc& d) { return few_logits_at(d) + (size_t)few_stretches(d) * d.T * d.E * 4; }
 
 int few_check(const fmoe_few_desc* d) {
     FMOE_REQUIRE(d, "fmoe_few_tokens: desc is NULL");
@@ -649,7 +725,7 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     if (!workspace || workspace_bytes < need)
         return fail(FMOE_ERR_WORKSPACE, "fmoe_few_tokens: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     FMOE_REQUIRE(aligned16(workspace), "fmoe_few_tokens: the workspace must be 16-byte aligned");
-    const FewParams p{d, workspace, (uint8_t*)workspace + few_hidden_at(d)};
+    const FewParams p{d, workspace, (uint8_t*)workspace + few_hidden_at(d), (const float*)((uint8_t*)workspace + few_logits_at(d)), few_stretches(d)};
     const int es = d.dtype == FMOE_F32 ? 4 : 2, wes = d.weight_dtype == FMOE_E4M3 ? 1 : es;
     // whole 16-byte chunks at 16-byte boundaries wherever rows are read
     auto whole = [](const void* q, int64_t elements, int size) { return aligned16(q) && elements * size % 16 == 0; };
@@ -665,7 +741,7 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     while (share_bits < 4 && (4 << share_bits) * step < d.D) ++share_bits;
     auto up = [&](auto kern, int nt) {
         const int64_t items = (int64_t)most_active * ((d.H + 15) / 16) * (nt == 2 && d.T > 32 ? 2 : 1), blocks = (items + (kWaves >> share_bits) - 1) / (kWaves >> share_bits);
-        kern<<<(unsigned)(blocks < 256 ? blocks : 256), kWaves * kWave, kRedBytes + few_align(16 * d.E * 4) + lists, stream>>>(p, share_bits);
+        kern<<<(unsigned)(blocks < 256 ? blocks : 256), kWaves * kWave, kRedBytes + (p.stretches ? 0 : few_align(16 * d.E * 4)) + lists, stream>>>(p, share_bits);
     };
     auto down = [&](auto kern, int parts) {
         const int cols = 16 / parts, waves = d.T > 32 ? kWaves / 2 : kWaves;        // (their sums for 64 tokens in 64 KB of LDS)
@@ -675,6 +751,11 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
 #define FMOE_FEW_UP(WT, VEC, NT) (gated ? up(few_up_kernel<WT, VEC, NT, true>, NT) : up(few_up_kernel<WT, VEC, NT, false>, NT))
 #define FMOE_FEW(WT, VEC)                                                   \
     do {                                                                    \
+        if (p.stretches) {                                                  \
+            few_logits_kernel<WT == kWF32, VEC><<<dim3((d.E + 15) / 16, (d.T + 15) / 16, p.stretches), kLogitWaves * kWave, 0, stream>>>(d, const_cast<float*>(p.logits)); \
+            const int first = check_launch("fmoe_few_tokens");              \
+            if (first != FMOE_OK) return first;                             \
+        }                                                                   \
         if (d.T <= 16) FMOE_FEW_UP(WT, VEC, 1); else FMOE_FEW_UP(WT, VEC, 2); \
         const int launched = check_launch("fmoe_few_tokens");               \
         if (launched != FMOE_OK) return launched;                           \
