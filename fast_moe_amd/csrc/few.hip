@@ -29,6 +29,9 @@ struct FewParams {
     void* h;                // hidden rows [T * k][H]
     const float* logits;    // [stretches][T][E]
     int stretches;          // of the router's own launch, 0: the router is few_up's
+    int tiles;              // of few_down that several blocks share, or 0
+    int32_t* arrivals;      // [tiles of few_down] blocks of a tile that have left their sums
+    float* partial;
 };
 
 enum { kWF32 = 0, kWBF16 = 1, kWE4M3 = 2 };
@@ -78,10 +81,9 @@ __device__ __forceinline__ bf16x8 e4m3_to_bf16(uint32_t lo, uint32_t hi) {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int w = (int)(i ? hi : lo);
-        const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-        r[2 * i] = cvt_pk_bf16(a[0], a[1]);
-        r[2 * i + 1] = cvt_pk_bf16(b[0], b[1]);
+        const uint32_t w = i ? hi : lo;
+        r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+        r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
     }
     return __builtin_bit_cast(bf16x8, r);
 }
@@ -135,20 +137,18 @@ __device__ __forceinline__ uint32_t order_key(float f) {
     return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
-struct FewLists {           // in LDS
-    int16_t* sel;           // [T * k] expert, -1: none
-    float* gate;            // [T * k]
+struct FewLists {           // in LDS, and as few_up's first block leaves them in the workspace
     unsigned long long* mask;   // [E] tokens
-    int16_t* rank;          // [E]
-    int16_t* act;           // [E]
-    int16_t* base;          // [E + 1] first of an active expert's slots
+    uint2* entry;           // [2 E] an expert and up to 16 * NT tokens of its: x = id | tokens << 16, y = first of their slots
+    float* gate;            // [T * k]
+    int16_t* sel;           // [T * k] expert, -1: none
     int16_t* slots;         // [T * k] t * k + j, by expert and token
-    int16_t* item;          // [2 E] active expert | 0x4000 for its tokens 32 .. 63 (16 .. where NT = 1: cannot be)
-    int* counts;            // [2] active experts, items
+    int16_t* first;         // [E] first of an expert's slots
+    int* entries;           // how many
 };
 __host__ __device__ constexpr int few_align(int bytes) { return (bytes + 15) & ~15; }
 __host__ __device__ inline int few_lists_bytes(int T, int E, int k) {
-    return 2 * few_align(T * k * 2) + few_align(T * k * 4) + few_align(E * 8) + 2 * few_align(E * 2) + few_align(E * 2 + 2) + few_align(E * 4) + 16;
+    return few_align(E * 8) + E * 16 + few_align(T * k * 4) + 2 * few_align(T * k * 2) + few_align(E * 2) + 16;
 }
 __device__ __forceinline__ FewLists few_lists(uint8_t* p, int T, int E, int k) {
     FewLists l;
@@ -158,19 +158,27 @@ __device__ __forceinline__ FewLists few_lists(uint8_t* p, int T, int E, int k) {
         return at;
     };
     l.mask = (unsigned long long*)take(E * 8);
+    l.entry = (uint2*)take(E * 16);
     l.gate = (float*)take(T * k * 4);
     l.sel = (int16_t*)take(T * k * 2);
     l.slots = (int16_t*)take(T * k * 2);
-    l.rank = (int16_t*)take(E * 2);
-    l.act = (int16_t*)take(E * 2);
-    l.base = (int16_t*)take(E * 2 + 2);
-    l.item = (int16_t*)take(E * 4);
-    l.counts = (int*)take(8);
+    l.first = (int16_t*)take(E * 2);
+    l.entries = (int*)take(16);
     return l;
 }
-// Sums that meet: of 8 shares of the router, or of 16 waves' two accumulators
-constexpr int kRedBytes = kWaves / 2 * 16 * kRouterRow * 4;
-static_assert(kRedBytes >= kWaves * 2 * kWave * 16, "the waves' accumulators lie in the router's buffer");
+// One of the entries, the same in all lanes (PARTS > 1 of few_down: in a part of them).
+struct Entry {
+    int e, n, first;
+};
+template <bool UNIFORM>
+__device__ __forceinline__ Entry few_entry(const FewLists& l, int i) {
+    const uint2 v = l.entry[i];
+    const int x = UNIFORM ? uniform((int)v.x) : (int)v.x, y = UNIFORM ? uniform((int)v.y) : (int)v.y;
+    return Entry{x & 0xffff, x >> 16, y};
+}
+// Sums that meet: two buffers of the 16 waves' two accumulators, or 8 shares of the router
+constexpr int kRedFloats = kWaves * 2 * kWave * 4, kRedBytes = 2 * kRedFloats * 4;
+static_assert(kRedBytes >= kWaves / 2 * 16 * kRouterRow * 4, "the router's sums lie in the same buffers");
 
 // Logits of tokens t0 .. t0 + 15 into LDS [16][E], 64 experts at a time: the waves' halves have 32 each and share the contraction in pieces of
 // 128 bytes per row (whole cache lines); their sums are added in wave order.
@@ -263,8 +271,8 @@ __global__ __launch_bounds__(kLogitWaves* kWave) void few_logits_kernel(fmoe_few
 }
 
 // The k experts of one token by one wave, from its logits: descending, equal ones by ascending id.
-template <typename Logit>
-__device__ __forceinline__ void select_token(const fmoe_few_desc& d, int t, Logit&& logit, const FewLists& l) {
+template <int R, typename Logit>
+__device__ __forceinline__ void select_token_of(const fmoe_few_desc& d, int t, Logit&& logit, const FewLists& l) {
     const int lane = lane_id();
     if (d.token_mask && !d.token_mask[t]) {
         if (lane < d.k) {
@@ -273,7 +281,6 @@ __device__ __forceinline__ void select_token(const fmoe_few_desc& d, int t, Logi
         }
         return;
     }
-    constexpr int R = kFewMostExperts / kWave;
     float v[R];
     uint32_t key[R];
 #pragma unroll
@@ -325,7 +332,15 @@ __device__ __forceinline__ void select_token(const fmoe_few_desc& d, int t, Logi
     }
 }
 
-// Who goes where, from every token's selection: per expert its tokens, the experts that have any, and the items (an expert, up to 16 * NT tokens).
+template <typename Logit>
+__device__ __forceinline__ void select_token(const fmoe_few_desc& d, int t, Logit&& logit, const FewLists& l) {
+    static_assert(kFewMostExperts == 4 * kWave, "a lane holds up to four experts");
+    if (d.E <= kWave) select_token_of<1>(d, t, logit, l);
+    else if (d.E <= 2 * kWave) select_token_of<2>(d, t, logit, l);
+    else select_token_of<4>(d, t, logit, l);
+}
+
+// Who goes where, from every token's selection.
 template <int NT>
 __device__ __forceinline__ void build_lists(const fmoe_few_desc& d, const FewLists& l) {
     const int lane = lane_id();
@@ -333,33 +348,26 @@ __device__ __forceinline__ void build_lists(const fmoe_few_desc& d, const FewLis
         if (l.sel[i] >= 0) atomicOr(&l.mask[l.sel[i]], 1ull << (i / d.k));
     __syncthreads();
     if (threadIdx.x < kWave) {
-        int active = 0, rows = 0, items = 0;
+        int sofar = 0;          // rows in the low half, entries in the high one
         for (int e0 = 0; e0 < d.E; e0 += kWave) {
             const int e = e0 + lane;
             const int n = e < d.E ? __popcll(l.mask[e]) : 0, groups = (n + 16 * NT - 1) / (16 * NT);
-            const unsigned long long any = __ballot(n > 0);
-            const int a = active + __popcll(any & ((1ull << lane) - 1));
-            const int upto = wave_inclusive_scan(n), item = wave_inclusive_scan(groups);
+            const int upto = sofar + wave_inclusive_scan(n | groups << 16);
             if (n > 0) {
-                l.rank[e] = (int16_t)a;
-                l.act[a] = (int16_t)e;
-                l.base[a] = (int16_t)(rows + upto - n);
-                for (int i = 0; i < groups; ++i) l.item[items + item - groups + i] = (int16_t)(a | i << 14);
+                const int first = (upto & 0xffff) - n, at = (upto >> 16) - groups;
+                l.first[e] = (int16_t)first;
+                for (int i = 0; i < groups; ++i)
+                    l.entry[at + i] = uint2{(uint32_t)(e | min(16 * NT, n - i * 16 * NT) << 16), (uint32_t)(first + i * 16 * NT)};
             }
-            active += __popcll(any);
-            rows += __shfl(upto, kWave - 1, kWave);
-            items += __shfl(item, kWave - 1, kWave);
+            sofar = __builtin_amdgcn_readlane(upto, kWave - 1);
         }
-        if (lane == 0) {
-            l.counts[0] = active;
-            l.counts[1] = items;
-        }
+        if (lane == 0) *l.entries = sofar >> 16;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < d.T * d.k; i += kWaves * kWave)
         if (l.sel[i] >= 0) {
             const int e = l.sel[i];
-            l.slots[l.base[l.rank[e]] + __popcll(l.mask[e] & ((1ull << (i / d.k)) - 1))] = (int16_t)i;
+            l.slots[l.first[e] + __popcll(l.mask[e] & ((1ull << (i / d.k)) - 1))] = (int16_t)i;
         }
     __syncthreads();
 }
@@ -396,65 +404,71 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
     }
     build_lists<NT>(d, l);
     if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < p.tiles; i += kWaves * kWave) p.arrivals[i] = 0;
+    if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < few_lists_bytes(d.T, d.E, d.k) / 16; i += kWaves * kWave)
             reinterpret_cast<u32x4*>(p.lists)[i] = reinterpret_cast<const u32x4*>(listed)[i];
     // Groups of `shares` waves have an item each and share its contraction in pieces of two steps.
     const int shares = 1 << share_bits, group = wave >> share_bits, share = wave & (shares - 1), groups = kWaves >> share_bits;
-    const int tiles = (d.H + 15) / 16, items = uniform(l.counts[1]) * tiles, steps = (d.D + STEP - 1) / STEP;
+    const int tiles = (d.H + 15) / 16, entries = uniform(*l.entries), steps = (d.D + STEP - 1) / STEP;
     const int batches = (steps + 2 * shares - 1) / (2 * shares);       // of two steps a wave
+    // An item is an entry's tile of 16 hidden columns; a group takes every `stride`th.  The groups of a block go through the barriers
+    // together, those behind the last item with nothing to do.
+    const int stride = gridDim.x * groups, over = stride / tiles, rest = stride - over * tiles;
     struct Item {
-        int e, n, h0;
-        const int16_t* slots;
+        int entry, tile;
     };
-    auto item = [&](int it) {
-        Item at = {0, 0, 0, l.slots};
-        if (it < items) {
-            const int entry = uniform(l.item[it / tiles]), a = entry & 0x3fff, first = (entry >> 14) * 16 * NT;
-            at.h0 = it % tiles * 16;
-            at.e = uniform(l.act[a]);
-            at.n = uniform(min(16 * NT, (int)__popcll(l.mask[at.e]) - first));
-            at.slots = l.slots + uniform(l.base[a]) + first;
+    auto step = [&](Item& it) {
+        it.entry += over;
+        it.tile += rest;
+        if (it.tile >= tiles) {
+            it.tile -= tiles;
+            ++it.entry;
         }
-        return at;
     };
-    const int step = gridDim.x * groups;
-    int base = blockIdx.x * groups;         // (the same in all waves: the groups of a block go through the barriers together)
+    const int start = blockIdx.x * groups;
+    Item loading = {(start + group) / tiles, (start + group) % tiles}, adding = loading;
+    const int total = entries * tiles, rounds = start < total ? (total - start + stride - 1) / stride : 0;
     // What is loaded runs AHEAD batches before what is multiplied, over the ends of items.
     Rows<ES, VEC> w[MATS];
     Rows<XES, VEC> x;
     x.at(d.x);
     uint32_t wrow = 0, xrow[NT];
-    int wcols = 0, xcols[NT], load_it = base + group, load_s = 0;
+    int wcols = 0, xcols[NT], load_s = 0;
     auto take = [&] {
-        const Item at = item(load_it);
-        const int64_t from = ((int64_t)at.e * d.w_stride_e + (int64_t)at.h0 * d.w_stride_n) * ES;
-        wrow = (uint32_t)(min(r16, d.H - 1 - at.h0) * (int)d.w_stride_n * ES);
-        wcols = at.n ? d.D : 0;
+        const bool any = loading.entry < entries;
+        const Entry at = any ? few_entry<true>(l, loading.entry) : Entry{0, 0, 0};
+        const int h0 = any ? 16 * loading.tile : 0;
+        const int64_t from = ((int64_t)at.e * d.w_stride_e + (int64_t)h0 * d.w_stride_n) * ES;
+        wrow = (uint32_t)(min(r16, d.H - 1 - h0) * (int)d.w_stride_n * ES);
+        wcols = any ? d.D : 0;
         w[0].at((const uint8_t*)d.w + from);
         if constexpr (GATED) w[1].at((const uint8_t*)d.wp + from);
 #pragma unroll
         for (int f = 0; f < NT; ++f) {
             const bool live = 16 * f + r16 < at.n;
-            xrow[f] = live ? (uint32_t)(at.slots[16 * f + r16] / d.k * (int)d.x_stride_row * XES) : 0u;
+            xrow[f] = live ? (uint32_t)(l.slots[at.first + 16 * f + r16] / d.k * (int)d.x_stride_row * XES) : 0u;
             xcols[f] = live ? d.D : 0;
         }
     };
     u32x4 wv[AHEAD][2][MATS], xv[AHEAD][2][NT][XC];
     auto load = [&](u32x4 (&wb)[2][MATS], u32x4 (&xb)[2][NT][XC]) {
+        // (the two halves of a row's 128-byte line behind one another, so that the L1 asks the L2 for the line once)
+        const int k = (load_s + 2 * share) * STEP + quarter * CE;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int k = (load_s + 2 * share + u) * STEP + quarter * CE;
+        for (int m = 0; m < MATS; ++m)
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) wb[u][m] = w[m].chunk(wrow, k, wcols);
+            for (int u = 0; u < 2; ++u) wb[u][m] = w[m].chunk(wrow, k + u * STEP, wcols);
 #pragma unroll
-            for (int f = 0; f < NT; ++f)
+        for (int f = 0; f < NT; ++f)
 #pragma unroll
-                for (int c = 0; c < XC; ++c) xb[u][f][c] = x.chunk(xrow[f], k + c * (16 / XES), xcols[f]);
-        }
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int c = 0; c < XC; ++c) xb[u][f][c] = x.chunk(xrow[f], k + u * STEP + c * (16 / XES), xcols[f]);
         load_s += 2 * shares;
         if (load_s >= steps) {
             load_s = 0;
-            load_it += step;
+            step(loading);
             take();
         }
     };
@@ -469,25 +483,47 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) load(wv[i], xv[i]);
     clear();
-    Item done = item(base + group);
-    auto finish = [&] {
+    int turn = 0, n = NT > 1 && adding.entry < entries ? few_entry<true>(l, adding.entry).n : 0;
+    // One wave of a group adds up, another one each time; the others go on to the next item at once (the buffers take turns, so that it has read one
+    // before that is written again: in between is a barrier that it has to reach).
+    auto finish = [&](int round) {
+        bool mine[NT], any = false;
+#pragma unroll
+        for (int f = 0; f < NT; ++f) {
+            mine[f] = ((round * NT + f) & (shares - 1)) == share && adding.entry < entries;
+            any |= mine[f];
+        }
+        const Entry at = any ? few_entry<true>(l, adding.entry) : Entry{0, 0, 0};
+        const int h0 = 16 * adding.tile, col0 = h0 + 4 * quarter;
+        // (asked for before the barrier)
+        float bias[MATS][4], div[MATS][4];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const void* const b = m ? d.bias_p : d.bias;
+                const int col = min(col0 + i, d.H - 1);
+                bias[m][i] = any && b ? element<F32>(b, (int64_t)at.e * d.bias_stride_e + col) : 0.0f;
+                if constexpr (WT == kWE4M3) div[m][i] = any ? (m ? d.wp_scale : d.w_scale)[(int64_t)at.e * d.H + col] : 1.0f;
+            }
         f32x4 sum[MATS][NT];
 #pragma unroll
         for (int m0 = 0; m0 < MATS; m0 += ROUND) {
-            if (m0 > 0) __syncthreads();
+            f32x4* const buf = reinterpret_cast<f32x4*>(red + turn * kRedFloats);
+            turn ^= 1;
 #pragma unroll
             for (int m = 0; m < ROUND; ++m)
 #pragma unroll
-                for (int f = 0; f < NT; ++f) reinterpret_cast<f32x4*>(red)[((wave * ROUND + m) * NT + f) * kWave + lane] = acc[m0 + m][f];
+                for (int f = 0; f < NT; ++f) buf[((wave * ROUND + m) * NT + f) * kWave + lane] = acc[m0 + m][f];
             __syncthreads();
 #pragma unroll
             for (int f = 0; f < NT; ++f)
-                if ((f & (shares - 1)) == share && 16 * f < done.n)
+                if (mine[f])
 #pragma unroll
                     for (int m = 0; m < ROUND; ++m) {
                         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
                         for (int w = 0; w < shares; ++w) {
-                            const f32x4 part = reinterpret_cast<f32x4*>(red)[(((group * shares + w) * ROUND + m) * NT + f) * kWave + lane];
+                            const f32x4 part = buf[(((group * shares + w) * ROUND + m) * NT + f) * kWave + lane];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) v[i] += part[i];
                         }
@@ -496,47 +532,53 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
         }
 #pragma unroll
         for (int f = 0; f < NT; ++f) {
-            if ((f & (shares - 1)) != share || 16 * f + r16 >= done.n) continue;
-            const int slot = done.slots[16 * f + r16];
+            if (!mine[f] || 16 * f + r16 >= at.n) continue;
+            const int slot = l.slots[at.first + 16 * f + r16];
             const float g = l.gate[slot];
+            float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int col = done.h0 + 4 * quarter + i;
-                if (col >= d.H) break;
-                float v = sum[0][f][i];
-                if constexpr (WT == kWE4M3) v /= d.w_scale[(int64_t)done.e * d.H + col];
-                if (d.bias) v += element<F32>(d.bias, (int64_t)done.e * d.bias_stride_e + col);
-                v = silu_f32(v);
+                float a = sum[0][f][i];
+                if constexpr (WT == kWE4M3) a /= div[0][i];
+                v[i] = silu_f32(a + bias[0][i]);
                 if constexpr (GATED) {
                     float u = sum[1][f][i];
-                    if constexpr (WT == kWE4M3) u /= d.wp_scale[(int64_t)done.e * d.H + col];
-                    if (d.bias_p) u += element<F32>(d.bias_p, (int64_t)done.e * d.bias_stride_e + col);
-                    v *= u;
+                    if constexpr (WT == kWE4M3) u /= div[1][i];
+                    v[i] *= u + bias[1][i];
                 }
-                // bf16: the one rounding between the two products, of the gated value (half a step of bf16, as of the layer's own hidden rows)
-                put_element<F32>(p.h, (int64_t)slot * d.H + col, g * v);
+                v[i] *= g;
+            }
+            // bf16: the one rounding between the two products, of the gated value (half a step of bf16, as of the layer's own hidden rows)
+            const int64_t to = (int64_t)slot * d.H + col0;
+            if (VEC && col0 + 4 <= d.H) {
+                if constexpr (F32) *reinterpret_cast<f32x4*>((float*)p.h + to) = f32x4{v[0], v[1], v[2], v[3]};
+                else *reinterpret_cast<u32x2*>((uint16_t*)p.h + to) = u32x2{cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col0 + i < d.H) put_element<F32>(p.h, to + i, v[i]);
             }
         }
         clear();
-        base += step;
-        done = item(base + group);
-        __syncthreads();
+        step(adding);
+        if constexpr (NT > 1) n = adding.entry < entries ? few_entry<true>(l, adding.entry).n : 0;
     };
-    for (int left = batches; base < items;) {
+    for (int round = 0, left = batches; round < rounds;) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            if (base >= items) break;
+            if (round >= rounds) break;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int f = 0; f < NT; ++f)
-                    if (f == 0 || 16 * f < done.n) {
+                    if (f == 0 || 16 * f < n) {
 #pragma unroll
                         for (int m = 0; m < MATS; ++m) mma<WT>(acc[m][f], wv[i][u][m], xv[i][u][f]);
                     }
             load(wv[i], xv[i]);
             if (--left == 0) {
-                finish();
+                finish(round);
+                ++round;
                 left = batches;
             }
         }
@@ -545,14 +587,15 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 
 // PARTS: a tile has 16 / PARTS output columns, and the MFMAs' rows (and columns: up to 16 / PARTS tokens) hold that many stretches of the
 // contraction side by side, of whose products the diagonal blocks count: more, smaller tiles where 16 columns each would leave CUs without one.
+// gridDim.y > 1: so many blocks share a tile's contraction; their sums go through memory, and the one that arrives last adds them in block order.
 template <int WT, bool VEC, int NT, int PARTS>
 __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
-    constexpr bool F32 = WT == kWF32;
+    constexpr bool F32 = WT == kWF32, ONE = PARTS == 1;
     constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, COLS = 16 / PARTS;
     constexpr int AHEAD = !VEC ? 1 : NT * XC == 1 ? 4 : NT * XC == 2 ? 3 : 2;      // pieces whose loads are in flight
     extern __shared__ uint8_t lds[];
     const fmoe_few_desc& d = p.d;
-    const int lane = lane_id(), wave = threadIdx.x / kWave, waves = blockDim.x / kWave, r16 = lane & 15, quarter = lane >> 4;
+    const int lane = lane_id(), wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave, r16 = lane & 15, quarter = lane >> 4;
     float* const sums = (float*)lds;                                        // [waves][T][16]
     uint8_t* const listed = lds + (size_t)waves * d.T * 64;
     const FewLists l = few_lists(listed, d.T, d.E, d.k);
@@ -560,76 +603,75 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
         reinterpret_cast<u32x4*>(listed)[i] = reinterpret_cast<const u32x4*>(p.lists)[i];
     for (int i = threadIdx.x; i < waves * d.T * 4; i += blockDim.x) reinterpret_cast<f32x4*>(sums)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     __syncthreads();
-    const int part = r16 / COLS, n0 = blockIdx.x * COLS, row = min(n0 + r16 % COLS, d.O - 1);
-    const int steps = (d.H + STEP - 1) / STEP, pieces = (steps + 1) / 2, total = l.counts[1] * pieces;
-    // every stretch (a wave's, or a part of its) takes as many pieces of two steps, experts after one another
-    const int per = (total + waves * PARTS - 1) / (waves * PARTS), from = (wave * PARTS + part) * per;
-    const int until = min(total, from + per);
-    struct Entry {
-        int index, e, n;
-        const int16_t* slots;
-    };
-    auto entry_of = [&](int index) {
-        const int item = l.item[index], a = item & 0x3fff, first = (item >> 14) * 16 * NT;
-        Entry en;
-        en.index = index;
-        en.e = l.act[a];
-        en.n = min(16 * NT, (int)__popcll(l.mask[en.e]) - first);
-        en.slots = l.slots + l.base[a] + first;
-        return en;
-    };
-    Entry next = {-1, 0, 0, l.slots}, cur = next;       // the expert whose loads are on their way, and whose products add up
-    int next_of[AHEAD];
+    const int part = ONE ? 0 : r16 / COLS, n0 = blockIdx.x * COLS, row = min(n0 + r16 % COLS, d.O - 1);
+    const int steps = (d.H + STEP - 1) / STEP, pieces = (steps + 1) / 2, total = uniform(*l.entries) * pieces;
+    // every stretch (a wave's, or a part of its) takes as many pieces of two steps, entries after one another
+    const int stretches = waves * PARTS * gridDim.y, per = (total + stretches - 1) / stretches;
+    const int from = ((blockIdx.y * waves + wave) * PARTS + part) * per, until = min(total, from + per);
+    Entry next = {0, 0, 0}, cur = {0, 0, 0};            // whose loads are on their way, and whose products add up
+    int next_index = -1, cur_index = -1, of[AHEAD];
     const uint8_t *wrow = nullptr, *xrow[NT] = {};
+    Rows<ES, VEC> w;
+    Rows<XES, VEC> x;
+    uint32_t xoff[NT] = {};
+    w.at(d.wo);
+    x.at(p.h);
+    const uint32_t woff = (uint32_t)((row - n0) * (int)d.wo_stride_n * ES);
     u32x4 wv[AHEAD][2], xv[AHEAD][2][NT][XC];
     int q = from, index = total ? from / pieces : 0, piece = from - index * pieces;
     auto load = [&](int& of, u32x4 (&wb)[2], u32x4 (&xb)[2][NT][XC]) {
         const bool any = q < until;
-        of = any ? index : next.index;
-        if (any && index != next.index) {
-            next = entry_of(index);
-            wrow = (const uint8_t*)d.wo + ((int64_t)next.e * d.wo_stride_e + (int64_t)row * d.wo_stride_n) * ES;
+        of = any ? index : next_index;
+        if (any && index != next_index) {
+            next = few_entry<ONE>(l, index);
+            next_index = index;
+            if constexpr (ONE) w.at((const uint8_t*)d.wo + ((int64_t)next.e * d.wo_stride_e + (int64_t)n0 * d.wo_stride_n) * ES);
+            else wrow = (const uint8_t*)d.wo + ((int64_t)next.e * d.wo_stride_e + (int64_t)row * d.wo_stride_n) * ES;
 #pragma unroll
             for (int f = 0; f < NT; ++f) {
                 const int c = 16 * f + r16 % COLS;
-                xrow[f] = c < next.n ? (const uint8_t*)p.h + (int64_t)next.slots[c] * d.H * XES : nullptr;
+                const uint32_t at = c < next.n ? (uint32_t)(l.slots[next.first + c] * d.H * XES) : ~0u;
+                if constexpr (ONE) xoff[f] = at;
+                else xrow[f] = at != ~0u ? (const uint8_t*)p.h + at : nullptr;
             }
         }
+        const int k = 2 * piece * STEP + quarter * CE;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int k = (2 * piece + s) * STEP + quarter * CE;
-            wb[s] = chunk<ES, VEC>(wrow, k, any ? d.H : 0);
-#pragma unroll
-            for (int f = 0; f < NT; ++f)
-#pragma unroll
-                for (int c = 0; c < XC; ++c) xb[s][f][c] = chunk<XES, VEC>(xrow[f], k + c * (16 / XES), any && xrow[f] ? d.H : 0);
+            if constexpr (ONE) wb[s] = w.chunk(woff, k + s * STEP, any ? d.H : 0);
+            else wb[s] = chunk<ES, VEC>(wrow, k + s * STEP, any ? d.H : 0);
         }
+#pragma unroll
+        for (int f = 0; f < NT; ++f)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int c = 0; c < XC; ++c) {
+                    const int at = k + s * STEP + c * (16 / XES);
+                    if constexpr (ONE) xb[s][f][c] = x.chunk(xoff[f], at, any && xoff[f] != ~0u ? d.H : 0);
+                    else xb[s][f][c] = chunk<XES, VEC>(xrow[f], at, any && xrow[f] ? d.H : 0);
+                }
         ++q;
         if (++piece == pieces) {
             piece = 0;
             ++index;
         }
     };
-    f32x4 acc[NT];
+    f32x4 acc[NT], inv = {1.0f, 1.0f, 1.0f, 1.0f};
 #pragma unroll
     for (int f = 0; f < NT; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     // An expert's products go to its own tokens' sums, and only there (a column without a token holds zeros, which an infinity among the weights
     // turns into NaN).
     auto flush = [&] {
-        if (cur.index >= 0) {
-            f32x4 inv = {1.0f, 1.0f, 1.0f, 1.0f};
-            if constexpr (WT == kWE4M3) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) inv[i] = 1.0f / d.wo_scale[(int64_t)cur.e * d.O + min(n0 + (4 * quarter + i) % COLS, d.O - 1)];
-            }
+        if (cur_index >= 0) {
 #pragma unroll
             for (int f = 0; f < NT; ++f) {
                 const int c = 16 * f + r16 % COLS;
-                if (c < cur.n && quarter * 4 / COLS == part) {
-                    f32x4* const to = reinterpret_cast<f32x4*>(sums + ((size_t)wave * d.T + cur.slots[c] / d.k) * 16 + 4 * quarter);
+                if (c < cur.n && (ONE || quarter * 4 / COLS == part)) {
+                    f32x4* const to = reinterpret_cast<f32x4*>(sums + ((size_t)wave * d.T + l.slots[cur.first + c] / d.k) * 16 + 4 * quarter);
                     f32x4 v = *to;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] += acc[f][i] * inv[i];
+                    for (int i = 0; i < 4; ++i) v[i] += WT == kWE4M3 ? acc[f][i] / inv[i] : acc[f][i];
                     *to = v;
                 }
             }
@@ -638,13 +680,19 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
         for (int f = 0; f < NT; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     };
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) load(next_of[i], wv[i], xv[i]);
+    for (int i = 0; i < AHEAD; ++i) load(of[i], wv[i], xv[i]);
     for (int done = 0; done < per; done += AHEAD) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {       // (behind a stretch's last piece come zeros)
-            if (__any(next_of[i] != cur.index)) {
+            if (ONE ? of[i] != cur_index : __any(of[i] != cur_index)) {
                 flush();
-                if (next_of[i] >= 0) cur = entry_of(next_of[i]);
+                if (of[i] >= 0) {
+                    cur = few_entry<ONE>(l, of[i]);
+                    cur_index = of[i];
+                    if constexpr (WT == kWE4M3)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) inv[j] = d.wo_scale[(int64_t)cur.e * d.O + min(n0 + (4 * quarter + j) % COLS, d.O - 1)];
+                }
             }
 #pragma unroll
             for (int f = 0; f < NT; ++f)
@@ -652,18 +700,38 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
                     mma<WT>(acc[f], wv[i][0], xv[i][0][f]);
                     mma<WT>(acc[f], wv[i][1], xv[i][1][f]);
                 }
-            load(next_of[i], wv[i], xv[i]);
+            load(of[i], wv[i], xv[i]);
         }
     }
     flush();
     __syncthreads();
-    for (int i = threadIdx.x; i < d.T * COLS; i += blockDim.x) {
-        const int t = i / COLS, c = i % COLS, col = n0 + c;
-        if (col >= d.O) continue;
+    float* const partial = p.partial + (int64_t)blockIdx.x * gridDim.y * d.T * COLS;        // [tile][block][T][COLS]
+    bool last = true;
+    auto own = [&](int t, int c) {
         float v = 0.0f;
         for (int w = 0; w < waves; ++w)
 #pragma unroll
             for (int q2 = 0; q2 < PARTS; ++q2) v += sums[((size_t)w * d.T + t) * 16 + q2 * COLS + c];
+        return v;
+    };
+    if (gridDim.y > 1) {
+        for (int i = threadIdx.x; i < d.T * COLS; i += blockDim.x) partial[(int64_t)blockIdx.y * d.T * COLS + i] = own(i / COLS, i % COLS);
+        __threadfence();
+        __syncthreads();
+        int* const arrived = (int*)lds;         // (the sums have been read)
+        if (threadIdx.x == 0) *arrived = atomicAdd(p.arrivals + blockIdx.x, 1);
+        __syncthreads();
+        last = *arrived == (int)gridDim.y - 1;
+        __threadfence();
+    }
+    if (!last) return;
+    for (int i = threadIdx.x; i < d.T * COLS; i += blockDim.x) {
+        const int t = i / COLS, c = i % COLS, col = n0 + c;
+        if (col >= d.O) continue;
+        float v = 0.0f;
+        if (gridDim.y > 1)
+            for (unsigned y = 0; y < gridDim.y; ++y) v += __hip_atomic_load(partial + (int64_t)y * d.T * COLS + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        else v = own(t, c);
         if (d.bias_out)
             for (int j = 0; j < d.k; ++j) {
                 const int e = l.sel[t * d.k + j];
@@ -681,7 +749,22 @@ int few_stretches(const fmoe_few_desc& d) {
     if ((int64_t)d.E * d.D * (d.dtype == FMOE_F32 ? 4 : 2) * ((d.T + 15) / 16) <= 32 * 1024) return 0;
     return d.T <= 16 ? 4 : 1;
 }
-size_t few_bytes(const fmoe_few_desc& d) { return few_logits_at(d) + (size_t)few_stretches(d) * d.T * d.E * 4; }
+size_t few_arrivals_at(const fmoe_few_desc& d) { return (few_logits_at(d) + (size_t)few_stretches(d) * d.T * d.E * 4 + 255) & ~(size_t)255; }
+// few_down's tiles: parts of an MFMA's rows (up to 16 / parts tokens) so that there are 256 of them, else blocks to a tile.
+struct DownPlan {
+    int parts, tiles, blocks;
+};
+DownPlan few_down_plan(const fmoe_few_desc& d) {
+    DownPlan p;
+    p.parts = d.O >= 16 * 256 || d.T > 8 ? 1 : d.O >= 8 * 256 || d.T > 4 ? 2 : 4;
+    p.tiles = (d.O + 16 / p.parts - 1) / (16 / p.parts);
+    p.blocks = p.parts > 1 || p.tiles > 128 ? 1 : 256 / p.tiles < 8 ? 256 / p.tiles : 8;
+    return p;
+}
+size_t few_bytes(const fmoe_few_desc& d) {
+    const DownPlan p = few_down_plan(d);
+    return few_arrivals_at(d) + (p.blocks > 1 ? (((size_t)p.tiles * 4 + 255) & ~(size_t)255) + (size_t)p.tiles * p.blocks * d.T * (16 / p.parts) * 4 : 0);
+}
 
 int few_check(const fmoe_few_desc* d) {
     FMOE_REQUIRE(d, "fmoe_few_tokens: desc is NULL");
@@ -725,7 +808,10 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     if (!workspace || workspace_bytes < need)
         return fail(FMOE_ERR_WORKSPACE, "fmoe_few_tokens: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     FMOE_REQUIRE(aligned16(workspace), "fmoe_few_tokens: the workspace must be 16-byte aligned");
-    const FewParams p{d, workspace, (uint8_t*)workspace + few_hidden_at(d), (const float*)((uint8_t*)workspace + few_logits_at(d)), few_stretches(d)};
+    const DownPlan plan = few_down_plan(d);
+    const FewParams p{d, workspace, (uint8_t*)workspace + few_hidden_at(d), (const float*)((uint8_t*)workspace + few_logits_at(d)), few_stretches(d), plan.blocks > 1 ? plan.tiles : 0,
+                      (int32_t*)((uint8_t*)workspace + few_arrivals_at(d)),
+                      (float*)((uint8_t*)workspace + few_arrivals_at(d) + (((size_t)plan.tiles * 4 + 255) & ~(size_t)255))};
     const int es = d.dtype == FMOE_F32 ? 4 : 2, wes = d.weight_dtype == FMOE_E4M3 ? 1 : es;
     // whole 16-byte chunks at 16-byte boundaries wherever rows are read
     auto whole = [](const void* q, int64_t elements, int size) { return aligned16(q) && elements * size % 16 == 0; };
@@ -736,19 +822,31 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     const int most_active = d.T * d.k < d.E ? d.T * d.k : d.E;
     hipStream_t stream = (hipStream_t)stream_;
     const int lists = few_lists_bytes(d.T, d.E, d.k), step = wes == 1 ? 64 : 64 / wes;
-    // waves to an item: four steps each where the rows are that long
+    const int64_t items = (int64_t)most_active * ((d.H + 15) / 16) * (d.T > 32 ? 2 : 1);
+    // waves to an item: so that each has four steps, and no CU is without an item for want of blocks
     int share_bits = 0;
-    while (share_bits < 4 && (4 << share_bits) * step < d.D) ++share_bits;
-    auto up = [&](auto kern, int nt) {
-        const int64_t items = (int64_t)most_active * ((d.H + 15) / 16) * (nt == 2 && d.T > 32 ? 2 : 1), blocks = (items + (kWaves >> share_bits) - 1) / (kWaves >> share_bits);
-        kern<<<(unsigned)(blocks < 256 ? blocks : 256), kWaves * kWave, kRedBytes + (p.stretches ? 0 : few_align(16 * d.E * 4)) + lists, stream>>>(p, share_bits);
+    while (share_bits < 4 && ((4 << share_bits) * step < d.D || (items << share_bits) < 256 * kWaves)) ++share_bits;
+    auto up = [&](auto kern, bool& reserved) {
+        const int bytes = kRedBytes + (p.stretches ? 0 : few_align(16 * d.E * 4)) + lists;
+        if (!reserved) {        // (more than 64 KB; the most that any call of this kernel asks for)
+            const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                       kRedBytes + few_align(16 * kFewMostExperts * 4) + few_lists_bytes(kFewMostTokens, kFewMostExperts, kFewMostK));
+            if (err != hipSuccess) return fail(FMOE_ERR_LAUNCH, "fmoe_few_tokens: cannot reserve %d B of LDS: %s", bytes, hipGetErrorString(err));
+            reserved = true;
+        }
+        const int64_t blocks = (items + (kWaves >> share_bits) - 1) / (kWaves >> share_bits);
+        kern<<<(unsigned)(blocks < 256 ? blocks : 256), kWaves * kWave, bytes, stream>>>(p, share_bits);
+        return check_launch("fmoe_few_tokens");
     };
-    auto down = [&](auto kern, int parts) {
-        const int cols = 16 / parts, waves = d.T > 32 ? kWaves / 2 : kWaves;        // (their sums for 64 tokens in 64 KB of LDS)
-        kern<<<(unsigned)((d.O + cols - 1) / cols), waves * kWave, waves * d.T * 64 + lists, stream>>>(p);
+    auto down = [&](auto kern) {
+        const int waves = d.T > 32 ? kWaves / 2 : kWaves;        // (their sums for 64 tokens in 32 KB of LDS)
+        kern<<<dim3(plan.tiles, plan.blocks), waves * kWave, waves * d.T * 64 + lists, stream>>>(p);
     };
-    const int parts = d.O >= 16 * 256 || d.T > 8 ? 1 : d.O >= 8 * 256 || d.T > 4 ? 2 : 4;
-#define FMOE_FEW_UP(WT, VEC, NT) (gated ? up(few_up_kernel<WT, VEC, NT, true>, NT) : up(few_up_kernel<WT, VEC, NT, false>, NT))
+#define FMOE_FEW_UP(WT, VEC, NT, GATED)                                     \
+    ([&] {                                                                  \
+        static bool reserved = false;                                       \
+        return up(few_up_kernel<WT, VEC, NT, GATED>, reserved);             \
+    })()
 #define FMOE_FEW(WT, VEC)                                                   \
     do {                                                                    \
         if (p.stretches) {                                                  \
@@ -756,13 +854,13 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
             const int first = check_launch("fmoe_few_tokens");              \
             if (first != FMOE_OK) return first;                             \
         }                                                                   \
-        if (d.T <= 16) FMOE_FEW_UP(WT, VEC, 1); else FMOE_FEW_UP(WT, VEC, 2); \
-        const int launched = check_launch("fmoe_few_tokens");               \
-        if (launched != FMOE_OK) return launched;                           \
-        if (d.T > 16) down(few_down_kernel<WT, VEC, 2, 1>, 1);              \
-        else if (parts == 1) down(few_down_kernel<WT, VEC, 1, 1>, 1);       \
-        else if (parts == 2) down(few_down_kernel<WT, VEC, 1, 2>, 2);       \
-        else down(few_down_kernel<WT, VEC, 1, 4>, 4);                       \
+        const int second = d.T <= 16 ? (gated ? FMOE_FEW_UP(WT, VEC, 1, true) : FMOE_FEW_UP(WT, VEC, 1, false)) \
+                                     : (gated ? FMOE_FEW_UP(WT, VEC, 2, true) : FMOE_FEW_UP(WT, VEC, 2, false)); \
+        if (second != FMOE_OK) return second;                               \
+        if (d.T > 16) down(few_down_kernel<WT, VEC, 2, 1>);                 \
+        else if (plan.parts == 1) down(few_down_kernel<WT, VEC, 1, 1>);     \
+        else if (plan.parts == 2) down(few_down_kernel<WT, VEC, 1, 2>);     \
+        else down(few_down_kernel<WT, VEC, 1, 4>);                          \
     } while (0)
     if (d.weight_dtype == FMOE_F32) {
         if (vec) FMOE_FEW(kWF32, true); else FMOE_FEW(kWF32, false);
