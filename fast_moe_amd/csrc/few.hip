@@ -522,11 +522,18 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 #pragma unroll
                     for (int m = 0; m < ROUND; ++m) {
                         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                        for (int w = 0; w < shares; ++w) {
-                            const f32x4 part = buf[(((group * shares + w) * ROUND + m) * NT + f) * kWave + lane];
+                        const auto add = [&](int from, int waves) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] += part[i];
-                        }
+                            for (int w = 0; w < waves; ++w) {
+                                const f32x4 part = buf[(((group * shares + from + w) * ROUND + m) * NT + f) * kWave + lane];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) v[i] += part[i];
+                            }
+                        };
+                        if (shares >= 4)
+                            for (int w = 0; w < shares; w += 4) add(w, 4);
+                        else
+                            for (int w = 0; w < shares; ++w) add(w, 1);
                         sum[m0 + m][f] = v;
                     }
         }
@@ -605,7 +612,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
     __syncthreads();
     const int part = ONE ? 0 : r16 / COLS, n0 = blockIdx.x * COLS, row = min(n0 + r16 % COLS, d.O - 1);
     const int steps = (d.H + STEP - 1) / STEP, pieces = (steps + 1) / 2, total = uniform(*l.entries) * pieces;
-    // every stretch (a wave's, or a part of its) takes as many pieces of two steps, entries after one another
+    // every stretch (a wave's, or a part of its) takes as many pieces of two steps, experts after one another
     const int stretches = waves * PARTS * gridDim.y, per = (total + stretches - 1) / stretches;
     const int from = ((blockIdx.y * waves + wave) * PARTS + part) * per, until = min(total, from + per);
     Entry next = {0, 0, 0}, cur = {0, 0, 0};            // whose loads are on their way, and whose products add up
@@ -709,20 +716,21 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
     bool last = true;
     auto own = [&](int t, int c) {
         float v = 0.0f;
-        for (int w = 0; w < waves; ++w)
+        for (int w0 = 0; w0 < waves; w0 += 8)       // (8 or 16)
 #pragma unroll
-            for (int q2 = 0; q2 < PARTS; ++q2) v += sums[((size_t)w * d.T + t) * 16 + q2 * COLS + c];
+            for (int w = 0; w < 8; ++w)
+#pragma unroll
+                for (int q2 = 0; q2 < PARTS; ++q2) v += sums[((w0 + w) * d.T + t) * 16 + q2 * COLS + c];
         return v;
     };
     if (gridDim.y > 1) {
         for (int i = threadIdx.x; i < d.T * COLS; i += blockDim.x) partial[(int64_t)blockIdx.y * d.T * COLS + i] = own(i / COLS, i % COLS);
-        __threadfence();
         __syncthreads();
         int* const arrived = (int*)lds;         // (the sums have been read)
-        if (threadIdx.x == 0) *arrived = atomicAdd(p.arrivals + blockIdx.x, 1);
+        // (one wave's release and acquire, behind and before a barrier, stand for the block's; a fence of every wave took 50 us)
+        if (threadIdx.x == 0) *arrived = __hip_atomic_fetch_add(p.arrivals + blockIdx.x, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         last = *arrived == (int)gridDim.y - 1;
-        __threadfence();
     }
     if (!last) return;
     for (int i = threadIdx.x; i < d.T * COLS; i += blockDim.x) {

@@ -45,6 +45,8 @@ decltype(&fmoe_invert_index) c_invert_index;
 decltype(&fmoe_gate_l1_bwd) c_gate_l1_bwd;
 decltype(&fmoe_weight_grad) c_weight_grad;
 decltype(&fmoe_weight_grad_pays) weight_grad_pays;
+decltype(&fmoe_few_tokens_workspace_bytes) few_tokens_workspace_bytes;
+decltype(&fmoe_few_tokens) c_few_tokens;
 decltype(&fmoe_last_error) last_error;
 
 constexpr int64_t kSlackRows = 128;      // ops.SLACK_ROWS
@@ -785,12 +787,94 @@ PyObject* py_weight_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// (x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out, token_mask, w_scale, wp_scale, wo_scale, k, renorm,
+// stream) -> [T, O]
+PyObject* py_few_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 16) return none();
+    enum { X, GATE, GATE_BIAS, W, BIAS, WP, BIAS_P, WO, BIAS_OUT, MASK, S, SP, SO, COUNT };
+    at::Tensor t[COUNT], out, workspace;
+    for (int i = 0; i < COUNT; ++i)
+        if (!optional_tensor(args[i], &t[i])) return none();
+    int64_t k, renorm, stream;
+    if (!as_int(args[13], &k) || !as_int(args[14], &renorm) || !as_int(args[15], &stream)) return none();
+    for (int i : {X, GATE, W, WO})
+        if (!t[i].defined()) return none();
+    fmoe_few_desc d = {};
+    const int status = run(
+        [&] {
+            const bool fp8 = t[S].defined();
+            const at::ScalarType type = t[X].scalar_type(), w_type = fp8 ? at::kFloat8_e4m3fn : type;
+            if (!float_matrix(t[X]) || !float_matrix(t[GATE]) || t[W].dim() != 3 || t[WO].dim() != 3 || (fp8 && type != at::kBFloat16)) return false;
+            const int64_t T = t[X].size(0), D = t[X].size(1), E = t[GATE].size(0), H = t[W].size(2), O = t[WO].size(2);
+            if (T < 1 || T > 64 || D < 1 || H < 1 || O < 1 || E > 256 || k < 1 || k > 16 || D > INT32_MAX || H > INT32_MAX || O > INT32_MAX) return false;
+            for (const at::Tensor& v : t)
+                if (!same_device(t[X], v)) return false;
+            if (t[GATE].scalar_type() != type || t[GATE].size(1) != D || t[X].stride(0) < D || t[GATE].stride(0) < D) return false;
+            auto weight = [&](const at::Tensor& v, int64_t in, int64_t cols) {
+                return v.scalar_type() == w_type && v.size(0) == E && v.size(1) == in && v.size(2) == cols && v.stride(1) == 1 && v.stride(2) >= in &&
+                       v.stride(0) >= 0;
+            };
+            if (!weight(t[W], D, H) || !weight(t[WO], H, O)) return false;
+            if (t[WP].defined() && (t[WP].dim() != 3 || !weight(t[WP], D, H) || t[WP].strides() != t[W].strides())) return false;
+            auto rows = [&](const at::Tensor& v, at::ScalarType of, int64_t cols) {
+                return !v.defined() || (v.scalar_type() == of && v.dim() == 2 && v.size(0) == E && v.size(1) == cols && v.is_contiguous());
+            };
+            if (!rows(t[BIAS], type, H) || !rows(t[BIAS_P], type, H) || !rows(t[BIAS_OUT], type, O) || !rows(t[S], at::kFloat, H) ||
+                !rows(t[SP], at::kFloat, H) || !rows(t[SO], at::kFloat, O))
+                return false;
+            if (t[SO].defined() != fp8 || t[SP].defined() != (fp8 && t[WP].defined()) || (t[BIAS_P].defined() && !t[WP].defined())) return false;
+            if (t[GATE_BIAS].defined() && (t[GATE_BIAS].scalar_type() != type || t[GATE_BIAS].dim() != 1 || t[GATE_BIAS].size(0) != E || !t[GATE_BIAS].is_contiguous()))
+                return false;
+            if (t[MASK].defined() && (t[MASK].scalar_type() != at::kBool || t[MASK].dim() != 1 || t[MASK].size(0) != T || !t[MASK].is_contiguous())) return false;
+            auto data = [&](int i) { return t[i].defined() ? t[i].data_ptr() : nullptr; };
+            d.T = (int32_t)T, d.E = (int32_t)E, d.k = (int32_t)k, d.D = (int32_t)D, d.H = (int32_t)H, d.O = (int32_t)O;
+            d.dtype = dtype_code(type);
+            d.weight_dtype = dtype_code(w_type);
+            d.renorm = renorm != 0;
+            d.x = data(X);
+            d.x_stride_row = t[X].stride(0);
+            d.gate_weight = data(GATE);
+            d.gate_stride_row = t[GATE].stride(0);
+            d.gate_bias = data(GATE_BIAS);
+            d.token_mask = (const uint8_t*)data(MASK);
+            d.w = data(W);
+            d.wp = data(WP);
+            d.w_stride_e = t[W].stride(0);
+            d.w_stride_n = t[W].stride(2);
+            d.wo = data(WO);
+            d.wo_stride_e = t[WO].stride(0);
+            d.wo_stride_n = t[WO].stride(2);
+            d.w_scale = (const float*)data(S);
+            d.wp_scale = (const float*)data(SP);
+            d.wo_scale = (const float*)data(SO);
+            d.bias = data(BIAS);
+            d.bias_p = data(BIAS_P);
+            d.bias_stride_e = H;
+            d.bias_out = data(BIAS_OUT);
+            d.bias_out_stride_e = O;
+            d.out_stride_row = O;
+            return true;
+        },
+        [&] {
+            out = empty({t[X].size(0), t[WO].size(2)}, t[X].scalar_type(), t[X]);
+            d.out = out.data_ptr();
+            const size_t bytes = few_tokens_workspace_bytes(&d);
+            if (!bytes) return (int)FMOE_ERR_ARGUMENT;      // (refused: left to the Python code)
+            workspace = empty({(int64_t)bytes}, at::kByte, t[X]);
+            return c_few_tokens(&d, workspace.data_ptr(), bytes, (void*)stream);
+        });
+    if (raised(status, "fmoe_few_tokens")) return nullptr;
+    return status == FMOE_OK ? wrap(out) : none();
+    END_HANDLE_TH_ERRORS
+}
+
 // init(addresses of the C entry points, in the order of the pointers above)
 PyObject* py_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void* const entry[] = {&route_workspace_bytes, &c_route_topk, &c_grouped_gemm, &c_combine, &c_quant_rows, &c_gate_softmax, &gemm_workspace_bytes,
                            &c_grouped_gemm_ws, &c_gemm_plan, &c_combine_bwd, &c_segment_colsum, &c_swiglu_bwd, &c_silu_mul, &c_gather_rows,
                            &c_invert_index, &c_gate_l1_bwd, &c_weight_grad, &weight_grad_pays, &gate_softmax_pays,
-                           &gate_route_pays, &last_error};
+                           &gate_route_pays, &few_tokens_workspace_bytes, &c_few_tokens, &last_error};
     constexpr Py_ssize_t count = sizeof(entry) / sizeof(entry[0]);
     if (n != count) {
         PyErr_Format(PyExc_TypeError, "init: %d addresses expected", (int)count);
@@ -825,6 +909,7 @@ PyMethodDef methods[] = {
     FASTCALL("weight_grad", py_weight_grad),
     FASTCALL("gate_softmax", py_gate_softmax),
     FASTCALL("mlp_forward", py_mlp_forward),
+    FASTCALL("few_tokens", py_few_tokens),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -840,6 +840,11 @@ def few_tokens(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias: Optional[t
     [E, H, O] are views of storage with the contraction contiguous (``stride(1) == 1``), of x's dtype or, with ``scales``
     (multipliers [E, H], [E, H], [E, O] in fp32), e4m3."""
     name = "fused_moe_few_tokens"
+    if x.is_cuda and x.get_device() == torch.cuda.current_device():
+        out = _lib.host().few_tokens(x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out, token_mask, *scales, k,
+                                     bool(renorm), _stream(x))
+        if out is not None:
+            return out
     dev = _need_cuda(name, x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out, token_mask, *scales)
     if x.dtype not in _DTYPE_CODE:
         raise NotImplementedError(f"{name}: the HIP kernels take bf16 or fp32 tokens, got {x.dtype}")
