@@ -1,0 +1,262 @@
+// The two pre-activations of a SwiGLU expert block in 8 bits between forward and backward (fmoe_swiglu_checkpoint and what reads it):
+//
+//   a block of 32 neighbours of a row shares the power of two X = 2^floor(log2(largest magnitude)), kept as its biased exponent in a byte;
+//   code = round(v / X * 64) to nearest even, held to +-127;  v' = code * X / 64            (the MXINT8 format of the OCP microscaling spec)
+//   backward on g', u':  s = sigmoid(g'),  h = g' s u',  dh = w d,  dg = dh u' s (1 + g' (1 - s)),  du = dh g' s,
+//   and, for the weight gradient behind it and the rows' own weights w: w h and the row sums of h d
+//
+// 33 / 32 bytes for a value of 2 or 4, error at most half a step of 1 / 64 (3 % of the blocks' largest, rounded down to +-127: a whole step at the
+// very top); every v' is exact in bf16.  A zero block has exponent 0; one with an infinity or NaN has 255 and reads as NaN.
+// All of it is bound by the bytes; a lane has 16 values to write and 8 to read with (the row sum wants rows in whole waves, and 1408 columns leave
+// a third of the lanes of 16 idle, 8 % of those of 8).
+#include "common.h"
+
+namespace fmoe {
+namespace {
+
+template <typename E> struct CE;
+template <> struct CE<float> { static constexpr int V = 4; };
+template <> struct CE<uint16_t> { static constexpr int V = 8; };
+
+template <typename E>
+__device__ __forceinline__ float value_of(E v) {
+    if constexpr (sizeof(E) == 4) return v;
+    else return bf16_bits_to_f32(v);
+}
+// n values (a multiple of a 16-byte chunk's), VEC: 16 bytes at a time; those from `left` on are zeros
+template <typename E, bool VEC, int N>
+__device__ __forceinline__ void load_values(const E* p, int left, float (&f)[N]) {
+    constexpr int V = CE<E>::V;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int c = 0; c < N / V; ++c) {
+            u32x4 v = {0, 0, 0, 0};
+            if (c * V < left) v = *reinterpret_cast<const u32x4*>(p + c * V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if constexpr (V == 4) f[c * V + i] = __uint_as_float(v[i]);
+                else f[c * V + i] = i & 1 ? __uint_as_float(v[i / 2] & 0xffff0000u) : __uint_as_float(v[i / 2] << 16);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = i < left ? value_of(p[i]) : 0.0f;
+    }
+}
+template <typename E, bool VEC, int N>
+__device__ __forceinline__ void store_values(E* p, int left, const float (&f)[N]) {
+    constexpr int V = CE<E>::V;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int c = 0; c < N / V; ++c) {
+            if (c * V >= left) continue;
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (V == 4) v[i] = __float_as_uint(f[c * V + i]);
+                else v[i] = cvt_pk_bf16(f[c * V + 2 * i], f[c * V + 2 * i + 1]);
+            }
+            *reinterpret_cast<u32x4*>(p + c * V) = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < left) {
+                if constexpr (sizeof(E) == 4) p[i] = f[i];
+                else p[i] = (uint16_t)f32_to_bf16_bits(f[i]);
+            }
+    }
+}
+
+struct CkptRows {
+    const void *g, *u;
+    int64_t g_stride, u_stride, rows;
+    int32_t cols, padded;       // padded: cols in whole blocks of 32
+    int8_t* q;                  // [rows][2][padded]
+    uint8_t* e;                 // [rows][2][padded / 32]
+};
+
+// 16 values a lane, two lanes a block; the lanes of a grid go over (row, matrix, half block) in memory order.
+template <typename E, bool VEC>
+__global__ __launch_bounds__(256) void swiglu_checkpoint_kernel(CkptRows p) {
+    const int halves = p.padded / 16, per_row = 2 * halves;
+    const int64_t first = (int64_t)blockIdx.x * 256, row0 = first / per_row;        // (once per wave, on the scalar unit)
+    const uint32_t at = (uint32_t)(first - row0 * per_row) + threadIdx.x;
+    const int64_t r = row0 + at / (uint32_t)per_row;
+    if (r >= p.rows) return;            // (whole blocks of 32: both lanes of one)
+    const int in_row = at % (uint32_t)per_row, m = in_row >= halves, c = 16 * (in_row - m * halves);
+    float f[16];
+    load_values<E, VEC>((const E*)(m ? p.u : p.g) + r * (m ? p.u_stride : p.g_stride) + c, p.cols - c, f);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0xB1, 0xF, 0xF, false));      // quad_perm [1,0,3,2]: the other half
+    const int biased = (int)(top >> 23);        // 255: not finite
+    u32x4 out;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float v = fminf(fmaxf(rintf(__builtin_amdgcn_ldexpf(f[4 * w + i], 133 - biased)), -127.0f), 127.0f);
+            word |= ((uint32_t)(int)v & 0xffu) << (8 * i);
+        }
+        out[w] = biased == 255 ? 0u : word;
+    }
+    const int64_t base = (2 * r + m) * p.padded + c;
+    *reinterpret_cast<u32x4*>(p.q + base) = out;
+    if (!(threadIdx.x & 1)) p.e[base / 32] = (uint8_t)biased;
+}
+
+// The scale of a block's codes, X / 64 (NaN for one that is not finite)
+__device__ __forceinline__ float code_scale(int biased) { return biased == 255 ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(1.0f, biased - 133); }
+
+// Eight codes
+__device__ __forceinline__ void decode(u32x2 q, float scale, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)(int)(int8_t)(q[i / 4] >> (8 * (i & 3))) * scale;
+}
+
+template <typename E, bool VEC>
+__global__ __launch_bounds__(256) void swiglu_checkpoint_read_kernel(CkptRows p) {
+    const int eighths = p.padded / 8, per_row = 2 * eighths;
+    const int64_t first = (int64_t)blockIdx.x * 256, row0 = first / per_row;
+    const uint32_t at = (uint32_t)(first - row0 * per_row) + threadIdx.x;
+    const int64_t r = row0 + at / (uint32_t)per_row;
+    if (r >= p.rows) return;
+    const int in_row = at % (uint32_t)per_row, m = in_row >= eighths, c = 8 * (in_row - m * eighths);
+    const int64_t base = (2 * r + m) * p.padded + c;
+    float f[8];
+    decode(*reinterpret_cast<const u32x2*>(p.q + base), code_scale(p.e[base / 32]), f);
+    store_values<E, VEC>((E*)(m ? p.u : p.g) + r * (m ? p.u_stride : p.g_stride) + c, p.cols - c, f);
+}
+
+struct CkptBwd {
+    const int8_t* q;
+    const uint8_t* e;
+    int64_t rows;
+    int32_t cols, padded;
+    const void* d;
+    int64_t d_stride;
+    const void* weight;
+    int32_t weight_f32;
+    void *dg, *du, *h;
+    int64_t dg_stride, h_stride;        // of dg and du, of h
+    float* dots;
+};
+
+// A wave per row, eight values a lane.
+template <typename E, bool VEC>
+__global__ __launch_bounds__(256) void swiglu_checkpoint_bwd_kernel(CkptBwd p) {
+    const int lane = lane_id();
+    const int64_t waves = (int64_t)gridDim.x * 4;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; r < p.rows; r += waves) {
+        const float w = !p.weight ? 1.0f : p.weight_f32 ? reinterpret_cast<const float*>(p.weight)[r] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p.weight)[r]);
+        const int8_t* const q = p.q + 2 * r * p.padded;
+        const uint8_t* const e = p.e + 2 * r * (p.padded / 32);
+        float dot = 0.0f;
+        for (int c = 8 * lane; c < p.cols; c += 8 * kWave) {
+            float g[8], u[8], d[8], dg[8], du[8], h[8];
+            const u32x2 qg = *reinterpret_cast<const u32x2*>(q + c), qu = *reinterpret_cast<const u32x2*>(q + p.padded + c);
+            const int eg = e[c / 32], eu = e[p.padded / 32 + c / 32];
+            load_values<E, VEC>((const E*)p.d + r * p.d_stride + c, p.cols - c, d);
+            decode(qg, code_scale(eg), g);
+            decode(qu, code_scale(eu), u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float s;
+                if constexpr (sizeof(E) == 4) s = 1.0f / (1.0f + expf(-g[i]));
+                else s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g[i] * -1.44269504088896341f));     // (rounded to bf16 behind it)
+                const float gs = g[i] * s, dh = w * d[i], hi = gs * u[i];
+                dg[i] = dh * u[i] * (s + gs * (1.0f - s));
+                du[i] = dh * gs;
+                h[i] = w * hi;
+                if (VEC || c + i < p.cols) dot = __builtin_fmaf(hi, d[i], dot);
+            }
+            store_values<E, VEC>((E*)p.dg + r * p.dg_stride + c, p.cols - c, dg);
+            store_values<E, VEC>((E*)p.du + r * p.dg_stride + c, p.cols - c, du);
+            if (p.h) store_values<E, VEC>((E*)p.h + r * p.h_stride + c, p.cols - c, h);
+        }
+        if (p.dots) {
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) dot += __shfl_xor(dot, o, kWave);
+            if (lane == 0) p.dots[r] = dot;
+        }
+    }
+}
+
+int ckpt_check(const char* name, int dtype, int64_t rows, int64_t cols, const void* q, const void* e) {
+    FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_BF16, "%s: bf16 or fp32 expected", name);
+    FMOE_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 24), "%s: rows >= 0 and 1 to 2^24 columns expected", name);
+    FMOE_REQUIRE(rows == 0 || (q && e), "%s: NULL tensor pointer", name);
+    FMOE_REQUIRE(aligned16(q), "%s: codes must be 16-byte aligned", name);
+    return FMOE_OK;
+}
+bool whole_rows(const void* p, int64_t stride, int dtype) { return aligned16(p) && stride * (dtype == FMOE_F32 ? 4 : 2) % 16 == 0; }
+
+}  // namespace
+}  // namespace fmoe
+
+using namespace fmoe;
+
+extern "C" int64_t fmoe_swiglu_checkpoint_cols(int64_t cols) { return (cols + 31) / 32 * 32; }
+
+static int ckpt_both(bool write, const char* name, void* g, void* u, int dtype, int64_t rows, int64_t cols, int64_t g_stride, int64_t u_stride, int8_t* q,
+                     uint8_t* e, fmoe_stream_t stream_) {
+    if (int rc = ckpt_check(name, dtype, rows, cols, q, e)) return rc;
+    if (rows == 0) return FMOE_OK;
+    FMOE_REQUIRE(g && u, "%s: NULL tensor pointer", name);
+    FMOE_REQUIRE(rows == 1 || (g_stride >= cols && u_stride >= cols), "%s: rows overlap", name);
+    const CkptRows p{g, u, g_stride, u_stride, rows, (int32_t)cols, (int32_t)fmoe_swiglu_checkpoint_cols(cols), q, e};
+    const bool vec = cols % 8 == 0 && whole_rows(g, g_stride, dtype) && whole_rows(u, u_stride, dtype);
+    const int64_t n = (rows * (2 * p.padded / (write ? 16 : 8)) + 255) / 256;
+    FMOE_REQUIRE(n < ((int64_t)1 << 31), "%s: too many values for one call", name);
+    const unsigned blocks = (unsigned)n;
+    hipStream_t stream = (hipStream_t)stream_;
+#define FMOE_CKPT(kern)                                                                                                    \
+    do {                                                                                                                   \
+        if (dtype == FMOE_F32) { if (vec) kern<float, true><<<blocks, 256, 0, stream>>>(p); else kern<float, false><<<blocks, 256, 0, stream>>>(p); } \
+        else { if (vec) kern<uint16_t, true><<<blocks, 256, 0, stream>>>(p); else kern<uint16_t, false><<<blocks, 256, 0, stream>>>(p); }           \
+    } while (0)
+    if (write) FMOE_CKPT(swiglu_checkpoint_kernel);
+    else FMOE_CKPT(swiglu_checkpoint_read_kernel);
+#undef FMOE_CKPT
+    return check_launch(name);
+}
+
+extern "C" int fmoe_swiglu_checkpoint(const void* g, const void* u, int dtype, int64_t rows, int64_t cols, int64_t g_stride_row, int64_t u_stride_row,
+                                      int8_t* q, uint8_t* e, fmoe_stream_t stream) {
+    return ckpt_both(true, "fmoe_swiglu_checkpoint", const_cast<void*>(g), const_cast<void*>(u), dtype, rows, cols, g_stride_row, u_stride_row, q, e, stream);
+}
+
+extern "C" int fmoe_swiglu_checkpoint_read(const int8_t* q, const uint8_t* e, void* g, void* u, int dtype, int64_t rows, int64_t cols,
+                                           int64_t g_stride_row, int64_t u_stride_row, fmoe_stream_t stream) {
+    return ckpt_both(false, "fmoe_swiglu_checkpoint_read", g, u, dtype, rows, cols, g_stride_row, u_stride_row, const_cast<int8_t*>(q),
+                     const_cast<uint8_t*>(e), stream);
+}
+
+extern "C" int fmoe_swiglu_checkpoint_bwd(const int8_t* q, const uint8_t* e, const void* d, int dtype, int64_t rows, int64_t cols, int64_t d_stride_row,
+                                          const void* weight, int weight_dtype, void* dg, void* du, int64_t dg_stride_row, void* h, int64_t h_stride_row,
+                                          float* dots, fmoe_stream_t stream_) {
+    const char* const name = "fmoe_swiglu_checkpoint_bwd";
+    if (int rc = ckpt_check(name, dtype, rows, cols, q, e)) return rc;
+    FMOE_REQUIRE(!weight || weight_dtype == FMOE_F32 || weight_dtype == FMOE_BF16, "%s: row weights must be bf16 or fp32", name);
+    if (rows == 0) return FMOE_OK;
+    FMOE_REQUIRE(d && dg && du, "%s: NULL tensor pointer", name);
+    FMOE_REQUIRE(rows == 1 || (d_stride_row >= cols && dg_stride_row >= cols && (!h || h_stride_row >= cols)), "%s: rows overlap", name);
+    const CkptBwd p{q, e, rows, (int32_t)cols, (int32_t)fmoe_swiglu_checkpoint_cols(cols), d, d_stride_row, weight, weight_dtype == FMOE_F32, dg, du, h,
+                    dg_stride_row, h_stride_row, dots};
+    const bool vec = cols % 8 == 0 && whole_rows(d, d_stride_row, dtype) && whole_rows(dg, dg_stride_row, dtype) && whole_rows(du, dg_stride_row, dtype) &&
+                     (!h || whole_rows(h, h_stride_row, dtype));
+    const int64_t n = (rows + 3) / 4;
+    const unsigned blocks = (unsigned)(n < 256 * 8 ? n : 256 * 8);
+    hipStream_t stream = (hipStream_t)stream_;
+    if (dtype == FMOE_F32) {
+        if (vec) swiglu_checkpoint_bwd_kernel<float, true><<<blocks, 256, 0, stream>>>(p);
+        else swiglu_checkpoint_bwd_kernel<float, false><<<blocks, 256, 0, stream>>>(p);
+    } else {
+        if (vec) swiglu_checkpoint_bwd_kernel<uint16_t, true><<<blocks, 256, 0, stream>>>(p);
+        else swiglu_checkpoint_bwd_kernel<uint16_t, false><<<blocks, 256, 0, stream>>>(p);
+    }
+    return check_launch(name);
+}

@@ -15,6 +15,8 @@ _PKG_DIR = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__fil
 LIB_PATH = os.environ.get("FMOE_LIB_PATH") or os.path.join(_PKG_DIR, "libfastmoe_hip.so")
 
 FMOE_F32, FMOE_BF16, FMOE_E4M3 = 0, 1, 2
+NORM_RMS, NORM_LAYER = 0, 1
+ROW_GATE_NONE, ROW_GATE_TOKEN, ROW_GATE_ELEMENT = 0, 1, 2
 EPI_NONE, EPI_SILU, EPI_SWIGLU, EPI_GATED = 0, 1, 2, 3
 PLAN_NONE, PLAN_RING, PLAN_STAGED, PLAN_STAGED_SHORT, PLAN_ELEMENT = -1, 0, 1, 2, 3
 
@@ -29,6 +31,8 @@ EXPORTED_SYMBOLS = (
     "fmoe_swiglu_bwd", "fmoe_combine_bwd", "fmoe_gather_rows", "fmoe_invert_index",
     "fmoe_gate_l1_bwd", "fmoe_gate_softmax_pays", "fmoe_gate_softmax", "fmoe_gate_route_pays", "fmoe_weight_grad_pays", "fmoe_weight_grad", "fmoe_route_topk_static", "fmoe_hbm_probe",
     "fmoe_few_tokens_workspace_bytes", "fmoe_few_tokens",
+    "fmoe_norm_add", "fmoe_norm_add_bwd_workspace_bytes", "fmoe_norm_add_bwd",
+    "fmoe_swiglu_checkpoint_cols", "fmoe_swiglu_checkpoint", "fmoe_swiglu_checkpoint_read", "fmoe_swiglu_checkpoint_bwd",
 )
 ROUTE_STATIC_MAX_POSITIONS, ROUTE_STATIC_MAX_EXPERTS = 1 << 20, 512
 
@@ -71,6 +75,21 @@ class FewDesc(ctypes.Structure):
         ("bias", c_void_p), ("bias_p", c_void_p), ("bias_stride_e", c_int64),
         ("bias_out", c_void_p), ("bias_out_stride_e", c_int64),
         ("out", c_void_p), ("out_stride_row", c_int64),
+    ]
+
+
+class NormDesc(ctypes.Structure):
+    """struct fmoe_norm_desc, field for field."""
+    _fields_ = [
+        ("rows", c_int64), ("cols", c_int32), ("dtype", c_int32), ("param_dtype", c_int32), ("norm", c_int32),
+        ("gate_mode", c_int32), ("gate_sigmoid", c_int32), ("eps", c_float), ("scale_value", c_float),
+        ("y", c_void_p), ("y_stride", c_int64), ("K", c_int32), ("merge_dtype", c_int32), ("value_rows", c_int64),
+        ("reverse_index", c_void_p), ("merge", c_void_p), ("merge_index", c_void_p),
+        ("residual", c_void_p), ("residual_stride", c_int64), ("gate", c_void_p), ("gate_stride", c_int64),
+        ("scale", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("next_weight", c_void_p), ("next_bias", c_void_p),
+        ("out", c_void_p), ("next", c_void_p), ("y_out", c_void_p), ("stats", c_void_p),
+        ("d_out", c_void_p), ("d_next", c_void_p), ("d_y", c_void_p), ("d_residual", c_void_p), ("d_gate", c_void_p),
+        ("d_scale", c_void_p), ("d_weight", c_void_p), ("d_bias", c_void_p), ("d_next_weight", c_void_p), ("d_next_bias", c_void_p),
     ]
 
 
@@ -163,6 +182,21 @@ def load() -> ctypes.CDLL:
     lib.fmoe_few_tokens_workspace_bytes.argtypes = [POINTER(FewDesc)]
     lib.fmoe_few_tokens.restype = c_int
     lib.fmoe_few_tokens.argtypes = [POINTER(FewDesc), c_void_p, c_size_t, c_void_p]
+    lib.fmoe_norm_add.restype = c_int
+    lib.fmoe_norm_add.argtypes = [POINTER(NormDesc), c_void_p]
+    lib.fmoe_norm_add_bwd_workspace_bytes.restype = c_size_t
+    lib.fmoe_norm_add_bwd_workspace_bytes.argtypes = [POINTER(NormDesc)]
+    lib.fmoe_norm_add_bwd.restype = c_int
+    lib.fmoe_norm_add_bwd.argtypes = [POINTER(NormDesc), c_void_p, c_size_t, c_void_p]
+    lib.fmoe_swiglu_checkpoint_cols.restype = c_int64
+    lib.fmoe_swiglu_checkpoint_cols.argtypes = [c_int64]
+    lib.fmoe_swiglu_checkpoint.restype = c_int
+    lib.fmoe_swiglu_checkpoint.argtypes = [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
+    lib.fmoe_swiglu_checkpoint_read.restype = c_int
+    lib.fmoe_swiglu_checkpoint_read.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p]
+    lib.fmoe_swiglu_checkpoint_bwd.restype = c_int
+    lib.fmoe_swiglu_checkpoint_bwd.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p,
+                                               c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]
     _lib = lib
     return lib
 

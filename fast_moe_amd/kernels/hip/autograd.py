@@ -131,6 +131,42 @@ def _input_grad(drow_list, weights, offsets, reverse_index) -> torch.Tensor:
     return ops.combine(value, rev)
 
 
+def _gather_gemm_grads(offsets, index, jagged, weight, bias, weight_p, bias_p, drows, both, need):
+    """Gradients of the operands (jagged, weight, bias, weight_p, bias_p) of a gather GEMM from those of its output rows; ``both``:
+    the two branches' row gradients as one operand, or None.  ``need``: which are wanted, in that order."""
+    swiglu = weight_p is not None
+    K, R = index.shape[-1], index.numel()
+    weights = [weight, weight_p] if swiglu else [weight]
+    d_jagged = d_w = d_b = d_wp = d_bp = None
+    if need[0]:
+        d_jagged = _input_grad(drows, weights, offsets, ops.invert_index(index)).view_as(jagged)
+    operand = None
+    if need[1] or (swiglu and need[3]):
+        operand = _WgradOperand(jagged, offsets, R, row_index=index.reshape(-1), index_div=K)
+    H = drows[0].shape[1]
+    pair = None
+    if both is not None and need[1] and need[3] and not (weight.stride(2) == 1 and weight.stride(1) != 1):
+        # one GEMM for both weight gradients (2H = 2816 rows per expert fill whole 256-row tiles
+        # where H = 1408 leaves every sixth one half empty), each into its own tensor
+        pair = operand.weight_grad_pair(both)
+    if pair is not None:
+        d_w, d_wp = pair[0].permute(0, 2, 1), pair[1].permute(0, 2, 1)
+    else:
+        if need[1]:
+            d_w = operand.weight_grad(drows[0], weight)
+        if swiglu and need[3]:
+            d_wp = operand.weight_grad(drows[1], weight_p)
+    if both is not None and bias is not None and bias_p is not None and need[2] and need[4]:
+        d_sum = ops.segment_colsum(both, offsets)
+        d_b, d_bp = d_sum[:, :H], d_sum[:, H:]
+    else:
+        if bias is not None and need[2]:
+            d_b = ops.segment_colsum(drows[0], offsets)
+        if swiglu and bias_p is not None and need[4]:
+            d_bp = ops.segment_colsum(drows[1], offsets)
+    return d_jagged, d_w, d_b, d_wp, d_bp
+
+
 class IndexSelectJaggedBmm(torch.autograd.Function):
     """index_select_jagged_bmm and index_select_jagged_bmm_swiglu (weight_p is None or not)."""
 
@@ -151,46 +187,18 @@ class IndexSelectJaggedBmm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         offsets, index, jagged, weight, bias, weight_p, bias_p, g, u = ctx.saved_tensors
-        K = index.shape[-1]
-        R = index.numel()
         dout = dout.contiguous()
         swiglu = weight_p is not None
         both = None
         if swiglu:      # dg | du side by side in one buffer: the GEMMs that need both read one operand
             dg, du = ops.swiglu_bwd(g, u, dout, joint=True)
             del g, u
-            drows, weights = [dg, du], [weight, weight_p]
+            drows = [dg, du]
             both = ops.joint_rows(dg, du)
         else:
-            drows, weights = [dout], [weight]
-        need = ctx.needs_input_grad
-        d_jagged = d_w = d_b = d_wp = d_bp = None
-        if need[2]:
-            d_jagged = _input_grad(drows, weights, offsets, ops.invert_index(index)).view_as(jagged)
-        operand = None
-        if need[3] or (swiglu and need[5]):
-            operand = _WgradOperand(jagged, offsets, R, row_index=index.reshape(-1), index_div=K)
-        H = drows[0].shape[1]
-        pair = None
-        if both is not None and need[3] and need[5] and not (weight.stride(2) == 1 and weight.stride(1) != 1):
-            # one GEMM for both weight gradients (2H = 2816 rows per expert fill whole 256-row tiles
-            # where H = 1408 leaves every sixth one half empty), each into its own tensor
-            pair = operand.weight_grad_pair(both)
-        if pair is not None:
-            d_w, d_wp = pair[0].permute(0, 2, 1), pair[1].permute(0, 2, 1)
-        else:
-            if need[3]:
-                d_w = operand.weight_grad(drows[0], weight)
-            if swiglu and need[5]:
-                d_wp = operand.weight_grad(drows[1], weight_p)
-        if both is not None and bias is not None and bias_p is not None and need[4] and need[6]:
-            d_sum = ops.segment_colsum(both, offsets)
-            d_b, d_bp = d_sum[:, :H], d_sum[:, H:]
-        else:
-            if bias is not None and need[4]:
-                d_b = ops.segment_colsum(drows[0], offsets)
-            if swiglu and bias_p is not None and need[6]:
-                d_bp = ops.segment_colsum(drows[1], offsets)
+            drows = [dout]
+        d_jagged, d_w, d_b, d_wp, d_bp = _gather_gemm_grads(offsets, index, jagged, weight, bias, weight_p, bias_p, drows, both,
+                                                            ctx.needs_input_grad[2:7])
         return None, None, d_jagged, d_w, d_b, d_wp, d_bp
 
 
@@ -451,3 +459,98 @@ def topk_gates(scores: torch.Tensor, k: int):
 
 def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class NormAdd(torch.autograd.Function):
+    """block_norm, block_norm_add and mul_merge_k_norm_add (reverse_index is None or not): (out, next).  The rows' sums are
+    kept from the forward pass, everything else is made again from y and the residual."""
+
+    @staticmethod
+    def forward(ctx, index, reverse_index, merge_index, merge, y, residual, weight, bias, gate, scale, next_weight, next_bias, gate_sigmoid, eps, norm):
+        args = ops.NormArgs(weight, bias, gate, gate_sigmoid, scale, next_weight, next_bias, eps, norm)
+        out, nxt, merged, stats = ops.norm_add(y, residual, args, reverse_index, merge, merge_index, for_backward=True)
+        tensor = isinstance(scale, torch.Tensor)
+        ctx.save_for_backward(index, merge_index, merge, y, merged, residual, weight, bias, gate, scale if tensor else None, next_weight, next_bias, stats)
+        ctx.rest = (gate_sigmoid, None if tensor else scale, eps, norm, 0 if reverse_index is None else reverse_index.shape[1])
+        ctx.set_materialize_grads(False)
+        return out, nxt
+
+    @staticmethod
+    def backward(ctx, d_out, d_next):
+        index, merge_index, merge, y, merged, residual, weight, bias, gate, scale, next_weight, next_bias, stats = ctx.saved_tensors
+        gate_sigmoid, value, eps, norm, K = ctx.rest
+        if d_out is None and d_next is None:
+            return (None,) * 15
+        args = ops.NormArgs(weight, bias, gate, gate_sigmoid, value if scale is None else scale, next_weight, next_bias, eps, norm)
+        names = ("merge", "y", "residual", "weight", "bias", "gate", "scale", "next_weight", "next_bias")
+        need = dict(zip(names, ctx.needs_input_grad[3:12]))
+        rows = need["y"], need["merge"]
+        need["y"] = need["y"] or need["merge"]
+        grads = ops.norm_add_bwd(merged if K else y, residual, args, stats, d_out, d_next, need)
+        d_merge, d_y = None, grads["y"]
+        if K and d_y is not None:
+            d_y, d_gate = ops.combine_bwd(d_y, y, index, K, merge, merge_index, need_gate_grad=rows[1])
+            if rows[1]:
+                d_merge = d_gate.view(merge.shape).to(merge.dtype)
+        return (None, None, None, d_merge, d_y if rows[0] else None, *(grads[n] for n in names[2:]), None, None, None)
+
+
+class SwigluBlockCheckpoint8(torch.autograd.Function):
+    """fused_jagged_bmm_swiglu_combine(checkpoint_bits=8): the expert block whose pre-activations are kept in 8 bits and nothing
+    else of its rows (2 H + H / 16 bytes a routed row in place of 6 H + 2 D_out in bf16); hidden rows, and with them the
+    gate gradient and the operand of the down projection's weight gradient, come from the codes in the backward pass.
+
+    With dr the gradient of a token's output in its routed rows' order, unweighted: d_h = dr W_out^T; the gate gradient is
+    <expert row, dr> = <h, d_h> + <bias_out, dr>; the weights of the rows go into h and the pre-activations' gradients."""
+
+    @staticmethod
+    def forward(ctx, offsets, index, jagged, weight, bias, weight_p, bias_p, weight_out, bias_out, gates, gates_index, reverse_index):
+        R, K = index.numel(), index.shape[1]
+        out_dtype = torch.float32 if jagged.dtype == torch.float32 else torch.bfloat16
+        pre = tuple(torch.empty((R, weight.shape[2]), dtype=out_dtype, device=jagged.device) for _ in range(2))
+        hidden = ops.grouped_gemm(offsets, jagged, weight, total_rows=R, row_index=index, index_div=K, bias=bias, b2=weight_p, bias2=bias_p,
+                                  epilogue=EPI_SWIGLU, aux=pre)
+        kept = ops.swiglu_checkpoint(*pre)
+        del pre
+        value = ops.grouped_gemm(offsets, hidden, weight_out, total_rows=R, bias=bias_out, epilogue=EPI_NONE)
+        ctx.save_for_backward(offsets, index, jagged, weight, bias, weight_p, bias_p, weight_out, bias_out, gates, gates_index, kept.q, kept.e)
+        ctx.kept = kept.cols, kept.dtype
+        return ops.combine(value, reverse_index, gates, gates_index)
+
+    @staticmethod
+    def backward(ctx, dy):
+        offsets, index, jagged, weight, bias, weight_p, bias_p, weight_out, bias_out, gates, gates_index, q, e = ctx.saved_tensors
+        kept = ops.SwigluCheckpoint(q, e, *ctx.kept)
+        K, need = index.shape[1], ctx.needs_input_grad
+        dy = dy.to(kept.dtype).contiguous()
+        flat = index.reshape(-1)
+        need_g = gates is not None and need[9]
+        dr = ops.gather_rows(dy, flat, K) if ops.gather_takes(dy) else dy[torch.div(flat, K, rounding_mode="floor")]
+        row_weight = None
+        if gates is not None:
+            row_weight = gates.reshape(-1) if gates_index is None else gates.reshape(-1)[gates_index.reshape(-1)]
+        d_h = ops.input_grad_gemm(offsets, dr, weight_out.permute(0, 2, 1))
+        joint = kept.dtype == torch.bfloat16 and kept.cols % 8 == 0
+        dg, du, h, dots = ops.swiglu_checkpoint_bwd(kept, d_h, row_weight, joint=joint, need_dots=need_g)
+        del d_h
+        d_wo = d_bo = d_gates = None
+        if need[7]:
+            d_wo = _WgradOperand(h, offsets, flat.numel()).weight_grad(dr, weight_out)
+        if bias_out is not None and (need[8] or need_g):
+            token = torch.div(flat, K, rounding_mode="floor")
+            lengths = (offsets[1:] - offsets[:-1]).clamp_min(0)
+            expert = torch.repeat_interleave(torch.arange(lengths.numel(), device=flat.device), lengths, output_size=flat.numel())
+            d_value, d_flat = ops.combine_bwd(dy, bias_out[expert] if need_g else None, token, K, gates, gates_index, need_gate_grad=need_g)
+            if need[8]:
+                d_bo = ops.segment_colsum(d_value, offsets)
+            if need_g:
+                d_gates = d_flat
+        if need_g:
+            if gates_index is not None:
+                ordered = torch.empty_like(dots)
+                ordered[gates_index.reshape(-1)] = dots
+                dots = ordered
+            d_gates = (dots if d_gates is None else dots + d_gates).view(gates.shape).to(gates.dtype)
+        d_jagged, d_w, d_b, d_wp, d_bp = _gather_gemm_grads(offsets, index, jagged, weight, bias, weight_p, bias_p, [dg, du],
+                                                            ops.joint_rows(dg, du), need[2:7])
+        return None, None, d_jagged, d_w, d_b, d_wp, d_bp, d_wo, d_bo, d_gates, None, None

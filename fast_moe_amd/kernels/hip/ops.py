@@ -7,12 +7,12 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
-from typing import Dict, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import EPI_GATED, EPI_NONE, EPI_SILU, EPI_SWIGLU, FMOE_BF16, FMOE_E4M3, FMOE_F32, FewDesc, GemmDesc
+from ._lib import EPI_GATED, EPI_NONE, EPI_SILU, EPI_SWIGLU, FMOE_BF16, FMOE_E4M3, FMOE_F32, FewDesc, GemmDesc, NormDesc
 
 _DTYPE_CODE = {torch.float32: FMOE_F32, torch.bfloat16: FMOE_BF16}
 FP8_DTYPE = torch.float8_e4m3fn
@@ -921,3 +921,233 @@ def few_tokens(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias: Optional[t
 def _plain_rows(t: torch.Tensor) -> torch.Tensor:
     """A 2-D t with contiguous rows that do not overlap."""
     return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+# ------------------------------------------------- norms around an expert block
+NORM_COLS = 8192        # most columns of fmoe_norm_add
+_NORMS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
+
+
+class NormArgs(NamedTuple):
+    """The operands of norm_add beside y and the residual."""
+    weight: Optional[torch.Tensor] = None
+    bias: Optional[torch.Tensor] = None
+    gate: Optional[torch.Tensor] = None
+    gate_sigmoid: bool = False
+    scale: Union[torch.Tensor, float, None] = None
+    next_weight: Optional[torch.Tensor] = None
+    next_bias: Optional[torch.Tensor] = None
+    eps: float = 1e-6
+    norm: str = "rms"
+
+
+def _norm_desc(name: str, y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, rows_of_y: int) -> Tuple[NormDesc, list]:
+    """The descriptor of a call, checked, and the tensors that have to live as long as it (copies among them)."""
+    scale = a.scale if isinstance(a.scale, torch.Tensor) else None
+    _need_cuda(name, residual, y, a.weight, a.bias, a.gate, scale, a.next_weight, a.next_bias)
+    if residual.dtype not in _DTYPE_CODE:
+        raise NotImplementedError(f"{name}: the HIP kernels take bf16 or fp32 rows, got {residual.dtype}")
+    if a.norm not in _NORMS:
+        raise ValueError(f"{name}: norm must be 'rms' or 'layer', got {a.norm!r}")
+    if residual.ndim != 2:
+        raise ValueError(f"{name}: rows must be [T, D], got {tuple(residual.shape)}")
+    T, D = residual.shape
+    if not 1 <= D <= NORM_COLS:
+        raise ValueError(f"{name}: takes 1 to {NORM_COLS} columns, got {D}")
+    if y is not None and (y.dtype != residual.dtype or tuple(y.shape) != (rows_of_y, D)):
+        raise ValueError(f"{name}: y must be {residual.dtype} [{rows_of_y}, {D}], got {y.dtype} {tuple(y.shape)}")
+    params = [("weight", a.weight), ("bias", a.bias), ("scale", scale), ("next_weight", a.next_weight), ("next_bias", a.next_bias)]
+    given = [t for _, t in params if t is not None]
+    for what, t in params:
+        if t is not None and (t.dtype not in _DTYPE_CODE or t.dtype != given[0].dtype or tuple(t.shape) != (D,)):
+            raise ValueError(f"{name}: {what} must be [{D}], in the one dtype (bf16 or fp32) of all of scale, weights and biases, got "
+                             f"{t.dtype} {tuple(t.shape)}")
+    if (a.bias is not None and a.weight is None) or (a.next_bias is not None and a.next_weight is None):
+        raise ValueError(f"{name}: a bias goes with its weight")
+    if y is None and a.next_weight is None:
+        raise ValueError(f"{name}: nothing to compute")
+    keep = [None if t is None else t.contiguous() for _, t in params]
+    d = NormDesc()
+    d.rows, d.cols, d.dtype, d.norm = T, D, _DTYPE_CODE[residual.dtype], _NORMS[a.norm]
+    d.param_dtype = _DTYPE_CODE[given[0].dtype] if given else d.dtype
+    d.eps, d.scale_value = a.eps, 1.0 if scale is not None or a.scale is None else float(a.scale)
+    d.weight, d.bias, d.scale, d.next_weight, d.next_bias = (_ptr(t) for t in keep)
+    residual = _plain_rows(residual)
+    d.residual, d.residual_stride = residual.data_ptr(), residual.stride(0)
+    keep.append(residual)
+    if y is not None:
+        y = _plain_rows(y)
+        d.y, d.y_stride = y.data_ptr(), y.stride(0)
+        keep.append(y)
+    if a.gate is not None:
+        gate = a.gate
+        if gate.dtype != residual.dtype or tuple(gate.shape) not in ((T,), (T, 1), (T, D)):
+            raise ValueError(f"{name}: gate must be {residual.dtype} [{T}], [{T}, 1] or [{T}, {D}], got {gate.dtype} {tuple(gate.shape)}")
+        if y is None:
+            raise ValueError(f"{name}: a gate goes with y")
+        element = gate.ndim == 2 and gate.shape[1] == D and D > 1
+        if element:
+            gate = _plain_rows(gate)
+        elif gate.stride(0) < 0 or (gate.stride(0) == 0 and T > 1):
+            gate = gate.contiguous()
+        d.gate_mode = _lib.ROW_GATE_ELEMENT if element else _lib.ROW_GATE_TOKEN
+        d.gate, d.gate_stride, d.gate_sigmoid = gate.data_ptr(), gate.stride(0), int(bool(a.gate_sigmoid))
+        keep.append(gate)
+    return d, keep
+
+
+def norm_add(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, reverse_index: Optional[torch.Tensor] = None,
+             merge: Optional[torch.Tensor] = None, merge_index: Optional[torch.Tensor] = None, for_backward: bool = False):
+    """-> (out, next, y, stats), see fmoe_norm_add; ``y`` is the merged one and it and ``stats`` are None unless ``for_backward``."""
+    name = "norm_add"
+    T = residual.shape[0] if residual.ndim else 0
+    K = 0
+    if reverse_index is not None:
+        _need_cuda(name, residual, reverse_index, merge, merge_index)
+        if reverse_index.ndim != 2 or reverse_index.shape[0] != T or not 1 <= reverse_index.shape[1] <= 64:
+            raise ValueError(f"{name}: reverse_index must be [{T}, K] with K <= 64, got {tuple(reverse_index.shape)}")
+        K = reverse_index.shape[1]
+    d, keep = _norm_desc(name, y, residual, a, T * K if K else T)
+    new = lambda: torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+    out = new() if y is not None else None
+    nxt = new() if a.next_weight is not None else None
+    merged = stats = None
+    if K:
+        reverse_index = _i64("reverse_index", reverse_index)
+        d.K, d.value_rows, d.reverse_index = K, T * K, reverse_index.data_ptr()
+        if merge is not None:
+            if merge.dtype not in _DTYPE_CODE or merge.numel() != T * K:
+                raise ValueError(f"{name}: the merge weights must be bf16 or fp32 with {T * K} entries")
+            merge = merge.contiguous()
+            d.merge, d.merge_dtype = merge.data_ptr(), _DTYPE_CODE[merge.dtype]
+            if merge_index is not None:
+                merge_index = _i64("merge_index", merge_index)
+                if merge_index.numel() != T * K:
+                    raise ValueError(f"{name}: merge_index must have {T * K} entries")
+                d.merge_index = merge_index.data_ptr()
+    if for_backward:
+        merged = new() if K else None
+        stats = torch.empty((T, 4), dtype=torch.float32, device=residual.device)
+    d.out, d.next, d.y_out, d.stats = _ptr(out), _ptr(nxt), _ptr(merged), _ptr(stats)
+    if T:
+        with _on_device(residual):
+            rc = _lib.load().fmoe_norm_add(ctypes.byref(d), _stream(residual))
+        _lib.check(rc, "fmoe_norm_add")
+    return out, nxt, merged, stats
+
+
+def norm_add_bwd(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, stats: torch.Tensor, d_out: Optional[torch.Tensor],
+                 d_next: Optional[torch.Tensor], need: Dict[str, bool]) -> Dict[str, Optional[torch.Tensor]]:
+    """Gradients of norm_add by operand name (those ``need`` asks for), see fmoe_norm_add_bwd."""
+    d, keep = _norm_desc("norm_add_bwd", y, residual, a, residual.shape[0])
+    T, D = residual.shape
+    rows = lambda t: None if t is None else t.to(residual.dtype).contiguous()
+    d_out, d_next = rows(d_out), rows(d_next)
+    d.stats, d.d_out, d.d_next = stats.data_ptr(), _ptr(d_out), _ptr(d_next)
+    grads = {}
+    like = {"y": residual, "residual": residual, "gate": a.gate, "scale": a.scale, "weight": a.weight, "bias": a.bias,
+            "next_weight": a.next_weight, "next_bias": a.next_bias}
+    for n, t in like.items():
+        grads[n] = torch.empty(t.shape, dtype=t.dtype, device=residual.device) if need.get(n) else None
+        if n.startswith("next") and need.get(n) and d_next is None:
+            grads[n].zero_()
+            continue
+        setattr(d, "d_" + n, _ptr(grads[n]))
+    if T == 0:
+        for n in ("scale", "weight", "bias", "next_weight", "next_bias"):
+            if grads[n] is not None:
+                grads[n].zero_()
+        return grads
+    lib = _lib.load()
+    with _on_device(residual):
+        ws_bytes = lib.fmoe_norm_add_bwd_workspace_bytes(ctypes.byref(d))
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=residual.device) if ws_bytes else None
+        rc = lib.fmoe_norm_add_bwd(ctypes.byref(d), _ptr(ws), ws_bytes, _stream(residual))
+    _lib.check(rc, "fmoe_norm_add_bwd")
+    return grads
+
+
+# ------------------------------------------------- activation checkpoints in 8 bits
+class SwigluCheckpoint(NamedTuple):
+    """The two pre-activations [R, H] of a SwiGLU expert block in 8 bits (fmoe_swiglu_checkpoint): ``q`` int8 [R, 2, P] codes
+    with P = H in whole blocks of 32, ``e`` uint8 [R, 2, P / 32] biased exponents of the blocks, the ``cols`` = H and the
+    dtype that they had."""
+    q: torch.Tensor
+    e: torch.Tensor
+    cols: int
+    dtype: torch.dtype
+
+
+def _check_kept(name: str, kept: SwigluCheckpoint) -> Tuple[torch.Tensor, torch.Tensor]:
+    q, e, H, dtype = kept
+    _need_cuda(name, q, e)
+    P = (H + 31) // 32 * 32
+    if (dtype not in _DTYPE_CODE or q.dtype != torch.int8 or e.dtype != torch.uint8 or q.ndim != 3 or tuple(q.shape[1:]) != (2, P) or H < 1
+            or tuple(e.shape) != (q.shape[0], 2, P // 32)):
+        raise ValueError(f"{name}: a checkpoint is int8 [R, 2, P] codes and uint8 [R, 2, P / 32] exponents with P = {P} for {H} columns, got "
+                         f"{q.dtype} {tuple(q.shape)} and {e.dtype} {tuple(e.shape)} of {dtype}")
+    q = q.contiguous()
+    return (q if q.data_ptr() % 16 == 0 else q.clone()), e.contiguous()
+
+
+def swiglu_checkpoint(g: torch.Tensor, u: torch.Tensor) -> SwigluCheckpoint:
+    name = "checkpoint_swiglu"
+    dev = _need_cuda(name, g, u)
+    if g.dtype not in _DTYPE_CODE:
+        raise NotImplementedError(f"{name}: the HIP kernels take bf16 or fp32, got {g.dtype}")
+    if g.ndim != 2 or u.shape != g.shape or u.dtype != g.dtype or g.shape[1] < 1:
+        raise ValueError(f"{name}: two [R, H] tensors of one dtype expected, got {g.dtype} {tuple(g.shape)} and {u.dtype} {tuple(u.shape)}")
+    R, H = g.shape
+    P = (H + 31) // 32 * 32
+    q = torch.empty((R, 2, P), dtype=torch.int8, device=dev)
+    e = torch.empty((R, 2, P // 32), dtype=torch.uint8, device=dev)
+    if R:
+        g, u = _plain_rows(g), _plain_rows(u)
+        with _on_device(g):
+            rc = _lib.load().fmoe_swiglu_checkpoint(g.data_ptr(), u.data_ptr(), _DTYPE_CODE[g.dtype], R, H, max(g.stride(0), H),
+                                                    max(u.stride(0), H), q.data_ptr(), e.data_ptr(), _stream(g))
+        _lib.check(rc, "fmoe_swiglu_checkpoint")
+    return SwigluCheckpoint(q, e, H, g.dtype)
+
+
+def swiglu_checkpoint_read(kept: SwigluCheckpoint) -> Tuple[torch.Tensor, torch.Tensor]:
+    q, e = _check_kept("read_checkpoint", kept)
+    R, H = q.shape[0], kept.cols
+    g, u = (torch.empty((R, H), dtype=kept.dtype, device=q.device) for _ in range(2))
+    if R:
+        with _on_device(q):
+            rc = _lib.load().fmoe_swiglu_checkpoint_read(q.data_ptr(), e.data_ptr(), g.data_ptr(), u.data_ptr(), _DTYPE_CODE[kept.dtype], R, H,
+                                                         H, H, _stream(q))
+        _lib.check(rc, "fmoe_swiglu_checkpoint_read")
+    return g, u
+
+
+def swiglu_checkpoint_bwd(kept: SwigluCheckpoint, d: torch.Tensor, weight: Optional[torch.Tensor] = None, joint: bool = False,
+                          need_dots: bool = True):
+    """-> (dg, du, h, dots), see fmoe_swiglu_checkpoint_bwd.  ``joint``: dg and du are the halves of one buffer, as
+    ``swiglu_bwd(joint=True)`` returns them; all have SLACK_ROWS behind them."""
+    name = "swiglu_checkpoint_bwd"
+    q, e = _check_kept(name, kept)
+    R, H = q.shape[0], kept.cols
+    _need_cuda(name, q, d, weight)
+    if d.dtype != kept.dtype or tuple(d.shape) != (R, H):
+        raise ValueError(f"{name}: the gradient must be {kept.dtype} [{R}, {H}], got {d.dtype} {tuple(d.shape)}")
+    if weight is not None and (weight.dtype not in _DTYPE_CODE or weight.numel() != R):
+        raise ValueError(f"{name}: the rows' weights must be bf16 or fp32 with {R} entries, got {weight.dtype} {tuple(weight.shape)}")
+    if joint:
+        both = empty_rows(R, 2 * H, kept.dtype, q.device)
+        dg, du = both[:, :H], both[:, H:]
+    else:
+        dg, du = empty_rows(R, H, kept.dtype, q.device), empty_rows(R, H, kept.dtype, q.device)
+    h = empty_rows(R, H, kept.dtype, q.device)
+    dots = torch.empty((R,), dtype=torch.float32, device=q.device) if need_dots else None
+    if R:
+        d = _plain_rows(d)
+        weight = None if weight is None else weight.contiguous()
+        with _on_device(q):
+            rc = _lib.load().fmoe_swiglu_checkpoint_bwd(
+                q.data_ptr(), e.data_ptr(), d.data_ptr(), _DTYPE_CODE[kept.dtype], R, H, max(d.stride(0), H), _ptr(weight),
+                _DTYPE_CODE[weight.dtype] if weight is not None else 0, dg.data_ptr(), du.data_ptr(), dg.stride(0), h.data_ptr(), h.stride(0),
+                _ptr(dots), _stream(q))
+        _lib.check(rc, "fmoe_swiglu_checkpoint_bwd")
+    return dg, du, h, dots

@@ -16,7 +16,7 @@ of /root/reference/kernels/moe.py:39-292.  Differences, all on purpose:
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -222,13 +222,25 @@ def fused_jagged_bmm_swiglu_combine(
     gates: Optional[torch.Tensor] = None,
     gates_index: Optional[torch.Tensor] = None,
     kernel: KernelType = KernelType.HIP,
+    *,
+    checkpoint_bits: Optional[int] = None,
 ) -> torch.Tensor:
     """kernels/pytorch/moe.py:306-391 (pytorch_fused_jagged_bmm_swiglu_combine): the whole expert
     block of a SwiGLU MoE, ``merge_k(gates * ((silu(x W + b) * (x Wp + bp)) W_out + b_out))`` ->
     [L, D].  Three launches (gather + SwiGLU GEMM, down GEMM, merge); differentiable through the
-    two operators it is made of."""
+    two operators it is made of.  ``checkpoint_bits=8``: the same values, but only the two pre-activations
+    are kept for the backward pass, in 8 bits (``checkpoint_swiglu``), and the gradients are those of what the codes
+    stand for: a third to a quarter of the memory, at errors of up to 1 / 128 of the largest of 32 neighbours."""
     require_hip_kernel(kernel, "fused_jagged_bmm_swiglu_combine")
     assert index.ndim == 2 and index.shape[1] == k, f"{index.shape=}, {k=}"
+    if checkpoint_bits not in (None, 8):
+        raise ValueError(f"fused_jagged_bmm_swiglu_combine: checkpoint_bits must be None or 8, got {checkpoint_bits}")
+    if checkpoint_bits and _ag.needs_grad(jagged, weight, bias, weight_p, bias_p, weight_out, bias_out, gates):
+        _check_gather_args("fused_jagged_bmm_swiglu_combine", index, jagged, weight)
+        if weight_p.stride() != weight.stride():
+            weight, weight_p = weight.contiguous(), weight_p.contiguous()
+        return _ag.SwigluBlockCheckpoint8.apply(offsets, index, jagged, weight, bias, weight_p, bias_p, weight_out, bias_out, gates, gates_index,
+                                                ops.invert_index(index))
     hidden = index_select_jagged_bmm_swiglu(0, offsets, index, jagged, weight, bias, weight_p, bias_p, kernel)
     token_index = torch.div(index.reshape(-1), k, rounding_mode="floor")
     reverse_index = ops.invert_index(index)
@@ -264,3 +276,82 @@ def fused_moe_few_tokens(
     require_hip_kernel(kernel, "fused_moe_few_tokens")
     ops._forward_only("fused_moe_few_tokens", x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out)
     return ops.few_tokens(x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out, k, renorm, token_mask)
+
+
+# ------------------------------------------------------------ around the expert block
+def _norm_call(index, reverse_index, merge_index, merge, y, residual, args: ops.NormArgs):
+    tensors = [merge, y, residual, *args[:3], args.scale if isinstance(args.scale, torch.Tensor) else None, args.next_weight, args.next_bias]
+    if _ag.needs_grad(*tensors):
+        return _ag.NormAdd.apply(index, reverse_index, merge_index, merge, y, residual, args.weight, args.bias, args.gate, args.scale,
+                                 args.next_weight, args.next_bias, args.gate_sigmoid, args.eps, args.norm)
+    return ops.norm_add(y, residual, args, reverse_index, merge, merge_index)[:2]
+
+
+def block_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, eps: float = 1e-6, norm: str = "rms",
+               kernel: KernelType = KernelType.HIP) -> torch.Tensor:
+    """The norm before the first block: ``norm(x) * weight + bias`` over the last dimension of x [T, D] (bf16 or fp32, up to 8192
+    columns), ``norm`` = "rms" or "layer"; fp32 inside, rounded once.  Differentiable.  No counterpart in the reference."""
+    require_hip_kernel(kernel, "block_norm")
+    return _norm_call(None, None, None, None, None, x, ops.NormArgs(next_weight=weight, next_bias=bias, eps=eps, norm=norm))[1]
+
+
+def block_norm_add(y: torch.Tensor, residual: torch.Tensor, *, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                   gate: Optional[torch.Tensor] = None, gate_sigmoid: bool = False, scale: Union[torch.Tensor, float, None] = None,
+                   next_weight: Optional[torch.Tensor] = None, next_bias: Optional[torch.Tensor] = None, eps: float = 1e-6, norm: str = "rms",
+                   kernel: KernelType = KernelType.HIP) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Between two blocks: ``out = residual + scale * gate * (norm(y) * weight + bias)`` and ``next = norm(out) * next_weight + next_bias``,
+    in one pass; returns (out, next), next None without ``next_weight``.  y, residual [T, D] of one dtype (bf16 or fp32, up to 8192
+    columns).  Without ``weight`` y is not normed.  ``gate``: [T] or [T, 1] (a gate per token) or [T, D], in their dtype, behind a sigmoid
+    with ``gate_sigmoid``.  ``scale``: [D] or a number.  scale, weights and biases share one dtype, bf16 or fp32.  fp32 inside, each output
+    rounded once, ``next`` from the unrounded out.  Differentiable in every tensor.  No counterpart in the reference."""
+    require_hip_kernel(kernel, "block_norm_add")
+    return _norm_call(None, None, None, None, y, residual,
+                      ops.NormArgs(weight, bias, gate, gate_sigmoid, scale, next_weight, next_bias, eps, norm))
+
+
+def mul_merge_k_norm_add(index: torch.Tensor, reverse_index: torch.Tensor, value: torch.Tensor, residual: torch.Tensor,
+                         merge_weight: Optional[torch.Tensor] = None, weight_index: Optional[torch.Tensor] = None, *,
+                         weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                         gate_sigmoid: bool = False, scale: Union[torch.Tensor, float, None] = None,
+                         next_weight: Optional[torch.Tensor] = None, next_bias: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                         norm: str = "rms", kernel: KernelType = KernelType.HIP) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``block_norm_add`` of the merge of an expert block's rows, without the merged rows' round trip: y is
+    ``mul_merge_k_add(index, reverse_index, value, weight=merge_weight, weight_index=weight_index)`` (index: the token of every row),
+    summed in fp32 and not rounded.  For the backward pass the merged rows are kept in value's dtype."""
+    require_hip_kernel(kernel, "mul_merge_k_norm_add")
+    N = index.shape[0]
+    L, K = reverse_index.shape
+    assert index.ndim == 1 and N == L * K and N == value.shape[0] and L == residual.shape[0], (
+        f"mul_merge_k_norm_add: {index.shape=}, {reverse_index.shape=}, {value.shape=}, {residual.shape=}")
+    assert merge_weight is None or (weight_index is not None and merge_weight.numel() == weight_index.numel() == N), (
+        "mul_merge_k_norm_add: merge_weight and weight_index need an entry per row")
+    return _norm_call(index, reverse_index, weight_index, merge_weight, value, residual,
+                      ops.NormArgs(weight, bias, gate, gate_sigmoid, scale, next_weight, next_bias, eps, norm))
+
+
+# ------------------------------------------------------- activation checkpoints in 8 bits
+SwigluCheckpoint = ops.SwigluCheckpoint
+
+
+def checkpoint_swiglu(gate: torch.Tensor, up: torch.Tensor, kernel: KernelType = KernelType.HIP) -> SwigluCheckpoint:
+    """The two pre-activations [R, H] of a SwiGLU expert block (bf16 or fp32) in 8 bits: blocks of 32 neighbours under a shared power of
+    two (MXINT8), 33 / 32 bytes a value.  A block holding an infinity or NaN reads as NaN.  Forward only (what it keeps stands in for the
+    saved tensors of a backward pass).  No counterpart in the reference, which keeps both in their own dtype."""
+    require_hip_kernel(kernel, "checkpoint_swiglu")
+    ops._forward_only("checkpoint_swiglu", gate, up)
+    return ops.swiglu_checkpoint(gate, up)
+
+
+def read_checkpoint(kept: SwigluCheckpoint, kernel: KernelType = KernelType.HIP) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(gate, up) that the codes stand for, in the dtype they had; exact in bf16."""
+    require_hip_kernel(kernel, "read_checkpoint")
+    return ops.swiglu_checkpoint_read(kept)
+
+
+def swiglu_checkpoint_bwd(kept: SwigluCheckpoint, d_hidden: torch.Tensor, row_weight: Optional[torch.Tensor] = None,
+                          kernel: KernelType = KernelType.HIP) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Backward of ``w * silu(gate) * up`` from the checkpoint, in one pass: d_hidden [R, H] is the gradient of the hidden rows behind the
+    rows' weights w ([R], bf16 or fp32; None: 1).  -> (d_gate, d_up, w * hidden, d_w fp32 [R])."""
+    require_hip_kernel(kernel, "swiglu_checkpoint_bwd")
+    ops._forward_only("swiglu_checkpoint_bwd", d_hidden, row_weight)
+    return ops.swiglu_checkpoint_bwd(kept, d_hidden, row_weight)

@@ -551,6 +551,75 @@ int fmoe_combine_bwd(const void* dy, const void* value, int value_dtype, int64_t
                      int64_t gates_stride_col, const int64_t* gates_index, void* d_value,
                      float* d_gates, fmoe_stream_t stream);
 
+/* ------------------------------------------- norms around an expert block */
+
+/*
+ * What stands before and behind an expert block in a pre- and post-normed transformer layer, in one pass over the rows (no counterpart in
+ * the reference, whose SGMoE layer calls torch's norms, kernels/tests/mrn_test.py:330-368):
+ *   z = norm(y) * weight + bias,  out = residual + scale * gate * z,  next = norm(out) * next_weight + next_bias
+ * norm: rms (v / sqrt(mean(v^2) + eps)) or layer norm ((v - mean) / sqrt(var + eps)); everything in fp32 from the loads to the one rounding
+ * of each output (next is the norm of the unrounded out).  Optional parts:
+ *   y NULL: only next = norm(residual);  weight NULL: z = y;  next_weight / next NULL: no next
+ *   K > 0: y [rows * K, cols] are the routed rows of an expert block, merged as fmoe_combine merges them (reverse_index [rows, K]; weight of
+ *          row r: merge[merge_index ? merge_index[r] : r], 1 if merge is NULL; indices outside [0, rows * K) are left out), in fp32
+ *   gate:  one per row (FMOE_GATE_TOKEN, gate[row * gate_stride]) or per element, raw or behind a sigmoid
+ *   scale: [cols], or scale_value where it is NULL
+ *   y_out [rows, cols]: receives the merged y;  stats [rows, 4] fp32: the rows' means and reciprocals, what the backward pass wants
+ * dtype: FMOE_BF16 or FMOE_F32 for y, residual, gate, outputs and their gradients; param_dtype: either, for scale, weights and biases.
+ * Outputs, y_out, gradients and merge are contiguous; up to 8192 columns.
+ * Backward (y merged already, K = 0): d_out and d_next (either may be NULL) -> every gradient whose pointer is set: d_y, d_residual [rows,
+ * cols], d_gate (per row contiguous, or [rows, cols]), d_scale, d_weight, d_bias, d_next_weight, d_next_bias [cols] in param_dtype, which take
+ * a workspace: their sums over rows are added in a fixed order.
+ */
+enum fmoe_norm_kind { FMOE_NORM_RMS = 0, FMOE_NORM_LAYER = 1 };
+enum fmoe_gate_mode { FMOE_GATE_NONE = 0, FMOE_GATE_TOKEN = 1, FMOE_GATE_ELEMENT = 2 };
+typedef struct fmoe_norm_desc {
+    int64_t rows;
+    int32_t cols, dtype, param_dtype, norm, gate_mode, gate_sigmoid;
+    float eps, scale_value;
+    const void* y;
+    int64_t y_stride;
+    int32_t K, merge_dtype;
+    int64_t value_rows;             /* rows * K                    */
+    const int64_t* reverse_index;
+    const void* merge;
+    const int64_t* merge_index;
+    const void* residual;
+    int64_t residual_stride;
+    const void* gate;
+    int64_t gate_stride;
+    const void *scale, *weight, *bias, *next_weight, *next_bias;
+    void *out, *next, *y_out;
+    float* stats;
+    const void *d_out, *d_next;
+    void *d_y, *d_residual, *d_gate, *d_scale, *d_weight, *d_bias, *d_next_weight, *d_next_bias;
+} fmoe_norm_desc;
+int fmoe_norm_add(const fmoe_norm_desc* desc /* host pointer */, fmoe_stream_t stream);
+size_t fmoe_norm_add_bwd_workspace_bytes(const fmoe_norm_desc* desc /* host pointer */);
+int fmoe_norm_add_bwd(const fmoe_norm_desc* desc /* host pointer */, void* workspace, size_t workspace_bytes, fmoe_stream_t stream);
+
+/* ------------------------------------------- activation checkpoints in 8 bits */
+
+/*
+ * The two pre-activations g, u [rows, cols] of a SwiGLU expert block in 8 bits between forward and backward (the reference keeps both in
+ * their own type, kernels/triton/triton_moe.py:2316-2345): blocks of 32 neighbours of a row under a shared power of two X = 2^floor(log2(largest
+ * magnitude)), codes round(v / X * 64) to nearest even within +-127 (the OCP microscaling format MXINT8).
+ *   q [rows, 2, P] codes (P = fmoe_swiglu_checkpoint_cols(cols): cols in whole blocks, zeros behind them), e [rows, 2, P / 32] biased exponents
+ *   (0: the block is zero or below the normal range; 255: it held an infinity or NaN and reads as NaN).
+ * fmoe_swiglu_checkpoint_bwd, with g', u' what the codes stand for, d [rows, cols] the gradient of the block's hidden rows before their own
+ * weights, w the rows' weights (fp32 or bf16; NULL: 1), s = sigmoid(g'), h = g' s u':
+ *   dg = w d u' (s + g' s (1 - s)),  du = w d g' s     rows at dg_stride_row (the halves of one buffer, say)
+ *   h_out = w h  (NULL: not wanted),  dots[r] = sum over the row of h d  (fp32, the gradient of w; NULL: not wanted)
+ */
+int64_t fmoe_swiglu_checkpoint_cols(int64_t cols);
+int fmoe_swiglu_checkpoint(const void* g, const void* u, int dtype, int64_t rows, int64_t cols, int64_t g_stride_row,
+                           int64_t u_stride_row, int8_t* q, uint8_t* e, fmoe_stream_t stream);
+int fmoe_swiglu_checkpoint_read(const int8_t* q, const uint8_t* e, void* g, void* u, int dtype, int64_t rows, int64_t cols,
+                                int64_t g_stride_row, int64_t u_stride_row, fmoe_stream_t stream);
+int fmoe_swiglu_checkpoint_bwd(const int8_t* q, const uint8_t* e, const void* d, int dtype, int64_t rows, int64_t cols,
+                               int64_t d_stride_row, const void* weight, int weight_dtype, void* dg, void* du,
+                               int64_t dg_stride_row, void* h, int64_t h_stride_row, float* dots, fmoe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
