@@ -18,6 +18,8 @@
 // a row), which leaves the backward pass two exchanges between waves per row in place of four.
 #include "common.h"
 
+#include <type_traits>
+
 namespace fmoe {
 namespace {
 
@@ -36,27 +38,63 @@ __device__ __forceinline__ void from_f32(uint16_t* p, float v) { *p = (uint16_t)
 template <typename E, bool VEC, int CH>
 struct Row {
     static constexpr int V = NE<E>::V, N = V * CH;
+    // what has been loaded and not been looked at: the chunks, or the values
+    struct Raw {
+        u32x4 v[VEC ? CH : 1];
+        E e[VEC ? 1 : N];
+    };
+    // one chunk
+    __device__ __forceinline__ static void unpack(const u32x4& v, float (&f)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (V == 4) f[i] = __uint_as_float(v[i]);
+            else f[i] = i & 1 ? __uint_as_float(v[i / 2] & 0xffff0000u) : __uint_as_float(v[i / 2] << 16);
+        }
+    }
+    __device__ __forceinline__ static void pack(E* p, const float (&f)[V]) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (V == 4) v[i] = __float_as_uint(f[i]);
+            else v[i] = cvt_pk_bf16(f[2 * i], f[2 * i + 1]);
+        }
+        *reinterpret_cast<u32x4*>(p) = v;
+    }
     int tid, threads, cols;
     __device__ __forceinline__ int col(int i) const {
         return VEC ? ((i / V) * threads + tid) * V + i % V : i * threads + tid;
     }
     __device__ __forceinline__ bool in(int i) const { return col(i) < cols; }       // (VEC: all of a chunk or none)
-    __device__ __forceinline__ void load(const E* p, float (&f)[N]) const {
+    __device__ __forceinline__ void fetch(const E* p, Raw& r) const {
         if constexpr (VEC) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                u32x4 v = {0, 0, 0, 0};
-                if (in(c * V)) v = *reinterpret_cast<const u32x4*>(p + col(c * V));
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    if constexpr (V == 4) f[c * V + i] = __uint_as_float(v[i]);
-                    else f[c * V + i] = i & 1 ? __uint_as_float(v[i / 2] & 0xffff0000u) : __uint_as_float(v[i / 2] << 16);
-                }
+                r.v[c] = u32x4{0, 0, 0, 0};
+                if (in(c * V)) r.v[c] = *reinterpret_cast<const u32x4*>(p + col(c * V));
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = in(i) ? to_f32(p[col(i)]) : 0.0f;
+            for (int i = 0; i < N; ++i) r.e[i] = in(i) ? p[col(i)] : E(0);
         }
+    }
+    __device__ __forceinline__ void take(const Raw& r, float (&f)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (!VEC) f[i] = to_f32(r.e[i]);
+            else if constexpr (V == 4) f[i] = __uint_as_float(r.v[i / V][i % V]);
+            else f[i] = i & 1 ? __uint_as_float(r.v[i / V][i % V / 2] & 0xffff0000u) : __uint_as_float(r.v[i / V][i % V / 2] << 16);
+        }
+    }
+    __device__ __forceinline__ void take_chunk(const Raw& r, int c, float (&f)[V]) const {
+        float all[N];
+        take(r, all);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = all[c * V + i];
+    }
+    __device__ __forceinline__ void load(const E* p, float (&f)[N]) const {
+        Raw r;
+        fetch(p, r);
+        take(r, f);
     }
     __device__ __forceinline__ void store(E* p, const float (&f)[N]) const {
         if constexpr (VEC) {
@@ -77,12 +115,31 @@ struct Row {
                 if (in(i)) from_f32(p + col(i), f[i]);
         }
     }
-    // a parameter of the columns, in fp32 or bf16 whatever the rows are
-    __device__ __forceinline__ void param(const void* p, int dtype, float (&f)[N], float none) const {
+    // a parameter of the columns of chunk c, in fp32 or bf16 whatever the rows are
+    __device__ __forceinline__ void param(const void* p, int dtype, int c, float (&f)[V], float none) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            f[i] = none;
-            if (p && in(i)) f[i] = dtype == FMOE_F32 ? reinterpret_cast<const float*>(p)[col(i)] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[col(i)]);
+        for (int i = 0; i < V; ++i) f[i] = none;
+        if (!p) return;
+        if constexpr (VEC) {
+            if (!in(c * V)) return;
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                if (dtype == FMOE_F32) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>((const float*)p + col(c * V) + i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) f[i + j] = v[j];
+                } else {
+                    const u32x2 v = *reinterpret_cast<const u32x2*>((const uint16_t*)p + col(c * V) + i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) f[i + j] = j & 1 ? __uint_as_float(v[j / 2] & 0xffff0000u) : __uint_as_float(v[j / 2] << 16);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int at = col(c * V + i);
+                if (at < cols) f[i] = dtype == FMOE_F32 ? reinterpret_cast<const float*>(p)[at] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[at]);
+            }
         }
     }
     __device__ __forceinline__ void store_f32(float* p, const float (&f)[N]) const {
@@ -151,229 +208,471 @@ __device__ __forceinline__ void row_stats(const R& row, const float (&f)[N], boo
 
 __device__ __forceinline__ float sigmoid_f32(float v) { return 1.0f / (1.0f + expf(-v)); }
 
-template <typename E, bool VEC, int CH>
+// A parameter where it is used: kept in registers over the rows where a lane has one chunk, asked for again (from the L1) where it has more.
+template <typename R, bool KEPT>
+struct Param {
+    static constexpr int V = R::V;
+    const void* p;
+    int dtype;
+    float none, kept[KEPT ? V : 1];
+    __device__ __forceinline__ Param(const R& row, const void* p, int dtype, float none) : p(p), dtype(dtype), none(none) {
+        if constexpr (KEPT) row.param(p, dtype, 0, kept, none);
+    }
+    __device__ __forceinline__ void get(const R& row, int c, float (&f)[V]) const {
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = kept[i];
+        } else {
+            row.param(p, dtype, c, f, none);
+        }
+    }
+};
+
+// MERGE: y is the merge of the token's rows.
+template <typename E, bool VEC, int CH, bool MERGE>
 __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_norm_desc d, int waves) {
     using R = Row<E, VEC, CH>;
-    constexpr int N = R::N;
+    using P = Param<R, CH == 1 && !MERGE>;
+    constexpr int N = R::N, V = R::V, BATCH = 4 / CH;        // rows of a merge on their way
     __shared__ float buf[2][kNormMostWaves][4];
-    const int per = waves == 1 ? blockDim.x / kWave : 1, wave = threadIdx.x / kWave;       // rows of a block at a time
+    const int per = waves == 1 ? blockDim.x / kWave : 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);       // rows of a block at a time
     const R row{waves == 1 ? (int)threadIdx.x % kWave : (int)threadIdx.x, waves * kWave, d.cols};
     Exchange x{buf, waves, wave, 0};
     const bool layer = d.norm == FMOE_NORM_LAYER;
-    float scale[N], weight[N], bias[N], next_w[N], next_b[N];
-    row.param(d.scale, d.param_dtype, scale, d.scale_value);
-    row.param(d.weight, d.param_dtype, weight, 1.0f);
-    row.param(d.bias, d.param_dtype, bias, 0.0f);
-    row.param(d.next_weight, d.param_dtype, next_w, 0.0f);
-    row.param(d.next_bias, d.param_dtype, next_b, 0.0f);
-    for (int64_t t = (int64_t)blockIdx.x * per + (waves == 1 ? wave : 0); t < d.rows; t += (int64_t)gridDim.x * per) {
-        float o[N], y[N], mean = 0.0f, rstd = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
-        row.load((const E*)d.residual + t * d.residual_stride, o);
+    const P scale(row, d.scale, d.param_dtype, d.scale_value), weight(row, d.weight, d.param_dtype, 1.0f), bias(row, d.bias, d.param_dtype, 0.0f),
+        next_weight(row, d.next_weight, d.param_dtype, 0.0f), next_bias(row, d.next_bias, d.param_dtype, 0.0f);
+    // The next row's loads are issued before this row's sums are exchanged.  Of a merge: the numbers and weights of the rows after it (a lane each), then
+    // the first BATCH of the next token's rows.
+    const int64_t first = (int64_t)blockIdx.x * per + (waves == 1 ? wave : 0), step = (int64_t)gridDim.x * per;
+    typename R::Raw ro, ry[MERGE ? BATCH : 1];
+    const int lane = lane_id();
+    int64_t from = -1;
+    float share = 0.0f;
+    auto number = [&](int64_t t) {
+        from = lane < d.K && t < d.rows ? d.reverse_index[t * d.K + lane] : -1;
+        if ((uint64_t)from >= (uint64_t)d.value_rows) from = -1;
+        share = 1.0f;
+        if (from >= 0 && d.merge) {
+            const int64_t at = d.merge_index ? d.merge_index[from] : from;
+            if ((uint64_t)at >= (uint64_t)d.value_rows) from = -1;
+            else share = d.merge_dtype == FMOE_F32 ? reinterpret_cast<const float*>(d.merge)[at] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(d.merge)[at]);
+        }
+    };
+    int from_lo = -1, from_hi = -1, share_bits = 0;         // of the token whose rows are being added
+    auto row_of = [&](int j) {
+        const int at = min(j, d.K - 1);
+        return j < d.K ? (int64_t)__builtin_amdgcn_readlane(from_hi, at) << 32 | (uint32_t)__builtin_amdgcn_readlane(from_lo, at) : -1;
+    };
+    auto fetch_rows = [&](int j0) {
+#pragma unroll
+        for (int j = 0; j < (MERGE ? BATCH : 1); ++j) {
+            const int64_t r = row_of(j0 + j);
+            if (r >= 0) row.fetch((const E*)d.y + r * d.y_stride, ry[j]);
+        }
+    };
+    auto fetch = [&](int64_t t) {
+        if constexpr (MERGE) {
+            from_lo = (int)(uint32_t)from, from_hi = (int)(from >> 32), share_bits = (int)__float_as_uint(share);
+            number(t + step);
+        }
+        if (t >= d.rows) return;
+        row.fetch((const E*)d.residual + t * d.residual_stride, ro);
+        if constexpr (MERGE) fetch_rows(0);
+        else if (d.y) row.fetch((const E*)d.y + t * d.y_stride, ry[0]);
+    };
+    if constexpr (MERGE) number(first);
+    fetch(first);
+    for (int64_t t = first; t < d.rows; t += step) {
+        float o[N], mean = 0.0f, rstd = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
+        row.take(ro, o);
         if (d.y) {
-            if (d.K) {
+            float y[N];
+            if constexpr (MERGE) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) y[i] = 0.0f;
-                for (int j = 0; j < d.K; ++j) {
-                    const int64_t r = d.reverse_index[t * d.K + j];
-                    if ((uint64_t)r >= (uint64_t)d.value_rows) continue;
-                    float w = 1.0f;
-                    if (d.merge) {
-                        const int64_t at = d.merge_index ? d.merge_index[r] : r;
-                        if ((uint64_t)at >= (uint64_t)d.value_rows) continue;
-                        w = d.merge_dtype == FMOE_F32 ? reinterpret_cast<const float*>(d.merge)[at]
-                                                      : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(d.merge)[at]);
-                    }
-                    float v[N];
-                    row.load((const E*)d.y + r * d.y_stride, v);
+                for (int j0 = 0; j0 < d.K; j0 += BATCH) {
+                    if (j0 > 0) fetch_rows(j0);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) y[i] = __builtin_fmaf(w, v[i], y[i]);
+                    for (int j = 0; j < BATCH; ++j) {
+                        if (row_of(j0 + j) < 0) continue;
+                        const float w = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(share_bits, min(j0 + j, d.K - 1)));
+                        float f[N];
+                        row.take(ry[j], f);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) y[i] = __builtin_fmaf(w, f[i], y[i]);
+                    }
                 }
+                fetch(t + step);
                 if (d.y_out) row.store((E*)d.y_out + t * d.cols, y);
             } else {
-                row.load((const E*)d.y + t * d.y_stride, y);
+                row.take(ry[0], y);
+                fetch(t + step);
             }
             if (d.weight) row_stats(row, y, layer, d.eps, x, mean, rstd);
-            float gate[N];
-            if (d.gate_mode == FMOE_GATE_ELEMENT) {
-                row.load((const E*)d.gate + t * d.gate_stride, gate);
-            } else {
-                const float g = d.gate_mode == FMOE_GATE_TOKEN ? to_f32(((const E*)d.gate)[t * d.gate_stride]) : 1.0f;
+            typename R::Raw rg;
+            const bool element = d.gate_mode == FMOE_GATE_ELEMENT;
+            float token = d.gate_mode == FMOE_GATE_TOKEN ? to_f32(((const E*)d.gate)[t * d.gate_stride]) : 1.0f;
+            if (element) row.fetch((const E*)d.gate + t * d.gate_stride, rg);
+            else if (d.gate_mode && d.gate_sigmoid) token = sigmoid_f32(token);
 #pragma unroll
-                for (int i = 0; i < N; ++i) gate[i] = g;
-            }
+            for (int c = 0; c < CH; ++c) {
+                float s[V], w[V], b[V], g[V];
+                scale.get(row, c, s);
+                weight.get(row, c, w);
+                bias.get(row, c, b);
+                if (element) {
+                    row.take_chunk(rg, c, g);
+                    if (d.gate_sigmoid)
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float g = d.gate_mode && d.gate_sigmoid ? sigmoid_f32(gate[i]) : gate[i];
-                const float z = (y[i] - mean) * rstd * weight[i] + bias[i];
-                if (row.in(i)) o[i] += scale[i] * g * z;
+                        for (int i = 0; i < V; ++i) g[i] = sigmoid_f32(g[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) g[i] = token;
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (row.in(c * V + i)) o[c * V + i] += s[i] * g[i] * ((y[c * V + i] - mean) * rstd * w[i] + b[i]);
             }
             if (d.out) row.store((E*)d.out + t * d.cols, o);
+        } else {
+            fetch(t + step);
         }
         if (d.next) {
             row_stats(row, o, layer, d.eps, x, mean2, rstd2);
-            float n[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) n[i] = (o[i] - mean2) * rstd2 * next_w[i] + next_b[i];
-            row.store((E*)d.next + t * d.cols, n);
+            for (int c = 0; c < CH; ++c) {
+                float w[V], b[V];
+                next_weight.get(row, c, w);
+                next_bias.get(row, c, b);
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[c * V + i] = (o[c * V + i] - mean2) * rstd2 * w[i] + b[i];
+            }
+            row.store((E*)d.next + t * d.cols, o);
         }
         if (d.stats && row.tid == 0) *reinterpret_cast<f32x4*>(d.stats + 4 * t) = f32x4{mean, rstd, mean2, rstd2};
     }
 }
 
-// Which of the five sums over rows are asked for, in the order of their partial sums [blocks][5][cols].
-enum { kDScale = 0, kDWeight, kDBias, kDNextWeight, kDNextBias, kSums };
-
-template <typename E, bool VEC, int CH>
-__global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_bwd_kernel(fmoe_norm_desc d, int waves, float* partial) {
-    using R = Row<E, VEC, CH>;
-    constexpr int N = R::N;
+// The merge of expert rows and what follows it where rows are whole 16-byte chunks of the parameters' own kind (P32: fp32 parameters) and a gate is per
+// token: norm_add_kernel<MERGE> without its cases, whose registers (186) let half as many rows be on their way.  A row's waves take BATCH rows of the merge
+// at a time, the first of them while the row before is normed.
+struct MergeParams {
+    int64_t rows, value_rows, y_stride, residual_stride, gate_stride;
+    int32_t cols, K, merge_f32, gate_mode, gate_sigmoid;
+    float eps, scale_value;
+    const void *y, *residual, *gate, *merge, *scale, *weight, *bias, *next_weight, *next_bias;
+    const int64_t *reverse_index, *merge_index;
+    void *out, *next, *y_out;
+    float* stats;
+};
+template <typename E, bool LAYER, bool P32, int BATCH>
+__global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(MergeParams p, int waves) {
+    using R = Row<E, true, 1>;
+    constexpr int V = R::V;
     __shared__ float buf[2][kNormMostWaves][4];
-    const int per = waves == 1 ? blockDim.x / kWave : 1, wave = threadIdx.x / kWave;
+    const int per = waves == 1 ? blockDim.x / kWave : 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+    const R row{waves == 1 ? lane : (int)threadIdx.x, waves * kWave, p.cols};
+    Exchange x{buf, waves, wave, 0};
+    const bool in = row.in(0);
+    const int col = row.col(0);
+    auto param = [&](const void* q, float (&f)[V], float none) {
+        if (q && in) {
+            if constexpr (P32) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] = reinterpret_cast<const float*>(q)[col + i];
+            } else {
+                R::unpack(*reinterpret_cast<const u32x4*>((const uint16_t*)q + col), f);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = none;
+        }
+    };
+    const int64_t first = (int64_t)blockIdx.x * per + (waves == 1 ? wave : 0), step = (int64_t)gridDim.x * per;
+    int64_t from = -1;
+    float share = 0.0f;
+    auto number = [&](int64_t t) {
+        from = lane < p.K && t < p.rows ? p.reverse_index[t * p.K + lane] : -1;
+        if ((uint64_t)from >= (uint64_t)p.value_rows) from = -1;
+        share = 1.0f;
+        if (from >= 0 && p.merge) {
+            const int64_t at = p.merge_index ? p.merge_index[from] : from;
+            if ((uint64_t)at >= (uint64_t)p.value_rows) from = -1;
+            else share = p.merge_f32 ? reinterpret_cast<const float*>(p.merge)[at] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p.merge)[at]);
+        }
+    };
+    int lo = -1, hi = -1, share_bits = 0;
+    u32x4 ro = {0, 0, 0, 0}, ry[BATCH];
+    auto rows = [&](int j0) {
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {       // (a row that is not there: row 0, and left out of the sum)
+            const int at = min(j0 + j, p.K - 1), h = __builtin_amdgcn_readlane(hi, at);
+            const int64_t r = h < 0 ? 0 : (int64_t)h << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, at);
+            ry[j] = u32x4{0, 0, 0, 0};
+            if (in) ry[j] = *reinterpret_cast<const u32x4*>((const E*)p.y + r * p.y_stride + col);
+        }
+    };
+    auto fetch = [&](int64_t t) {
+        lo = (int)(uint32_t)from, hi = (int)(from >> 32), share_bits = (int)__float_as_uint(share);
+        number(t + step);
+        if (t >= p.rows) return;
+        if (in) ro = *reinterpret_cast<const u32x4*>((const E*)p.residual + t * p.residual_stride + col);
+        rows(0);
+    };
+    auto stats = [&](const float (&f)[V], float& mean, float& rstd) { row_stats(row, f, LAYER, p.eps, x, mean, rstd); };
+    number(first);
+    fetch(first);
+    for (int64_t t = first; t < p.rows; t += step) {
+        float y[V], o[V], f[V], g[V], mean = 0.0f, rstd = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[i] = 0.0f;
+        for (int j0 = 0; j0 < p.K; j0 += BATCH) {
+            if (j0 > 0) rows(j0);
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                if (j0 + j >= p.K || __builtin_amdgcn_readlane(hi, min(j0 + j, p.K - 1)) < 0) continue;
+                const float w = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(share_bits, min(j0 + j, p.K - 1)));
+                R::unpack(ry[j], f);
+#pragma unroll
+                for (int i = 0; i < V; ++i) y[i] = __builtin_fmaf(w, f[i], y[i]);
+            }
+        }
+        R::unpack(ro, o);
+        fetch(t + step);
+        if (p.y_out && in) R::pack((E*)p.y_out + t * p.cols + col, y);
+        if (p.weight) stats(y, mean, rstd);
+        float gate = p.gate_mode ? to_f32(((const E*)p.gate)[t * p.gate_stride]) : 1.0f;
+        if (p.gate_sigmoid) gate = sigmoid_f32(gate);
+        param(p.weight, f, 1.0f);
+        param(p.bias, g, 0.0f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[i] = (y[i] - mean) * rstd * f[i] + g[i];
+        param(p.scale, f, p.scale_value);
+        if (in)
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] += f[i] * gate * y[i];
+        if (in) R::pack((E*)p.out + t * p.cols + col, o);
+        if (p.next) {
+            stats(o, mean2, rstd2);
+            param(p.next_weight, f, 0.0f);
+            param(p.next_bias, g, 0.0f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = (o[i] - mean2) * rstd2 * f[i] + g[i];
+            if (in) R::pack((E*)p.next + t * p.cols + col, o);
+        }
+        if (p.stats && row.tid == 0) *reinterpret_cast<f32x4*>(p.stats + 4 * t) = f32x4{mean, rstd, mean2, rstd2};
+    }
+}
+
+// Which of the five sums over rows are asked for, in the order of their partial sums [blocks][5][cols].
+enum { kDScale = 0, kDWeight, kDNextWeight, kDBias, kDNextBias, kSums };
+
+// The next row's loads are issued before this row's sums are exchanged.
+template <typename E, bool VEC, int CH, bool LAYER, bool ELEMENT, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d, int waves, float* partial) {
+    using R = Row<E, VEC, CH>;
+    using P = Param<R, CH == 1>;
+    constexpr int N = R::N, V = R::V, SUMS = LAYER ? kSums : 3;       // rms norm: no biases
+    __shared__ float buf[2][kNormMostWaves][4];
+    const int per = waves == 1 ? blockDim.x / kWave : 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const R row{waves == 1 ? (int)threadIdx.x % kWave : (int)threadIdx.x, waves * kWave, d.cols};
     Exchange x{buf, waves, wave, 0};
-    const bool layer = d.norm == FMOE_NORM_LAYER;
     const float inv = 1.0f / (float)d.cols;
-    float scale[N], weight[N], bias[N], next_w[N], sums[kSums][N];
-    row.param(d.scale, d.param_dtype, scale, d.scale_value);
-    row.param(d.weight, d.param_dtype, weight, 1.0f);
-    row.param(d.bias, d.param_dtype, bias, 0.0f);
-    row.param(d.next_weight, d.param_dtype, next_w, 0.0f);
+    const P scale(row, d.scale, d.param_dtype, d.scale_value), weight(row, d.weight, d.param_dtype, 1.0f), bias(row, LAYER ? d.bias : nullptr, d.param_dtype, 0.0f),
+        next_weight(row, d.next_weight, d.param_dtype, 0.0f);
+    float sums[SUMS][N];
 #pragma unroll
-    for (int s = 0; s < kSums; ++s)
+    for (int s = 0; s < SUMS; ++s)
 #pragma unroll
         for (int i = 0; i < N; ++i) sums[s][i] = 0.0f;
     const int first = blockIdx.x * per + (waves == 1 ? wave : 0);
-    for (int64_t t = first; t < d.rows; t += (int64_t)gridDim.x * per) {
-        const f32x4 st = *reinterpret_cast<const f32x4*>(d.stats + 4 * t);
-        float a[N], o[N], gate[N], dn[N], dt[N];
-        row.load((const E*)d.residual + t * d.residual_stride, o);
-        if (d.y) row.load((const E*)d.y + t * d.y_stride, a);
-        if (d.d_next) row.load((const E*)d.d_next + t * d.cols, dn);
-        if (d.d_out) row.load((const E*)d.d_out + t * d.cols, dt);
-        if (!d.d_out)
+    const int64_t step = (int64_t)gridDim.x * per;
+    typename R::Raw ry, ro, rn, rt, rg;
+    f32x4 st;
+    auto fetch = [&](int64_t t) {
+        if (t >= d.rows) return;
+        st = *reinterpret_cast<const f32x4*>(d.stats + 4 * t);
+        row.fetch((const E*)d.residual + t * d.residual_stride, ro);
+        if (d.y) row.fetch((const E*)d.y + t * d.y_stride, ry);
+        if (d.d_next) row.fetch((const E*)d.d_next + t * d.cols, rn);
+        if (d.d_out) row.fetch((const E*)d.d_out + t * d.cols, rt);
+        if constexpr (ELEMENT) row.fetch((const E*)d.gate + t * d.gate_stride, rg);
+    };
+    fetch(first);
+    for (int64_t t = first; t < d.rows; t += step) {
+        const float m = st[0], r = st[1], m2 = st[2], r2 = st[3];
+        float a[N], o[N], dn[N], dt[N], gates[ELEMENT ? N : 1];
+        row.take(ro, o);
+        if (d.y) row.take(ry, a);
+        if (d.d_next) row.take(rn, dn);
+        if (d.d_out) row.take(rt, dt);
+        else
 #pragma unroll
             for (int i = 0; i < N; ++i) dt[i] = 0.0f;
+        if constexpr (ELEMENT) {
+            row.take(rg, gates);
+            if (d.gate_sigmoid)
+#pragma unroll
+                for (int i = 0; i < N; ++i) gates[i] = sigmoid_f32(gates[i]);
+        } else {
+            gates[0] = d.gate_mode == FMOE_GATE_TOKEN ? to_f32(((const E*)d.gate)[t * d.gate_stride]) : 1.0f;
+            if (d.gate_mode && d.gate_sigmoid) gates[0] = sigmoid_f32(gates[0]);
+        }
+        fetch(t + step);
+        auto gate = [&](int i) { return gates[ELEMENT ? i : 0]; };
         if (d.y) {
-            if (d.gate_mode == FMOE_GATE_ELEMENT) {
-                row.load((const E*)d.gate + t * d.gate_stride, gate);
-            } else {
-                const float g = d.gate_mode == FMOE_GATE_TOKEN ? to_f32(((const E*)d.gate)[t * d.gate_stride]) : 1.0f;
 #pragma unroll
-                for (int i = 0; i < N; ++i) gate[i] = g;
-            }
+            for (int c = 0; c < CH; ++c) {
+                float s[V], w[V], b[V];
+                scale.get(row, c, s);
+                weight.get(row, c, w);
+                if constexpr (LAYER) bias.get(row, c, b);
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if (d.gate_mode && d.gate_sigmoid) gate[i] = sigmoid_f32(gate[i]);
-                a[i] = row.in(i) ? (a[i] - st[0]) * st[1] : 0.0f;
-                if (row.in(i)) o[i] += scale[i] * gate[i] * (a[i] * weight[i] + bias[i]);
+                for (int j = 0; j < V; ++j) {
+                    const int i = c * V + j;
+                    a[i] = row.in(i) ? (a[i] - m) * r : 0.0f;
+                    if (row.in(i)) o[i] += s[j] * gate(i) * (a[i] * w[j] + (LAYER ? b[j] : 0.0f));
+                }
             }
         }
         if (d.d_next) {
-            float s[2] = {0.0f, 0.0f}, b[N];
+            float s[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                b[i] = row.in(i) ? (o[i] - st[2]) * st[3] : 0.0f;
-                sums[kDNextWeight][i] += dn[i] * b[i];
-                sums[kDNextBias][i] += dn[i];
-                dn[i] *= next_w[i];
-                s[0] += dn[i] * b[i];
-                s[1] += dn[i];
+            for (int c = 0; c < CH; ++c) {
+                float w[V];
+                next_weight.get(row, c, w);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int i = c * V + j;
+                    o[i] = row.in(i) ? (o[i] - m2) * r2 : 0.0f;
+                    sums[kDNextWeight][i] += dn[i] * o[i];
+                    if constexpr (LAYER) sums[kDNextBias][i] += dn[i];
+                    dn[i] *= w[j];
+                    s[0] += dn[i] * o[i];
+                    if constexpr (LAYER) s[1] += dn[i];
+                }
             }
             x.sum(s);
 #pragma unroll
-            for (int i = 0; i < N; ++i) dt[i] += st[3] * (dn[i] - b[i] * (s[0] * inv) - (layer ? s[1] * inv : 0.0f));
+            for (int i = 0; i < N; ++i) dt[i] += r2 * (dn[i] - o[i] * (s[0] * inv) - (LAYER ? s[1] * inv : 0.0f));
         }
         if (d.d_residual) row.store((E*)d.d_residual + t * d.cols, dt);
         if (d.y) {
-            float s[3] = {0.0f, 0.0f, 0.0f}, dz[N];
+            float q[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float z = a[i] * weight[i] + bias[i], dsz = dt[i] * scale[i];
-                dz[i] = dsz * gate[i];
-                sums[kDScale][i] += dt[i] * gate[i] * z;
-                sums[kDWeight][i] += dz[i] * a[i];
-                sums[kDBias][i] += dz[i];
-                const float da = dz[i] * weight[i];
-                float dg = dsz * z;
-                if (d.gate_sigmoid) dg *= gate[i] * (1.0f - gate[i]);
-                if (row.in(i)) {
-                    s[0] += da * a[i];
-                    s[1] += da;
-                    s[2] += dg;
+            for (int c = 0; c < CH; ++c) {
+                float s[V], w[V], b[V];
+                scale.get(row, c, s);
+                weight.get(row, c, w);
+                if constexpr (LAYER) bias.get(row, c, b);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int i = c * V + j;
+                    const float z = a[i] * w[j] + (LAYER ? b[j] : 0.0f), g = gate(i), dsz = dt[i] * s[j], dz = dsz * g, da = dz * w[j];
+                    sums[kDScale][i] += dt[i] * g * z;
+                    sums[kDWeight][i] += dz * a[i];
+                    if constexpr (LAYER) sums[kDBias][i] += dz;
+                    float dg = dsz * z;
+                    if (d.gate_sigmoid) dg *= g * (1.0f - g);
+                    if (row.in(i)) {
+                        q[0] += da * a[i];
+                        if constexpr (LAYER) q[1] += da;
+                        if constexpr (!ELEMENT) q[2] += dg;
+                    }
+                    dt[i] = da;
+                    if constexpr (ELEMENT) gates[i] = dg;
                 }
-                dz[i] = da;
-                gate[i] = dg;
             }
-            if (d.weight || d.gate_mode == FMOE_GATE_TOKEN) x.sum(s);
+            if (d.weight || d.gate_mode == FMOE_GATE_TOKEN) x.sum(q);
             if (d.d_gate) {
-                if (d.gate_mode == FMOE_GATE_ELEMENT) row.store((E*)d.d_gate + t * d.cols, gate);
-                else if (row.tid == 0) from_f32((E*)d.d_gate + t, s[2]);
+                if constexpr (ELEMENT) row.store((E*)d.d_gate + t * d.cols, gates);
+                else if (row.tid == 0) from_f32((E*)d.d_gate + t, q[2]);
             }
             if (d.d_y) {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (d.weight) dz[i] = st[1] * (dz[i] - a[i] * (s[0] * inv) - (layer ? s[1] * inv : 0.0f));
-                row.store((E*)d.d_y + t * d.cols, dz);
+                    if (d.weight) dt[i] = r * (dt[i] - a[i] * (q[0] * inv) - (LAYER ? q[1] * inv : 0.0f));
+                row.store((E*)d.d_y + t * d.cols, dt);
             }
         }
     }
     if (partial) {      // a group without a row leaves zeros
         float* const at = partial + (int64_t)first * kSums * d.cols;
-        void* const want[kSums] = {d.d_scale, d.d_weight, d.d_bias, d.d_next_weight, d.d_next_bias};
+        void* const want[kSums] = {d.d_scale, d.d_weight, d.d_next_weight, d.d_bias, d.d_next_bias};
 #pragma unroll
-        for (int s = 0; s < kSums; ++s)
+        for (int s = 0; s < SUMS; ++s)
             if (want[s]) row.store_f32(at + (int64_t)s * d.cols, sums[s]);
     }
 }
 
-// The groups' partial sums added in order: 64 columns a block, its waves share the groups.
-constexpr int kSumWaves = 8;
+// The groups' partial sums added in order: 32 columns a block, its 32 half waves share the groups.
+constexpr int kSumWaves = 16, kSumCols = 32;
 __global__ __launch_bounds__(kSumWaves* kWave) void norm_sums_kernel(fmoe_norm_desc d, const float* partial, int groups) {
-    __shared__ float part[kSumWaves][kWave];
-    const int lane = lane_id(), wave = threadIdx.x / kWave, which = blockIdx.y, col = blockIdx.x * kWave + lane;
-    void* const to[kSums] = {d.d_scale, d.d_weight, d.d_bias, d.d_next_weight, d.d_next_bias};
+    __shared__ float part[2 * kSumWaves][kSumCols];
+    const int lane = threadIdx.x % kSumCols, share = threadIdx.x / kSumCols, which = blockIdx.y, col = blockIdx.x * kSumCols + lane;
+    void* const to[kSums] = {d.d_scale, d.d_weight, d.d_next_weight, d.d_bias, d.d_next_bias};
     void* out = nullptr;
 #pragma unroll
     for (int s = 0; s < kSums; ++s)
         if (which == s) out = to[s];
     if (!out) return;
-    const int per = (groups + kSumWaves - 1) / kSumWaves, from = wave * per, until = min(groups, from + per);
+    const int per = (groups + 2 * kSumWaves - 1) / (2 * kSumWaves), from = share * per, until = min(groups, from + per);
     float v = 0.0f;
-    if (col < d.cols)
-        for (int g = from; g < until; ++g) v += partial[((int64_t)g * kSums + which) * d.cols + col];
-    part[wave][lane] = v;
-    __syncthreads();
-    if (wave == 0 && col < d.cols) {
+    if (col < d.cols) {
+        const float* const at = partial + (int64_t)which * d.cols + col;
+        int g = from;
+        for (; g + 8 <= until; g += 8) {
+            float p[8];
 #pragma unroll
-        for (int w = 1; w < kSumWaves; ++w) v += part[w][lane];
+            for (int i = 0; i < 8; ++i) p[i] = at[(int64_t)(g + i) * kSums * d.cols];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v += p[i];
+        }
+        for (; g < until; ++g) v += at[(int64_t)g * kSums * d.cols];
+    }
+    part[share][lane] = v;
+    __syncthreads();
+    if (share == 0 && col < d.cols) {
+#pragma unroll
+        for (int w = 1; w < 2 * kSumWaves; ++w) v += part[w][lane];
         if (d.param_dtype == FMOE_F32) reinterpret_cast<float*>(out)[col] = v;
         else reinterpret_cast<uint16_t*>(out)[col] = (uint16_t)f32_to_bf16_bits(v);
     }
 }
 
-constexpr int kNormMostCols = 8192;
+constexpr int kNormMostCols = 8192, kNormBwdWaves = 8;
 
 struct NormPlan {
     bool vec;
     int chunks, waves, per, threads;
 };
-NormPlan norm_plan(const fmoe_norm_desc& d) {
+// Chunks of a lane and waves of a row: one chunk, the row spread over as many lanes as it has chunks, as far as 16 waves (8 in the backward pass, whose
+// sums over rows take registers) go.  A row per wave of four chunks each, with no barrier, was slower: 16384 x 2048 bf16 forward 97 us against 67 (the
+// parameters are asked for again for every row, and 245 registers leave two waves to a SIMD).
+NormPlan norm_plan(const fmoe_norm_desc& d, bool backward) {
     const int v = d.dtype == FMOE_F32 ? 4 : 8, es = d.dtype == FMOE_F32 ? 4 : 2;
     auto whole = [&](const void* p, int64_t stride) { return aligned16(p) && stride * es % 16 == 0; };
     NormPlan p;
     p.vec = d.cols % v == 0 && whole(d.y, d.y_stride) && whole(d.residual, d.residual_stride) && whole(d.out, 0) && whole(d.next, 0) && whole(d.y_out, 0) &&
             (d.gate_mode != FMOE_GATE_ELEMENT || whole(d.gate, d.gate_stride)) && whole(d.d_out, 0) && whole(d.d_next, 0) && whole(d.d_y, 0) &&
-            whole(d.d_residual, 0) && (d.gate_mode != FMOE_GATE_ELEMENT || whole(d.d_gate, 0));
+            whole(d.d_residual, 0) && (d.gate_mode != FMOE_GATE_ELEMENT || whole(d.d_gate, 0)) && aligned16(d.scale) && aligned16(d.weight) &&
+            aligned16(d.bias) && aligned16(d.next_weight) && aligned16(d.next_bias);
     const int lanes = (d.cols + v - 1) / v;                      // one chunk each
-    p.chunks = lanes <= kNormMostWaves * kWave ? 1 : 2;
-    p.waves = (lanes + p.chunks * kWave - 1) / (p.chunks * kWave);
+    auto waves = [&](int chunks) { return (lanes + chunks * kWave - 1) / (chunks * kWave); };
+    p.chunks = 1;
+    if (backward) {
+        while (waves(p.chunks) > (p.vec ? kNormBwdWaves : kNormMostWaves)) p.chunks *= 2;
+    } else if (waves(1) > kNormMostWaves) {
+        p.chunks = 2;
+    }
+    p.waves = waves(p.chunks);
     p.per = p.waves == 1 ? 4 : 1;
     p.threads = (p.waves == 1 ? 4 : p.waves) * kWave;
     return p;
 }
-// Groups (blocks, or waves where a wave has a row) of the backward pass: as many as the chip holds at once, fewer where that is many partial sums to a row
+// Groups (blocks, or waves where a wave has a row) of the backward pass: as many as the chip holds at once
 int norm_groups(const fmoe_norm_desc& d, const NormPlan& p) {
-    const int64_t most = p.waves == 1 ? 2048 : 1024;
+    const int64_t most = 256 * 12 / p.waves;
     return (int)(d.rows < most ? d.rows : most);
 }
 
@@ -409,6 +708,12 @@ int norm_check(const fmoe_norm_desc* d, bool backward) {
     return FMOE_OK;
 }
 
+template <typename F>
+void with_bool(bool b, F&& f) {
+    if (b) f(std::true_type());
+    else f(std::false_type());
+}
+
 bool norm_wants_sums(const fmoe_norm_desc& d) { return d.d_scale || d.d_weight || d.d_bias || d.d_next_weight || d.d_next_bias; }
 
 }  // namespace
@@ -416,29 +721,48 @@ bool norm_wants_sums(const fmoe_norm_desc& d) { return d.d_scale || d.d_weight |
 
 using namespace fmoe;
 
-#define FMOE_NORM(kern, ...)                                                                                             \
-    do {                                                                                                                 \
-        if (d.dtype == FMOE_F32) {                                                                                       \
-            if (p.vec) { if (p.chunks == 1) kern<float, true, 1> __VA_ARGS__; else kern<float, true, 2> __VA_ARGS__; }   \
-            else { if (p.chunks == 1) kern<float, false, 1> __VA_ARGS__; else kern<float, false, 2> __VA_ARGS__; }       \
-        } else {                                                                                                         \
-            if (p.vec) kern<uint16_t, true, 1> __VA_ARGS__; else kern<uint16_t, false, 1> __VA_ARGS__;                   \
-        }                                                                                                                \
-    } while (0)
-
 extern "C" int fmoe_norm_add(const fmoe_norm_desc* desc, fmoe_stream_t stream) {
     const int rc = norm_check(desc, false);
     if (rc != FMOE_OK || desc->rows == 0) return rc;
     const fmoe_norm_desc& d = *desc;
-    const NormPlan p = norm_plan(d);
-    const int64_t blocks = (d.rows + p.per - 1) / p.per, most = 256 * 32 / (p.threads / kWave);
-    FMOE_NORM(norm_add_kernel, <<<(unsigned)(blocks < most ? blocks : most), p.threads, 0, (hipStream_t)stream>>>(d, p.waves));
+    const NormPlan p = norm_plan(d, false);
+    const int64_t blocks = (d.rows + p.per - 1) / p.per, most = 256 * 16 / (p.threads / kWave);
+    auto go = [&](auto kern) { kern<<<(unsigned)(blocks < most ? blocks : most), p.threads, 0, (hipStream_t)stream>>>(d, p.waves); };
+    auto of = [&](auto vec, auto merge) {
+        constexpr bool VEC = decltype(vec)::value, MERGE = decltype(merge)::value;
+        if (d.dtype == FMOE_F32) {
+            if (p.chunks == 1) go(norm_add_kernel<float, VEC, 1, MERGE>);
+            else go(norm_add_kernel<float, VEC, 2, MERGE>);
+        } else {
+            go(norm_add_kernel<uint16_t, VEC, 1, MERGE>);
+        }
+    };
+    const bool p32 = d.param_dtype == FMOE_F32, own = p32 || d.dtype == FMOE_BF16;      // (fp32 rows with bf16 parameters: the general kernel)
+    if (d.K && p.vec && p.chunks == 1 && own && d.gate_mode != FMOE_GATE_ELEMENT) {
+        const MergeParams m{d.rows, d.value_rows, d.y_stride, d.residual_stride, d.gate_stride, d.cols, d.K, d.merge_dtype == FMOE_F32, d.gate_mode, d.gate_mode && d.gate_sigmoid,
+                            d.eps, d.scale_value, d.y, d.residual, d.gate, d.merge, d.scale, d.weight, d.bias, d.next_weight, d.next_bias, d.reverse_index, d.merge_index,
+                            d.out, d.next, d.y_out, d.stats};
+        with_bool(d.norm == FMOE_NORM_LAYER, [&](auto layer) {
+            constexpr bool LAYER = decltype(layer)::value;
+            auto run = [&](auto kern) { kern<<<(unsigned)(blocks < most ? blocks : most), p.threads, 0, (hipStream_t)stream>>>(m, p.waves); };
+            auto batch = [&](auto two, auto four, auto eight) {
+                if (d.K <= 2) run(two);
+                else if (d.K <= 4) run(four);
+                else run(eight);
+            };
+            if (d.dtype == FMOE_F32) batch(norm_merge_kernel<float, LAYER, true, 2>, norm_merge_kernel<float, LAYER, true, 4>, norm_merge_kernel<float, LAYER, true, 8>);
+            else if (p32) batch(norm_merge_kernel<uint16_t, LAYER, true, 2>, norm_merge_kernel<uint16_t, LAYER, true, 4>, norm_merge_kernel<uint16_t, LAYER, true, 8>);
+            else batch(norm_merge_kernel<uint16_t, LAYER, false, 2>, norm_merge_kernel<uint16_t, LAYER, false, 4>, norm_merge_kernel<uint16_t, LAYER, false, 8>);
+        });
+        return check_launch("fmoe_norm_add");
+    }
+    with_bool(p.vec, [&](auto vec) { with_bool(d.K > 0, [&](auto merge) { of(vec, merge); }); });
     return check_launch("fmoe_norm_add");
 }
 
 extern "C" size_t fmoe_norm_add_bwd_workspace_bytes(const fmoe_norm_desc* desc) {
     if (norm_check(desc, true) != FMOE_OK || desc->rows == 0 || !norm_wants_sums(*desc)) return 0;
-    const NormPlan p = norm_plan(*desc);
+    const NormPlan p = norm_plan(*desc, true);
     const int64_t groups = norm_groups(*desc, p), all = (groups + p.per - 1) / p.per * p.per;
     return (size_t)all * kSums * desc->cols * sizeof(float);
 }
@@ -447,15 +771,31 @@ extern "C" int fmoe_norm_add_bwd(const fmoe_norm_desc* desc, void* workspace, si
     const int rc = norm_check(desc, true);
     if (rc != FMOE_OK || desc->rows == 0) return rc;
     const fmoe_norm_desc& d = *desc;
-    const NormPlan p = norm_plan(d);
+    const NormPlan p = norm_plan(d, true);
     const size_t need = fmoe_norm_add_bwd_workspace_bytes(desc);
     if (need && (!workspace || workspace_bytes < need))
         return fail(FMOE_ERR_WORKSPACE, "fmoe_norm_add_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     float* const partial = need ? (float*)workspace : nullptr;
     const int blocks = (norm_groups(d, p) + p.per - 1) / p.per;
-    FMOE_NORM(norm_add_bwd_kernel, <<<blocks, p.threads, 0, (hipStream_t)stream>>>(d, p.waves, partial));
+    auto go = [&](auto kern) { kern<<<blocks, p.threads, 0, (hipStream_t)stream>>>(d, p.waves, partial); };
+    with_bool(p.vec, [&](auto vec) {
+        with_bool(d.norm == FMOE_NORM_LAYER || d.bias || d.next_bias, [&](auto layer) {
+            with_bool(d.gate_mode == FMOE_GATE_ELEMENT, [&](auto element) {
+                constexpr bool VEC = decltype(vec)::value, LAYER = decltype(layer)::value, ELEMENT = decltype(element)::value;
+                constexpr int THREADS = VEC ? kNormBwdWaves * kWave : kNormMostWaves * kWave;
+                if (d.dtype == FMOE_F32) {
+                    if (p.chunks == 1) go(norm_add_bwd_kernel<float, VEC, 1, LAYER, ELEMENT, THREADS>);
+                    else if (p.chunks == 2) go(norm_add_bwd_kernel<float, VEC, 2, LAYER, ELEMENT, THREADS>);
+                    else if constexpr (VEC) go(norm_add_bwd_kernel<float, VEC, 4, LAYER, ELEMENT, THREADS>);
+                } else {
+                    if (p.chunks == 1) go(norm_add_bwd_kernel<uint16_t, VEC, 1, LAYER, ELEMENT, THREADS>);
+                    else if constexpr (VEC) go(norm_add_bwd_kernel<uint16_t, VEC, 2, LAYER, ELEMENT, THREADS>);
+                }
+            });
+        });
+    });
     const int launched = check_launch("fmoe_norm_add_bwd");
     if (launched != FMOE_OK || !need) return launched;
-    norm_sums_kernel<<<dim3((d.cols + kWave - 1) / kWave, kSums), kSumWaves * kWave, 0, (hipStream_t)stream>>>(d, partial, blocks * p.per);
+    norm_sums_kernel<<<dim3((d.cols + kSumCols - 1) / kSumCols, kSums), kSumWaves * kWave, 0, (hipStream_t)stream>>>(d, partial, blocks * p.per);
     return check_launch("fmoe_norm_add_bwd");
 }
