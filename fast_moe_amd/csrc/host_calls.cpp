@@ -47,6 +47,12 @@ decltype(&fmoe_weight_grad) c_weight_grad;
 decltype(&fmoe_weight_grad_pays) weight_grad_pays;
 decltype(&fmoe_few_tokens_workspace_bytes) few_tokens_workspace_bytes;
 decltype(&fmoe_few_tokens) c_few_tokens;
+decltype(&fmoe_norm_add) c_norm_add;
+decltype(&fmoe_norm_add_bwd_workspace_bytes) norm_add_bwd_workspace_bytes;
+decltype(&fmoe_norm_add_bwd) c_norm_add_bwd;
+decltype(&fmoe_swiglu_checkpoint) c_checkpoint;
+decltype(&fmoe_swiglu_checkpoint_read) c_checkpoint_read;
+decltype(&fmoe_swiglu_checkpoint_bwd) c_checkpoint_bwd;
 decltype(&fmoe_last_error) last_error;
 
 constexpr int64_t kSlackRows = 128;      // ops.SLACK_ROWS
@@ -869,12 +875,281 @@ PyObject* py_few_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// What the norms' forward and backward calls have in common, in this order: y, residual, weight, bias, gate, scale, next_weight, next_bias, gate_sigmoid,
+// scale_value, eps, norm
+struct Norm {
+    enum { Y, RESIDUAL, WEIGHT, BIAS, GATE, SCALE, NEXT_WEIGHT, NEXT_BIAS, TENSORS, ARGS = TENSORS + 4 };
+    at::Tensor t[TENSORS];
+    int64_t sigmoid, kind;
+    double scale_value, eps;
+    fmoe_norm_desc d = {};
+
+    bool parse(PyObject* const* args) {
+        for (int i = 0; i < TENSORS; ++i)
+            if (!optional_tensor(args[i], &t[i])) return false;
+        if (!t[RESIDUAL].defined() || !as_int(args[TENSORS], &sigmoid) || !PyFloat_CheckExact(args[TENSORS + 1]) || !PyFloat_CheckExact(args[TENSORS + 2]) ||
+            !as_int(args[TENSORS + 3], &kind))
+            return false;
+        scale_value = PyFloat_AS_DOUBLE(args[TENSORS + 1]);
+        eps = PyFloat_AS_DOUBLE(args[TENSORS + 2]);
+        return true;
+    }
+    bool ok(int64_t K) {
+        const at::Tensor& r = t[RESIDUAL];
+        if (!float_matrix(r)) return false;
+        const int64_t T = r.size(0), D = r.size(1);
+        if (T < 1 || D < 1 || D > 8192 || (T > 1 && r.stride(0) < D)) return false;
+        for (const at::Tensor& v : t)
+            if (!same_device(r, v)) return false;
+        const at::Tensor& y = t[Y];
+        const int64_t rows = K ? T * K : T;
+        if (y.defined() && (!float_matrix(y) || y.scalar_type() != r.scalar_type() || y.size(0) != rows || y.size(1) != D || (rows > 1 && y.stride(0) < D)))
+            return false;
+        int param = -1;
+        for (int i : {WEIGHT, BIAS, SCALE, NEXT_WEIGHT, NEXT_BIAS})
+            if (t[i].defined()) {
+                const int code = dtype_code(t[i].scalar_type());
+                if ((code != FMOE_F32 && code != FMOE_BF16) || (param >= 0 && code != param) || t[i].dim() != 1 || t[i].size(0) != D || !t[i].is_contiguous())
+                    return false;
+                param = code;
+            }
+        if ((t[BIAS].defined() && !t[WEIGHT].defined()) || (t[NEXT_BIAS].defined() && !t[NEXT_WEIGHT].defined()) || (!y.defined() && !t[NEXT_WEIGHT].defined()))
+            return false;
+        auto data = [&](int i) { return t[i].defined() ? t[i].data_ptr() : nullptr; };
+        d.rows = T;
+        d.cols = (int32_t)D;
+        d.dtype = dtype_code(r.scalar_type());
+        d.param_dtype = param < 0 ? d.dtype : param;
+        d.norm = (int32_t)kind;
+        d.eps = (float)eps;
+        d.scale_value = (float)scale_value;
+        d.y = data(Y);
+        d.y_stride = y.defined() ? y.stride(0) : 0;
+        d.residual = data(RESIDUAL);
+        d.residual_stride = r.stride(0);
+        d.scale = data(SCALE);
+        d.weight = data(WEIGHT);
+        d.bias = data(BIAS);
+        d.next_weight = data(NEXT_WEIGHT);
+        d.next_bias = data(NEXT_BIAS);
+        const at::Tensor& g = t[GATE];
+        if (g.defined()) {
+            const bool element = g.dim() == 2 && g.size(1) == D && D > 1;
+            if (!y.defined() || g.scalar_type() != r.scalar_type() || g.dim() < 1 || g.dim() > 2 || g.size(0) != T || (g.dim() == 2 && !element && g.size(1) != 1) ||
+                (element ? g.stride(1) != 1 || (T > 1 && g.stride(0) < D) : T > 1 && g.stride(0) < 1))
+                return false;
+            d.gate_mode = element ? FMOE_GATE_ELEMENT : FMOE_GATE_TOKEN;
+            d.gate = g.data_ptr();
+            d.gate_stride = g.stride(0);
+            d.gate_sigmoid = sigmoid != 0;
+        }
+        return true;
+    }
+};
+
+// (Norm's, reverse_index, merge, merge_index, for_backward, stream) -> (out, next, merged y, stats)
+PyObject* py_norm_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != Norm::ARGS + 5) return none();
+    Norm c;
+    at::Tensor reverse, merge, merge_index, out, next, merged, stats;
+    int64_t keep, stream;
+    if (!c.parse(args) || !optional_tensor(args[Norm::ARGS], &reverse) || !optional_tensor(args[Norm::ARGS + 1], &merge) ||
+        !optional_tensor(args[Norm::ARGS + 2], &merge_index) || !as_int(args[Norm::ARGS + 3], &keep) || !as_int(args[Norm::ARGS + 4], &stream))
+        return none();
+    const at::Tensor& r = c.t[Norm::RESIDUAL];
+    const int status = run(
+        [&] {
+            int64_t K = 0;
+            if (reverse.defined()) {
+                if (reverse.dim() != 2 || r.dim() != 2 || reverse.size(0) != r.size(0)) return false;
+                K = reverse.size(1);
+                if (K < 1 || K > 64 || !c.t[Norm::Y].defined() || !i64_list(reverse, r.size(0) * K) || !same_device(r, reverse)) return false;
+            }
+            if (!c.ok(K)) return false;
+            if (K) {
+                c.d.K = (int32_t)K;
+                c.d.value_rows = c.d.rows * K;
+                c.d.reverse_index = reverse.data_ptr<int64_t>();
+                if (merge.defined()) {
+                    const int code = dtype_code(merge.scalar_type());
+                    if ((code != FMOE_F32 && code != FMOE_BF16) || !merge.is_contiguous() || merge.numel() != c.d.value_rows || !same_device(r, merge)) return false;
+                    c.d.merge = merge.data_ptr();
+                    c.d.merge_dtype = code;
+                    if (merge_index.defined()) {
+                        if (!i64_list(merge_index, c.d.value_rows) || !same_device(r, merge_index)) return false;
+                        c.d.merge_index = merge_index.data_ptr<int64_t>();
+                    }
+                }
+            }
+            return true;
+        },
+        [&] {
+            if (c.t[Norm::Y].defined()) {
+                out = empty(r.sizes(), r.scalar_type(), r);
+                c.d.out = out.data_ptr();
+            }
+            if (c.d.next_weight) {
+                next = empty(r.sizes(), r.scalar_type(), r);
+                c.d.next = next.data_ptr();
+            }
+            if (keep) {
+                stats = empty({c.d.rows, 4}, at::kFloat, r);
+                c.d.stats = stats.data_ptr<float>();
+                if (c.d.K) {
+                    merged = empty(r.sizes(), r.scalar_type(), r);
+                    c.d.y_out = merged.data_ptr();
+                }
+            }
+            return c_norm_add(&c.d, (void*)stream);
+        });
+    if (raised(status, "fmoe_norm_add")) return nullptr;
+    return status == FMOE_OK ? Py_BuildValue("(NNNN)", wrap_or_none(out), wrap_or_none(next), wrap_or_none(merged), wrap_or_none(stats)) : none();
+    END_HANDLE_TH_ERRORS
+}
+
+// (Norm's, stats, d_out, d_next, need (bits in the order of Norm's tensors), stream) -> the gradients of Norm's tensors
+PyObject* py_norm_add_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != Norm::ARGS + 5) return none();
+    Norm c;
+    at::Tensor stats, d_out, d_next, grad[Norm::TENSORS], workspace;
+    int64_t need, stream;
+    if (!c.parse(args) || !optional_tensor(args[Norm::ARGS], &stats) || !optional_tensor(args[Norm::ARGS + 1], &d_out) ||
+        !optional_tensor(args[Norm::ARGS + 2], &d_next) || !as_int(args[Norm::ARGS + 3], &need) || !as_int(args[Norm::ARGS + 4], &stream))
+        return none();
+    const at::Tensor& r = c.t[Norm::RESIDUAL];
+    const int status = run(
+        [&] {
+            if (!c.ok(0) || !stats.defined() || !d_next.defined()) return false;
+            for (const at::Tensor* v : {&d_out, &d_next})
+                if (v->defined() && (v->scalar_type() != r.scalar_type() || v->sizes() != r.sizes() || !v->is_contiguous() || !same_device(r, *v))) return false;
+            if (stats.scalar_type() != at::kFloat || !stats.is_contiguous() || stats.numel() != 4 * c.d.rows || !same_device(r, stats)) return false;
+            for (int i = 0; i < Norm::TENSORS; ++i)
+                if ((need >> i & 1) && !c.t[i].defined()) return false;
+            return true;
+        },
+        [&] {
+            void** const to[Norm::TENSORS] = {&c.d.d_y, &c.d.d_residual, &c.d.d_weight, &c.d.d_bias, &c.d.d_gate, &c.d.d_scale, &c.d.d_next_weight, &c.d.d_next_bias};
+            for (int i = 0; i < Norm::TENSORS; ++i)
+                if (need >> i & 1) {
+                    grad[i] = empty(i == Norm::Y ? r.sizes() : c.t[i].sizes(), c.t[i].scalar_type(), r);
+                    *to[i] = grad[i].data_ptr();
+                }
+            c.d.stats = stats.data_ptr<float>();
+            c.d.d_out = d_out.defined() ? d_out.data_ptr() : nullptr;
+            c.d.d_next = d_next.data_ptr();
+            const size_t bytes = norm_add_bwd_workspace_bytes(&c.d);
+            if (bytes) workspace = empty({(int64_t)bytes}, at::kByte, r);
+            return c_norm_add_bwd(&c.d, bytes ? workspace.data_ptr() : nullptr, bytes, (void*)stream);
+        });
+    if (raised(status, "fmoe_norm_add_bwd")) return nullptr;
+    if (status != FMOE_OK) return none();
+    PyObject* out = PyTuple_New(Norm::TENSORS);
+    if (!out) return nullptr;
+    for (int i = 0; i < Norm::TENSORS; ++i) PyTuple_SET_ITEM(out, i, wrap_or_none(grad[i]));
+    return out;
+    END_HANDLE_TH_ERRORS
+}
+
+bool rows_apart(const at::Tensor& t) { return t.size(0) <= 1 || t.stride(0) >= t.size(1); }
+
+// (g [R, H], u [R, H], stream) -> (codes, exponents)
+PyObject* py_checkpoint(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3) return none();
+    const at::Tensor g = gpu_tensor(args[0]), u = gpu_tensor(args[1]);
+    at::Tensor q, e;
+    int64_t stream;
+    if (!g.defined() || !u.defined() || !as_int(args[2], &stream)) return none();
+    const int status = run(
+        [&] {
+            return float_matrix(g) && float_matrix(u) && g.scalar_type() == u.scalar_type() && g.sizes() == u.sizes() && g.numel() > 0 && same_device(g, u) &&
+                   rows_apart(g) && rows_apart(u);
+        },
+        [&] {
+            const int64_t R = g.size(0), H = g.size(1), P = (H + 31) / 32 * 32;
+            q = empty({R, 2, P}, at::kChar, g);
+            e = empty({R, 2, P / 32}, at::kByte, g);
+            return c_checkpoint(g.data_ptr(), u.data_ptr(), dtype_code(g.scalar_type()), R, H, g.stride(0), u.stride(0), q.data_ptr<int8_t>(),
+                                e.data_ptr<uint8_t>(), (void*)stream);
+        });
+    if (raised(status, "fmoe_swiglu_checkpoint")) return nullptr;
+    return status == FMOE_OK ? Py_BuildValue("(NN)", wrap(q), wrap(e)) : none();
+    END_HANDLE_TH_ERRORS
+}
+
+bool checkpoint_ok(const at::Tensor& q, const at::Tensor& e, int64_t H) {
+    const int64_t P = (H + 31) / 32 * 32;
+    return H >= 1 && q.scalar_type() == at::kChar && e.scalar_type() == at::kByte && q.dim() == 3 && e.dim() == 3 && q.size(0) > 0 && q.size(1) == 2 && q.size(2) == P &&
+           e.size(0) == q.size(0) && e.size(1) == 2 && e.size(2) == P / 32 && q.is_contiguous() && e.is_contiguous() && same_device(q, e) &&
+           (uintptr_t)q.data_ptr() % 16 == 0;
+}
+
+// (codes, exponents, columns, fp32?, stream) -> (g, u)
+PyObject* py_checkpoint_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5) return none();
+    const at::Tensor q = gpu_tensor(args[0]), e = gpu_tensor(args[1]);
+    at::Tensor g, u;
+    int64_t H, f32, stream;
+    if (!q.defined() || !e.defined() || !as_int(args[2], &H) || !as_int(args[3], &f32) || !as_int(args[4], &stream)) return none();
+    const int status = run([&] { return checkpoint_ok(q, e, H); },
+                           [&] {
+                               const at::ScalarType type = f32 ? at::kFloat : at::kBFloat16;
+                               g = empty({q.size(0), H}, type, q);
+                               u = empty({q.size(0), H}, type, q);
+                               return c_checkpoint_read(q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(), g.data_ptr(), u.data_ptr(), dtype_code(type), q.size(0), H, H, H,
+                                                        (void*)stream);
+                           });
+    if (raised(status, "fmoe_swiglu_checkpoint_read")) return nullptr;
+    return status == FMOE_OK ? Py_BuildValue("(NN)", wrap(g), wrap(u)) : none();
+    END_HANDLE_TH_ERRORS
+}
+
+// (codes, exponents, columns, d [R, H], weight or None, joint, dots?, stream) -> (dg, du, h, dots or None), with slack rows
+PyObject* py_checkpoint_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 8) return none();
+    const at::Tensor q = gpu_tensor(args[0]), e = gpu_tensor(args[1]), d = gpu_tensor(args[3]);
+    at::Tensor w, dg, du, h, dots;
+    int64_t H, joint, want, stream;
+    if (!q.defined() || !e.defined() || !d.defined() || !as_int(args[2], &H) || !optional_tensor(args[4], &w) || !as_int(args[5], &joint) || !as_int(args[6], &want) ||
+        !as_int(args[7], &stream))
+        return none();
+    const int status = run(
+        [&] {
+            if (!checkpoint_ok(q, e, H) || !float_matrix(d) || d.size(0) != q.size(0) || d.size(1) != H || !rows_apart(d) || !same_device(q, d)) return false;
+            return !w.defined() || ((w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16) && w.numel() == q.size(0) && w.is_contiguous() && same_device(q, w));
+        },
+        [&] {
+            const int64_t R = q.size(0);
+            if (joint) {
+                const at::Tensor both = empty_rows(R, 2 * H, d.scalar_type(), d);
+                dg = both.narrow(1, 0, H);
+                du = both.narrow(1, H, H);
+            } else {
+                dg = empty_rows(R, H, d.scalar_type(), d);
+                du = empty_rows(R, H, d.scalar_type(), d);
+            }
+            h = empty_rows(R, H, d.scalar_type(), d);
+            if (want) dots = empty({R}, at::kFloat, d);
+            return c_checkpoint_bwd(q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(), d.data_ptr(), dtype_code(d.scalar_type()), R, H, d.stride(0),
+                                    w.defined() ? w.data_ptr() : nullptr, w.defined() ? dtype_code(w.scalar_type()) : 0, dg.data_ptr(), du.data_ptr(), dg.stride(0),
+                                    h.data_ptr(), h.stride(0), want ? dots.data_ptr<float>() : nullptr, (void*)stream);
+        });
+    if (raised(status, "fmoe_swiglu_checkpoint_bwd")) return nullptr;
+    return status == FMOE_OK ? Py_BuildValue("(NNNN)", wrap(dg), wrap(du), wrap(h), wrap_or_none(dots)) : none();
+    END_HANDLE_TH_ERRORS
+}
+
 // init(addresses of the C entry points, in the order of the pointers above)
 PyObject* py_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void* const entry[] = {&route_workspace_bytes, &c_route_topk, &c_grouped_gemm, &c_combine, &c_quant_rows, &c_gate_softmax, &gemm_workspace_bytes,
                            &c_grouped_gemm_ws, &c_gemm_plan, &c_combine_bwd, &c_segment_colsum, &c_swiglu_bwd, &c_silu_mul, &c_gather_rows,
                            &c_invert_index, &c_gate_l1_bwd, &c_weight_grad, &weight_grad_pays, &gate_softmax_pays,
-                           &gate_route_pays, &few_tokens_workspace_bytes, &c_few_tokens, &last_error};
+                           &gate_route_pays, &few_tokens_workspace_bytes, &c_few_tokens, &c_norm_add, &norm_add_bwd_workspace_bytes,
+                           &c_norm_add_bwd, &c_checkpoint, &c_checkpoint_read, &c_checkpoint_bwd, &last_error};
     constexpr Py_ssize_t count = sizeof(entry) / sizeof(entry[0]);
     if (n != count) {
         PyErr_Format(PyExc_TypeError, "init: %d addresses expected", (int)count);
@@ -910,6 +1185,11 @@ PyMethodDef methods[] = {
     FASTCALL("gate_softmax", py_gate_softmax),
     FASTCALL("mlp_forward", py_mlp_forward),
     FASTCALL("few_tokens", py_few_tokens),
+    FASTCALL("norm_add", py_norm_add),
+    FASTCALL("norm_add_bwd", py_norm_add_bwd),
+    FASTCALL("checkpoint", py_checkpoint),
+    FASTCALL("checkpoint_read", py_checkpoint_read),
+    FASTCALL("checkpoint_bwd", py_checkpoint_bwd),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -827,6 +827,11 @@ def gate_l1_bwd(scores: torch.Tensor, topk_idx: torch.Tensor, d_gates: torch.Ten
 FEW_TOKENS, FEW_EXPERTS, FEW_K = 64, 256, 16       # limits of fmoe_few_tokens
 
 
+def _is_current(t: torch.Tensor) -> bool:
+    """Whether t lives on the current device, where the native calls launch."""
+    return t.is_cuda and t.get_device() == torch.cuda.current_device()
+
+
 def _on_device(t: torch.Tensor):
     """t's device as the current one while kernels are launched on a stream of it (nothing where it is already)."""
     return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
@@ -840,7 +845,7 @@ def few_tokens(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias: Optional[t
     [E, H, O] are views of storage with the contraction contiguous (``stride(1) == 1``), of x's dtype or, with ``scales``
     (multipliers [E, H], [E, H], [E, O] in fp32), e4m3."""
     name = "fused_moe_few_tokens"
-    if x.is_cuda and x.get_device() == torch.cuda.current_device():
+    if _is_current(x):
         out = _lib.host().few_tokens(x, gate_weight, gate_bias, weight, bias, weight_p, bias_p, weight_out, bias_out, token_mask, *scales, k,
                                      bool(renorm), _stream(x))
         if out is not None:
@@ -941,6 +946,13 @@ class NormArgs(NamedTuple):
     norm: str = "rms"
 
 
+def _norm_operands(a: NormArgs):
+    """The arguments of the native calls behind y and the residual."""
+    tensor = isinstance(a.scale, torch.Tensor)
+    return (a.weight, a.bias, a.gate, a.scale if tensor else None, a.next_weight, a.next_bias, bool(a.gate_sigmoid),
+            1.0 if tensor or a.scale is None else float(a.scale), float(a.eps), _NORMS.get(a.norm))
+
+
 def _norm_desc(name: str, y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, rows_of_y: int) -> Tuple[NormDesc, list]:
     """The descriptor of a call, checked, and the tensors that have to live as long as it (copies among them)."""
     scale = a.scale if isinstance(a.scale, torch.Tensor) else None
@@ -1000,6 +1012,10 @@ def norm_add(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, rev
              merge: Optional[torch.Tensor] = None, merge_index: Optional[torch.Tensor] = None, for_backward: bool = False):
     """-> (out, next, y, stats), see fmoe_norm_add; ``y`` is the merged one and it and ``stats`` are None unless ``for_backward``."""
     name = "norm_add"
+    if _is_current(residual):
+        parts = _lib.host().norm_add(y, residual, *_norm_operands(a), reverse_index, merge, merge_index, int(for_backward), _stream(residual))
+        if parts is not None:
+            return parts
     T = residual.shape[0] if residual.ndim else 0
     K = 0
     if reverse_index is not None:
@@ -1039,10 +1055,16 @@ def norm_add(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, rev
 def norm_add_bwd(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, stats: torch.Tensor, d_out: Optional[torch.Tensor],
                  d_next: Optional[torch.Tensor], need: Dict[str, bool]) -> Dict[str, Optional[torch.Tensor]]:
     """Gradients of norm_add by operand name (those ``need`` asks for), see fmoe_norm_add_bwd."""
-    d, keep = _norm_desc("norm_add_bwd", y, residual, a, residual.shape[0])
-    T, D = residual.shape
     rows = lambda t: None if t is None else t.to(residual.dtype).contiguous()
     d_out, d_next = rows(d_out), rows(d_next)
+    if _is_current(residual):
+        names = ("y", "residual", "weight", "bias", "gate", "scale", "next_weight", "next_bias")
+        parts = _lib.host().norm_add_bwd(y, residual, *_norm_operands(a), stats, d_out, d_next, sum(1 << i for i, n in enumerate(names) if need.get(n)),
+                                         _stream(residual))
+        if parts is not None:
+            return dict(zip(names, parts))
+    d, keep = _norm_desc("norm_add_bwd", y, residual, a, residual.shape[0])
+    T, D = residual.shape
     d.stats, d.d_out, d.d_next = stats.data_ptr(), _ptr(d_out), _ptr(d_next)
     grads = {}
     like = {"y": residual, "residual": residual, "gate": a.gate, "scale": a.scale, "weight": a.weight, "bias": a.bias,
@@ -1092,6 +1114,10 @@ def _check_kept(name: str, kept: SwigluCheckpoint) -> Tuple[torch.Tensor, torch.
 
 def swiglu_checkpoint(g: torch.Tensor, u: torch.Tensor) -> SwigluCheckpoint:
     name = "checkpoint_swiglu"
+    if _is_current(g):
+        parts = _lib.host().checkpoint(g, u, _stream(g))
+        if parts is not None:
+            return SwigluCheckpoint(*parts, g.shape[1], g.dtype)
     dev = _need_cuda(name, g, u)
     if g.dtype not in _DTYPE_CODE:
         raise NotImplementedError(f"{name}: the HIP kernels take bf16 or fp32, got {g.dtype}")
@@ -1111,6 +1137,10 @@ def swiglu_checkpoint(g: torch.Tensor, u: torch.Tensor) -> SwigluCheckpoint:
 
 
 def swiglu_checkpoint_read(kept: SwigluCheckpoint) -> Tuple[torch.Tensor, torch.Tensor]:
+    if _is_current(kept.q) and kept.dtype in _DTYPE_CODE:
+        parts = _lib.host().checkpoint_read(kept.q, kept.e, kept.cols, kept.dtype == torch.float32, _stream(kept.q))
+        if parts is not None:
+            return parts
     q, e = _check_kept("read_checkpoint", kept)
     R, H = q.shape[0], kept.cols
     g, u = (torch.empty((R, H), dtype=kept.dtype, device=q.device) for _ in range(2))
@@ -1127,6 +1157,10 @@ def swiglu_checkpoint_bwd(kept: SwigluCheckpoint, d: torch.Tensor, weight: Optio
     """-> (dg, du, h, dots), see fmoe_swiglu_checkpoint_bwd.  ``joint``: dg and du are the halves of one buffer, as
     ``swiglu_bwd(joint=True)`` returns them; all have SLACK_ROWS behind them."""
     name = "swiglu_checkpoint_bwd"
+    if _is_current(kept.q) and d.dtype == kept.dtype:
+        parts = _lib.host().checkpoint_bwd(kept.q, kept.e, kept.cols, d, weight, int(joint), int(need_dots), _stream(kept.q))
+        if parts is not None:
+            return parts
     q, e = _check_kept(name, kept)
     R, H = q.shape[0], kept.cols
     _need_cuda(name, q, d, weight)
