@@ -244,7 +244,9 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_no
     // The next row's loads are issued before this row's sums are exchanged.  Of a merge: the numbers and weights of the rows after it (a lane each), then
     // the first BATCH of the next token's rows.
     const int64_t first = (int64_t)blockIdx.x * per + (waves == 1 ? wave : 0), step = (int64_t)gridDim.x * per;
-    typename R::Raw ro, ry[MERGE ? BATCH : 1];
+    typename R::Raw ro, rg, ry[MERGE ? BATCH : 1];
+    const bool element = d.gate_mode == FMOE_GATE_ELEMENT;
+    E token_gate = E(0);
     const int lane = lane_id();
     int64_t from = -1;
     float share = 0.0f;
@@ -277,6 +279,8 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_no
         }
         if (t >= d.rows) return;
         row.fetch((const E*)d.residual + t * d.residual_stride, ro);
+        if (element) row.fetch((const E*)d.gate + t * d.gate_stride, rg);
+        else if (d.gate_mode) token_gate = ((const E*)d.gate)[t * d.gate_stride];
         if constexpr (MERGE) fetch_rows(0);
         else if (d.y) row.fetch((const E*)d.y + t * d.y_stride, ry[0]);
     };
@@ -285,6 +289,9 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_no
     for (int64_t t = first; t < d.rows; t += step) {
         float o[N], mean = 0.0f, rstd = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
         row.take(ro, o);
+        const typename R::Raw gates = rg;
+        float token = d.gate_mode == FMOE_GATE_TOKEN ? to_f32(token_gate) : 1.0f;
+        if (d.gate_mode == FMOE_GATE_TOKEN && d.gate_sigmoid) token = sigmoid_f32(token);
         if (d.y) {
             float y[N];
             if constexpr (MERGE) {
@@ -309,11 +316,6 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_no
                 fetch(t + step);
             }
             if (d.weight) row_stats(row, y, layer, d.eps, x, mean, rstd);
-            typename R::Raw rg;
-            const bool element = d.gate_mode == FMOE_GATE_ELEMENT;
-            float token = d.gate_mode == FMOE_GATE_TOKEN ? to_f32(((const E*)d.gate)[t * d.gate_stride]) : 1.0f;
-            if (element) row.fetch((const E*)d.gate + t * d.gate_stride, rg);
-            else if (d.gate_mode && d.gate_sigmoid) token = sigmoid_f32(token);
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 float s[V], w[V], b[V], g[V];
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_no
                 weight.get(row, c, w);
                 bias.get(row, c, b);
                 if (element) {
-                    row.take_chunk(rg, c, g);
+                    row.take_chunk(gates, c, g);
                     if (d.gate_sigmoid)
 #pragma unroll
                         for (int i = 0; i < V; ++i) g[i] = sigmoid_f32(g[i]);
@@ -403,6 +405,7 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(Merge
     };
     int lo = -1, hi = -1, share_bits = 0;
     u32x4 ro = {0, 0, 0, 0}, ry[BATCH];
+    E token_gate = E(0);
     auto rows = [&](int j0) {
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {       // (a row that is not there: row 0, and left out of the sum)
@@ -417,6 +420,7 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(Merge
         number(t + step);
         if (t >= p.rows) return;
         if (in) ro = *reinterpret_cast<const u32x4*>((const E*)p.residual + t * p.residual_stride + col);
+        if (p.gate_mode) token_gate = ((const E*)p.gate)[t * p.gate_stride];
         rows(0);
     };
     auto stats = [&](const float (&f)[V], float& mean, float& rstd) { row_stats(row, f, LAYER, p.eps, x, mean, rstd); };
@@ -438,11 +442,11 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(Merge
             }
         }
         R::unpack(ro, o);
+        float gate = p.gate_mode ? to_f32(token_gate) : 1.0f;
+        if (p.gate_sigmoid) gate = sigmoid_f32(gate);
         fetch(t + step);
         if (p.y_out && in) R::pack((E*)p.y_out + t * p.cols + col, y);
         if (p.weight) stats(y, mean, rstd);
-        float gate = p.gate_mode ? to_f32(((const E*)p.gate)[t * p.gate_stride]) : 1.0f;
-        if (p.gate_sigmoid) gate = sigmoid_f32(gate);
         param(p.weight, f, 1.0f);
         param(p.bias, g, 0.0f);
 #pragma unroll
@@ -489,6 +493,7 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
     const int64_t step = (int64_t)gridDim.x * per;
     typename R::Raw ry, ro, rn, rt, rg;
     f32x4 st;
+    E token_gate = E(0);
     auto fetch = [&](int64_t t) {
         if (t >= d.rows) return;
         st = *reinterpret_cast<const f32x4*>(d.stats + 4 * t);
@@ -497,6 +502,7 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
         if (d.d_next) row.fetch((const E*)d.d_next + t * d.cols, rn);
         if (d.d_out) row.fetch((const E*)d.d_out + t * d.cols, rt);
         if constexpr (ELEMENT) row.fetch((const E*)d.gate + t * d.gate_stride, rg);
+        else if (d.gate_mode) token_gate = ((const E*)d.gate)[t * d.gate_stride];
     };
     fetch(first);
     for (int64_t t = first; t < d.rows; t += step) {
@@ -515,7 +521,7 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
 #pragma unroll
                 for (int i = 0; i < N; ++i) gates[i] = sigmoid_f32(gates[i]);
         } else {
-            gates[0] = d.gate_mode == FMOE_GATE_TOKEN ? to_f32(((const E*)d.gate)[t * d.gate_stride]) : 1.0f;
+            gates[0] = d.gate_mode ? to_f32(token_gate) : 1.0f;
             if (d.gate_mode && d.gate_sigmoid) gates[0] = sigmoid_f32(gates[0]);
         }
         fetch(t + step);
