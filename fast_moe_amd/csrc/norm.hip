@@ -43,23 +43,6 @@ struct Row {
         u32x4 v[VEC ? CH : 1];
         E e[VEC ? 1 : N];
     };
-    // one chunk
-    __device__ __forceinline__ static void unpack(const u32x4& v, float (&f)[V]) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if constexpr (V == 4) f[i] = __uint_as_float(v[i]);
-            else f[i] = i & 1 ? __uint_as_float(v[i / 2] & 0xffff0000u) : __uint_as_float(v[i / 2] << 16);
-        }
-    }
-    __device__ __forceinline__ static void pack(E* p, const float (&f)[V]) {
-        u32x4 v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (V == 4) v[i] = __float_as_uint(f[i]);
-            else v[i] = cvt_pk_bf16(f[2 * i], f[2 * i + 1]);
-        }
-        *reinterpret_cast<u32x4*>(p) = v;
-    }
     int tid, threads, cols;
     __device__ __forceinline__ int col(int i) const {
         return VEC ? ((i / V) * threads + tid) * V + i % V : i * threads + tid;
@@ -228,12 +211,12 @@ struct Param {
     }
 };
 
-// MERGE: y is the merge of the token's rows.
-template <typename E, bool VEC, int CH, bool MERGE>
+// y given, or none (only the next norm).
+template <typename E, bool VEC, int CH>
 __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_norm_desc d, int waves) {
     using R = Row<E, VEC, CH>;
-    using P = Param<R, CH == 1 && !MERGE>;
-    constexpr int N = R::N, V = R::V, BATCH = 4 / CH;        // rows of a merge on their way
+    using P = Param<R, CH == 1>;
+    constexpr int N = R::N, V = R::V;
     __shared__ float buf[2][kNormMostWaves][4];
     const int per = waves == 1 ? blockDim.x / kWave : 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);       // rows of a block at a time
     const R row{waves == 1 ? (int)threadIdx.x % kWave : (int)threadIdx.x, waves * kWave, d.cols};
@@ -241,50 +224,18 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_no
     const bool layer = d.norm == FMOE_NORM_LAYER;
     const P scale(row, d.scale, d.param_dtype, d.scale_value), weight(row, d.weight, d.param_dtype, 1.0f), bias(row, d.bias, d.param_dtype, 0.0f),
         next_weight(row, d.next_weight, d.param_dtype, 0.0f), next_bias(row, d.next_bias, d.param_dtype, 0.0f);
-    // The next row's loads are issued before this row's sums are exchanged.  Of a merge: the numbers and weights of the rows after it (a lane each), then
-    // the first BATCH of the next token's rows.
+    // The next row's loads are issued before this row's sums are exchanged.
     const int64_t first = (int64_t)blockIdx.x * per + (waves == 1 ? wave : 0), step = (int64_t)gridDim.x * per;
-    typename R::Raw ro, rg, ry[MERGE ? BATCH : 1];
+    typename R::Raw ro, rg, ry;
     const bool element = d.gate_mode == FMOE_GATE_ELEMENT;
     E token_gate = E(0);
-    const int lane = lane_id();
-    int64_t from = -1;
-    float share = 0.0f;
-    auto number = [&](int64_t t) {
-        from = lane < d.K && t < d.rows ? d.reverse_index[t * d.K + lane] : -1;
-        if ((uint64_t)from >= (uint64_t)d.value_rows) from = -1;
-        share = 1.0f;
-        if (from >= 0 && d.merge) {
-            const int64_t at = d.merge_index ? d.merge_index[from] : from;
-            if ((uint64_t)at >= (uint64_t)d.value_rows) from = -1;
-            else share = d.merge_dtype == FMOE_F32 ? reinterpret_cast<const float*>(d.merge)[at] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(d.merge)[at]);
-        }
-    };
-    int from_lo = -1, from_hi = -1, share_bits = 0;         // of the token whose rows are being added
-    auto row_of = [&](int j) {
-        const int at = min(j, d.K - 1);
-        return j < d.K ? (int64_t)__builtin_amdgcn_readlane(from_hi, at) << 32 | (uint32_t)__builtin_amdgcn_readlane(from_lo, at) : -1;
-    };
-    auto fetch_rows = [&](int j0) {
-#pragma unroll
-        for (int j = 0; j < (MERGE ? BATCH : 1); ++j) {
-            const int64_t r = row_of(j0 + j);
-            if (r >= 0) row.fetch((const E*)d.y + r * d.y_stride, ry[j]);
-        }
-    };
     auto fetch = [&](int64_t t) {
-        if constexpr (MERGE) {
-            from_lo = (int)(uint32_t)from, from_hi = (int)(from >> 32), share_bits = (int)__float_as_uint(share);
-            number(t + step);
-        }
         if (t >= d.rows) return;
         row.fetch((const E*)d.residual + t * d.residual_stride, ro);
         if (element) row.fetch((const E*)d.gate + t * d.gate_stride, rg);
         else if (d.gate_mode) token_gate = ((const E*)d.gate)[t * d.gate_stride];
-        if constexpr (MERGE) fetch_rows(0);
-        else if (d.y) row.fetch((const E*)d.y + t * d.y_stride, ry[0]);
+        if (d.y) row.fetch((const E*)d.y + t * d.y_stride, ry);
     };
-    if constexpr (MERGE) number(first);
     fetch(first);
     for (int64_t t = first; t < d.rows; t += step) {
         float o[N], mean = 0.0f, rstd = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
@@ -294,27 +245,8 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_no
         if (d.gate_mode == FMOE_GATE_TOKEN && d.gate_sigmoid) token = sigmoid_f32(token);
         if (d.y) {
             float y[N];
-            if constexpr (MERGE) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) y[i] = 0.0f;
-                for (int j0 = 0; j0 < d.K; j0 += BATCH) {
-                    if (j0 > 0) fetch_rows(j0);
-#pragma unroll
-                    for (int j = 0; j < BATCH; ++j) {
-                        if (row_of(j0 + j) < 0) continue;
-                        const float w = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(share_bits, min(j0 + j, d.K - 1)));
-                        float f[N];
-                        row.take(ry[j], f);
-#pragma unroll
-                        for (int i = 0; i < N; ++i) y[i] = __builtin_fmaf(w, f[i], y[i]);
-                    }
-                }
-                fetch(t + step);
-                if (d.y_out) row.store((E*)d.y_out + t * d.cols, y);
-            } else {
-                row.take(ry[0], y);
-                fetch(t + step);
-            }
+            row.take(ry, y);
+            fetch(t + step);
             if (d.weight) row_stats(row, y, layer, d.eps, x, mean, rstd);
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -355,9 +287,8 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_no
     }
 }
 
-// The merge of expert rows and what follows it where rows are whole 16-byte chunks of the parameters' own kind (P32: fp32 parameters) and a gate is per
-// token: norm_add_kernel<MERGE> without its cases, whose registers (186) let half as many rows be on their way.  A row's waves take BATCH rows of the merge
-// at a time, the first of them while the row before is normed.
+// The merge of expert rows and what follows it.  A row's waves take BATCH rows of the merge at a time, the first of them while the row before is normed; the
+// rows' numbers and weights come a lane each, another row ahead.
 struct MergeParams {
     int64_t rows, value_rows, y_stride, residual_stride, gate_stride;
     int32_t cols, K, merge_f32, gate_mode, gate_sigmoid;
@@ -367,29 +298,16 @@ struct MergeParams {
     void *out, *next, *y_out;
     float* stats;
 };
-template <typename E, bool LAYER, bool P32, int BATCH>
+template <typename E, bool VEC, int CH, bool LAYER, bool P32, int BATCH>
 __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(MergeParams p, int waves) {
-    using R = Row<E, true, 1>;
-    constexpr int V = R::V;
+    using R = Row<E, VEC, CH>;
+    constexpr int V = R::V, N = R::N;
     __shared__ float buf[2][kNormMostWaves][4];
     const int per = waves == 1 ? blockDim.x / kWave : 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
     const R row{waves == 1 ? lane : (int)threadIdx.x, waves * kWave, p.cols};
     Exchange x{buf, waves, wave, 0};
-    const bool in = row.in(0);
-    const int col = row.col(0);
-    auto param = [&](const void* q, float (&f)[V], float none) {
-        if (q && in) {
-            if constexpr (P32) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) f[i] = reinterpret_cast<const float*>(q)[col + i];
-            } else {
-                R::unpack(*reinterpret_cast<const u32x4*>((const uint16_t*)q + col), f);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = none;
-        }
-    };
+    const bool element = p.gate_mode == FMOE_GATE_ELEMENT;
+    auto param = [&](const void* q, int c, float (&f)[V], float none) { row.param(q, P32 ? FMOE_F32 : FMOE_BF16, c, f, none); };
     const int64_t first = (int64_t)blockIdx.x * per + (waves == 1 ? wave : 0), step = (int64_t)gridDim.x * per;
     int64_t from = -1;
     float share = 0.0f;
@@ -404,65 +322,83 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(Merge
         }
     };
     int lo = -1, hi = -1, share_bits = 0;
-    u32x4 ro = {0, 0, 0, 0}, ry[BATCH];
+    typename R::Raw ro, rg, ry[BATCH];
     E token_gate = E(0);
     auto rows = [&](int j0) {
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {       // (a row that is not there: row 0, and left out of the sum)
             const int at = min(j0 + j, p.K - 1), h = __builtin_amdgcn_readlane(hi, at);
             const int64_t r = h < 0 ? 0 : (int64_t)h << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, at);
-            ry[j] = u32x4{0, 0, 0, 0};
-            if (in) ry[j] = *reinterpret_cast<const u32x4*>((const E*)p.y + r * p.y_stride + col);
+            row.fetch((const E*)p.y + r * p.y_stride, ry[j]);
         }
     };
     auto fetch = [&](int64_t t) {
         lo = (int)(uint32_t)from, hi = (int)(from >> 32), share_bits = (int)__float_as_uint(share);
         number(t + step);
         if (t >= p.rows) return;
-        if (in) ro = *reinterpret_cast<const u32x4*>((const E*)p.residual + t * p.residual_stride + col);
-        if (p.gate_mode) token_gate = ((const E*)p.gate)[t * p.gate_stride];
+        row.fetch((const E*)p.residual + t * p.residual_stride, ro);
+        if (element) row.fetch((const E*)p.gate + t * p.gate_stride, rg);
+        else if (p.gate_mode) token_gate = ((const E*)p.gate)[t * p.gate_stride];
         rows(0);
     };
-    auto stats = [&](const float (&f)[V], float& mean, float& rstd) { row_stats(row, f, LAYER, p.eps, x, mean, rstd); };
     number(first);
     fetch(first);
     for (int64_t t = first; t < p.rows; t += step) {
-        float y[V], o[V], f[V], g[V], mean = 0.0f, rstd = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
+        float y[N], o[N], mean = 0.0f, rstd = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = 0.0f;
+        for (int i = 0; i < N; ++i) y[i] = 0.0f;
         for (int j0 = 0; j0 < p.K; j0 += BATCH) {
             if (j0 > 0) rows(j0);
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
                 if (j0 + j >= p.K || __builtin_amdgcn_readlane(hi, min(j0 + j, p.K - 1)) < 0) continue;
                 const float w = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(share_bits, min(j0 + j, p.K - 1)));
-                R::unpack(ry[j], f);
+                float f[N];
+                row.take(ry[j], f);
 #pragma unroll
-                for (int i = 0; i < V; ++i) y[i] = __builtin_fmaf(w, f[i], y[i]);
+                for (int i = 0; i < N; ++i) y[i] = __builtin_fmaf(w, f[i], y[i]);
             }
         }
-        R::unpack(ro, o);
-        float gate = p.gate_mode ? to_f32(token_gate) : 1.0f;
-        if (p.gate_sigmoid) gate = sigmoid_f32(gate);
+        row.take(ro, o);
+        const typename R::Raw gates = rg;
+        float token = p.gate_mode && !element ? to_f32(token_gate) : 1.0f;
+        if (p.gate_sigmoid && !element) token = sigmoid_f32(token);
         fetch(t + step);
-        if (p.y_out && in) R::pack((E*)p.y_out + t * p.cols + col, y);
-        if (p.weight) stats(y, mean, rstd);
-        param(p.weight, f, 1.0f);
-        param(p.bias, g, 0.0f);
+        if (p.y_out) row.store((E*)p.y_out + t * p.cols, y);
+        if (p.weight) row_stats(row, y, LAYER, p.eps, x, mean, rstd);
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = (y[i] - mean) * rstd * f[i] + g[i];
-        param(p.scale, f, p.scale_value);
-        if (in)
+        for (int c = 0; c < CH; ++c) {
+            float f[V], g[V];
+            param(p.weight, c, f, 1.0f);
+            param(p.bias, c, g, 0.0f);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] += f[i] * gate * y[i];
-        if (in) R::pack((E*)p.out + t * p.cols + col, o);
+            for (int i = 0; i < V; ++i) y[c * V + i] = (y[c * V + i] - mean) * rstd * f[i] + g[i];
+            param(p.scale, c, f, p.scale_value);
+            if (element) {
+                row.take_chunk(gates, c, g);
+                if (p.gate_sigmoid)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) g[i] = sigmoid_f32(g[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] = token;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (row.in(c * V + i)) o[c * V + i] += f[i] * g[i] * y[c * V + i];
+        }
+        if (p.out) row.store((E*)p.out + t * p.cols, o);
         if (p.next) {
-            stats(o, mean2, rstd2);
-            param(p.next_weight, f, 0.0f);
-            param(p.next_bias, g, 0.0f);
+            row_stats(row, o, LAYER, p.eps, x, mean2, rstd2);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = (o[i] - mean2) * rstd2 * f[i] + g[i];
-            if (in) R::pack((E*)p.next + t * p.cols + col, o);
+            for (int c = 0; c < CH; ++c) {
+                float f[V], g[V];
+                param(p.next_weight, c, f, 0.0f);
+                param(p.next_bias, c, g, 0.0f);
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[c * V + i] = (o[c * V + i] - mean2) * rstd2 * f[i] + g[i];
+            }
+            row.store((E*)p.next + t * p.cols, o);
         }
         if (p.stats && row.tid == 0) *reinterpret_cast<f32x4*>(p.stats + 4 * t) = f32x4{mean, rstd, mean2, rstd2};
     }
@@ -734,35 +670,40 @@ extern "C" int fmoe_norm_add(const fmoe_norm_desc* desc, fmoe_stream_t stream) {
     const NormPlan p = norm_plan(d, false);
     const int64_t blocks = (d.rows + p.per - 1) / p.per, most = 256 * 16 / (p.threads / kWave);
     auto go = [&](auto kern) { kern<<<(unsigned)(blocks < most ? blocks : most), p.threads, 0, (hipStream_t)stream>>>(d, p.waves); };
-    auto of = [&](auto vec, auto merge) {
-        constexpr bool VEC = decltype(vec)::value, MERGE = decltype(merge)::value;
-        if (d.dtype == FMOE_F32) {
-            if (p.chunks == 1) go(norm_add_kernel<float, VEC, 1, MERGE>);
-            else go(norm_add_kernel<float, VEC, 2, MERGE>);
-        } else {
-            go(norm_add_kernel<uint16_t, VEC, 1, MERGE>);
-        }
-    };
-    const bool p32 = d.param_dtype == FMOE_F32, own = p32 || d.dtype == FMOE_BF16;      // (fp32 rows with bf16 parameters: the general kernel)
-    if (d.K && p.vec && p.chunks == 1 && own && d.gate_mode != FMOE_GATE_ELEMENT) {
-        const MergeParams m{d.rows, d.value_rows, d.y_stride, d.residual_stride, d.gate_stride, d.cols, d.K, d.merge_dtype == FMOE_F32, d.gate_mode, d.gate_mode && d.gate_sigmoid,
-                            d.eps, d.scale_value, d.y, d.residual, d.gate, d.merge, d.scale, d.weight, d.bias, d.next_weight, d.next_bias, d.reverse_index, d.merge_index,
-                            d.out, d.next, d.y_out, d.stats};
-        with_bool(d.norm == FMOE_NORM_LAYER, [&](auto layer) {
-            constexpr bool LAYER = decltype(layer)::value;
-            auto run = [&](auto kern) { kern<<<(unsigned)(blocks < most ? blocks : most), p.threads, 0, (hipStream_t)stream>>>(m, p.waves); };
-            auto batch = [&](auto two, auto four, auto eight) {
-                if (d.K <= 2) run(two);
-                else if (d.K <= 4) run(four);
-                else run(eight);
-            };
-            if (d.dtype == FMOE_F32) batch(norm_merge_kernel<float, LAYER, true, 2>, norm_merge_kernel<float, LAYER, true, 4>, norm_merge_kernel<float, LAYER, true, 8>);
-            else if (p32) batch(norm_merge_kernel<uint16_t, LAYER, true, 2>, norm_merge_kernel<uint16_t, LAYER, true, 4>, norm_merge_kernel<uint16_t, LAYER, true, 8>);
-            else batch(norm_merge_kernel<uint16_t, LAYER, false, 2>, norm_merge_kernel<uint16_t, LAYER, false, 4>, norm_merge_kernel<uint16_t, LAYER, false, 8>);
+    if (d.K) {
+        const MergeParams m{d.rows, d.value_rows, d.y_stride, d.residual_stride, d.gate_stride, d.cols, d.K, d.merge_dtype == FMOE_F32, d.gate_mode,
+                            d.gate_mode && d.gate_sigmoid, d.eps, d.scale_value, d.y, d.residual, d.gate, d.merge, d.scale, d.weight, d.bias, d.next_weight, d.next_bias,
+                            d.reverse_index, d.merge_index, d.out, d.next, d.y_out, d.stats};
+        auto run = [&](auto kern) { kern<<<(unsigned)(blocks < most ? blocks : most), p.threads, 0, (hipStream_t)stream>>>(m, p.waves); };
+        auto of = [&](auto value, auto vec, auto layer, auto p32) {
+            using E = decltype(value);
+            constexpr bool VEC = decltype(vec)::value, LAYER = decltype(layer)::value, P32 = decltype(p32)::value;
+            if constexpr (sizeof(E) == 4) {
+                if (p.chunks == 2) return run(norm_merge_kernel<E, VEC, 2, LAYER, P32, 2>);
+            }
+            if constexpr (VEC) {
+                if (d.K <= 2) return run(norm_merge_kernel<E, VEC, 1, LAYER, P32, 2>);
+                if (d.K > 4) return run(norm_merge_kernel<E, VEC, 1, LAYER, P32, 8>);
+            }
+            // (a row read element by element takes a register for every one)
+            run(norm_merge_kernel<E, VEC, 1, LAYER, P32, VEC || sizeof(E) == 4 ? 4 : 2>);
+        };
+        with_bool(p.vec, [&](auto vec) {
+            with_bool(d.norm == FMOE_NORM_LAYER, [&](auto layer) {
+                with_bool(d.param_dtype == FMOE_F32, [&](auto p32) {
+                    if (d.dtype == FMOE_F32) of(float(), vec, layer, p32);
+                    else of(uint16_t(), vec, layer, p32);
+                });
+            });
         });
         return check_launch("fmoe_norm_add");
     }
-    with_bool(p.vec, [&](auto vec) { with_bool(d.K > 0, [&](auto merge) { of(vec, merge); }); });
+    with_bool(p.vec, [&](auto vec) {
+        constexpr bool VEC = decltype(vec)::value;
+        if (d.dtype == FMOE_BF16) go(norm_add_kernel<uint16_t, VEC, 1>);
+        else if (p.chunks == 1) go(norm_add_kernel<float, VEC, 1>);
+        else go(norm_add_kernel<float, VEC, 2>);
+    });
     return check_launch("fmoe_norm_add");
 }
 
@@ -794,7 +735,8 @@ extern "C" int fmoe_norm_add_bwd(const fmoe_norm_desc* desc, void* workspace, si
                     else if (p.chunks == 2) go(norm_add_bwd_kernel<float, VEC, 2, LAYER, ELEMENT, THREADS>);
                     else if constexpr (VEC) go(norm_add_bwd_kernel<float, VEC, 4, LAYER, ELEMENT, THREADS>);
                 } else {
-                    if (p.chunks == 1) go(norm_add_bwd_kernel<uint16_t, VEC, 1, LAYER, ELEMENT, THREADS>);
+                    if (p.chunks == 1 && p.waves <= kNormBwdWaves) go(norm_add_bwd_kernel<uint16_t, VEC, 1, LAYER, ELEMENT, kNormBwdWaves * kWave>);
+                    else if (p.chunks == 1) go(norm_add_bwd_kernel<uint16_t, VEC, 1, LAYER, ELEMENT, THREADS>);
                     else if constexpr (VEC) go(norm_add_bwd_kernel<uint16_t, VEC, 2, LAYER, ELEMENT, THREADS>);
                 }
             });
