@@ -7,9 +7,11 @@
 //
 // 33 / 32 bytes for a value of 2 or 4, error at most half a step of 1 / 64 (3 % of the blocks' largest, rounded down to +-127: a whole step at the
 // very top); every v' is exact in bf16.  A zero block has exponent 0; one with an infinity or NaN has 255 and reads as NaN.
-// All of it is bound by the bytes; a lane has 16 values to write and 8 to read with (the row sum wants rows in whole waves, and 1408 columns leave
+// All of it is bound by the bytes; a lane has 16 values to write and 8 to read with (a row's sum wants its lanes in one wave, and 1408 columns leave
 // a third of the lanes of 16 idle, 8 % of those of 8).
 #include "common.h"
+
+#include <type_traits>
 
 namespace fmoe {
 namespace {
@@ -18,53 +20,52 @@ template <typename E> struct CE;
 template <> struct CE<float> { static constexpr int V = 4; };
 template <> struct CE<uint16_t> { static constexpr int V = 8; };
 
-template <typename E>
-__device__ __forceinline__ float value_of(E v) {
-    if constexpr (sizeof(E) == 4) return v;
-    else return bf16_bits_to_f32(v);
-}
-// n values (a multiple of a 16-byte chunk's), VEC: 16 bytes at a time; those from `left` on are zeros
-template <typename E, bool VEC, int N>
+// N values (whole 16-byte chunks) at any address an element may have; those from `left` on are zeros, or not written.  WHOLE: `left` is whole chunks;
+// otherwise the last one goes by elements.
+template <typename E, bool WHOLE, int N>
 __device__ __forceinline__ void load_values(const E* p, int left, float (&f)[N]) {
     constexpr int V = CE<E>::V;
-    if constexpr (VEC) {
 #pragma unroll
-        for (int c = 0; c < N / V; ++c) {
-            u32x4 v = {0, 0, 0, 0};
-            if (c * V < left) v = *reinterpret_cast<const u32x4*>(p + c * V);
+    for (int c = 0; c < N / V; ++c) {
+        u32x4 v = {0, 0, 0, 0};
+        if (WHOLE ? c * V < left : (c + 1) * V <= left) {
+            __builtin_memcpy(&v, p + c * V, 16);
+        } else if (!WHOLE && c * V < left) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if constexpr (V == 4) f[c * V + i] = __uint_as_float(v[i]);
-                else f[c * V + i] = i & 1 ? __uint_as_float(v[i / 2] & 0xffff0000u) : __uint_as_float(v[i / 2] << 16);
-            }
+            for (int i = 0; i < V; ++i)
+                if (c * V + i < left) {
+                    if constexpr (V == 4) v[i] = __float_as_uint(p[c * V + i]);
+                    else v[i / 2] |= (uint32_t)p[c * V + i] << (16 * (i & 1));
+                }
         }
-    } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = i < left ? value_of(p[i]) : 0.0f;
+        for (int i = 0; i < V; ++i) {
+            if constexpr (V == 4) f[c * V + i] = __uint_as_float(v[i]);
+            else f[c * V + i] = i & 1 ? __uint_as_float(v[i / 2] & 0xffff0000u) : __uint_as_float(v[i / 2] << 16);
+        }
     }
 }
-template <typename E, bool VEC, int N>
+template <typename E, bool WHOLE, int N>
 __device__ __forceinline__ void store_values(E* p, int left, const float (&f)[N]) {
     constexpr int V = CE<E>::V;
-    if constexpr (VEC) {
 #pragma unroll
-        for (int c = 0; c < N / V; ++c) {
-            if (c * V >= left) continue;
+    for (int c = 0; c < N / V; ++c) {
+        if (WHOLE ? c * V < left : (c + 1) * V <= left) {
             u32x4 v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (V == 4) v[i] = __float_as_uint(f[c * V + i]);
                 else v[i] = cvt_pk_bf16(f[c * V + 2 * i], f[c * V + 2 * i + 1]);
             }
-            *reinterpret_cast<u32x4*>(p + c * V) = v;
-        }
-    } else {
+            __builtin_memcpy(p + c * V, &v, 16);
+        } else if (!WHOLE && c * V < left) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < left) {
-                if constexpr (sizeof(E) == 4) p[i] = f[i];
-                else p[i] = (uint16_t)f32_to_bf16_bits(f[i]);
-            }
+            for (int i = 0; i < V; ++i)
+                if (c * V + i < left) {
+                    if constexpr (sizeof(E) == 4) p[c * V + i] = f[c * V + i];
+                    else p[c * V + i] = (uint16_t)f32_to_bf16_bits(f[c * V + i]);
+                }
+        }
     }
 }
 
@@ -77,7 +78,7 @@ struct CkptRows {
 };
 
 // 16 values a lane, two lanes a block; the lanes of a grid go over (row, matrix, half block) in memory order.
-template <typename E, bool VEC>
+template <typename E, bool WHOLE>
 __global__ __launch_bounds__(256) void swiglu_checkpoint_kernel(CkptRows p) {
     const int halves = p.padded / 16, per_row = 2 * halves;
     const int64_t first = (int64_t)blockIdx.x * 256, row0 = first / per_row;        // (once per wave, on the scalar unit)
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(256) void swiglu_checkpoint_kernel(CkptRows p) {
     if (r >= p.rows) return;            // (whole blocks of 32: both lanes of one)
     const int in_row = at % (uint32_t)per_row, m = in_row >= halves, c = 16 * (in_row - m * halves);
     float f[16];
-    load_values<E, VEC>((const E*)(m ? p.u : p.g) + r * (m ? p.u_stride : p.g_stride) + c, p.cols - c, f);
+    load_values<E, WHOLE>((const E*)(m ? p.u : p.g) + r * (m ? p.u_stride : p.g_stride) + c, p.cols - c, f);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
@@ -117,7 +118,7 @@ __device__ __forceinline__ void decode(u32x2 q, float scale, float (&f)[8]) {
     for (int i = 0; i < 8; ++i) f[i] = (float)(int)(int8_t)(q[i / 4] >> (8 * (i & 3))) * scale;
 }
 
-template <typename E, bool VEC>
+template <typename E, bool WHOLE>
 __global__ __launch_bounds__(256) void swiglu_checkpoint_read_kernel(CkptRows p) {
     const int eighths = p.padded / 8, per_row = 2 * eighths;
     const int64_t first = (int64_t)blockIdx.x * 256, row0 = first / per_row;
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(256) void swiglu_checkpoint_read_kernel(CkptRows p)
     const int64_t base = (2 * r + m) * p.padded + c;
     float f[8];
     decode(*reinterpret_cast<const u32x2*>(p.q + base), code_scale(p.e[base / 32]), f);
-    store_values<E, VEC>((E*)(m ? p.u : p.g) + r * (m ? p.u_stride : p.g_stride) + c, p.cols - c, f);
+    store_values<E, WHOLE>((E*)(m ? p.u : p.g) + r * (m ? p.u_stride : p.g_stride) + c, p.cols - c, f);
 }
 
 struct CkptBwd {
@@ -145,21 +146,22 @@ struct CkptBwd {
     float* dots;
 };
 
-// A wave per row, eight values a lane.
-template <typename E, bool VEC>
+// Eight values a lane; LANES of a wave to a row (all of them, or as many as a shorter row has eighths, rounded up to a power of two).
+template <typename E, bool WHOLE, int LANES>
 __global__ __launch_bounds__(256) void swiglu_checkpoint_bwd_kernel(CkptBwd p) {
-    const int lane = lane_id();
-    const int64_t waves = (int64_t)gridDim.x * 4;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; r < p.rows; r += waves) {
+    constexpr int ROWS = kWave / LANES;
+    const int lane = lane_id() % LANES;
+    const int64_t step = (int64_t)gridDim.x * 4 * ROWS;
+    for (int64_t r = ((int64_t)blockIdx.x * 4 + threadIdx.x / kWave) * ROWS + lane_id() / LANES; r < p.rows; r += step) {
         const float w = !p.weight ? 1.0f : p.weight_f32 ? reinterpret_cast<const float*>(p.weight)[r] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p.weight)[r]);
         const int8_t* const q = p.q + 2 * r * p.padded;
         const uint8_t* const e = p.e + 2 * r * (p.padded / 32);
         float dot = 0.0f;
-        for (int c = 8 * lane; c < p.cols; c += 8 * kWave) {
+        for (int c = 8 * lane; c < p.cols; c += 8 * LANES) {
             float g[8], u[8], d[8], dg[8], du[8], h[8];
             const u32x2 qg = *reinterpret_cast<const u32x2*>(q + c), qu = *reinterpret_cast<const u32x2*>(q + p.padded + c);
             const int eg = e[c / 32], eu = e[p.padded / 32 + c / 32];
-            load_values<E, VEC>((const E*)p.d + r * p.d_stride + c, p.cols - c, d);
+            load_values<E, WHOLE>((const E*)p.d + r * p.d_stride + c, p.cols - c, d);
             decode(qg, code_scale(eg), g);
             decode(qu, code_scale(eu), u);
 #pragma unroll
@@ -171,15 +173,15 @@ __global__ __launch_bounds__(256) void swiglu_checkpoint_bwd_kernel(CkptBwd p) {
                 dg[i] = dh * u[i] * (s + gs * (1.0f - s));
                 du[i] = dh * gs;
                 h[i] = w * hi;
-                if (VEC || c + i < p.cols) dot = __builtin_fmaf(hi, d[i], dot);
+                if (WHOLE || c + i < p.cols) dot = __builtin_fmaf(hi, d[i], dot);
             }
-            store_values<E, VEC>((E*)p.dg + r * p.dg_stride + c, p.cols - c, dg);
-            store_values<E, VEC>((E*)p.du + r * p.dg_stride + c, p.cols - c, du);
-            if (p.h) store_values<E, VEC>((E*)p.h + r * p.h_stride + c, p.cols - c, h);
+            store_values<E, WHOLE>((E*)p.dg + r * p.dg_stride + c, p.cols - c, dg);
+            store_values<E, WHOLE>((E*)p.du + r * p.dg_stride + c, p.cols - c, du);
+            if (p.h) store_values<E, WHOLE>((E*)p.h + r * p.h_stride + c, p.cols - c, h);
         }
-        if (p.dots) {
+        if (p.dots) {           // (the lanes of a row stay together: they have the same r)
 #pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) dot += __shfl_xor(dot, o, kWave);
+            for (int o = LANES / 2; o >= 1; o >>= 1) dot += __shfl_xor(dot, o, kWave);
             if (lane == 0) p.dots[r] = dot;
         }
     }
@@ -192,7 +194,6 @@ int ckpt_check(const char* name, int dtype, int64_t rows, int64_t cols, const vo
     FMOE_REQUIRE(aligned16(q), "%s: codes must be 16-byte aligned", name);
     return FMOE_OK;
 }
-bool whole_rows(const void* p, int64_t stride, int dtype) { return aligned16(p) && stride * (dtype == FMOE_F32 ? 4 : 2) % 16 == 0; }
 
 }  // namespace
 }  // namespace fmoe
@@ -208,15 +209,15 @@ static int ckpt_both(bool write, const char* name, void* g, void* u, int dtype, 
     FMOE_REQUIRE(g && u, "%s: NULL tensor pointer", name);
     FMOE_REQUIRE(rows == 1 || (g_stride >= cols && u_stride >= cols), "%s: rows overlap", name);
     const CkptRows p{g, u, g_stride, u_stride, rows, (int32_t)cols, (int32_t)fmoe_swiglu_checkpoint_cols(cols), q, e};
-    const bool vec = cols % 8 == 0 && whole_rows(g, g_stride, dtype) && whole_rows(u, u_stride, dtype);
+    const bool whole = cols % 8 == 0;
     const int64_t n = (rows * (2 * p.padded / (write ? 16 : 8)) + 255) / 256;
     FMOE_REQUIRE(n < ((int64_t)1 << 31), "%s: too many values for one call", name);
     const unsigned blocks = (unsigned)n;
     hipStream_t stream = (hipStream_t)stream_;
 #define FMOE_CKPT(kern)                                                                                                    \
     do {                                                                                                                   \
-        if (dtype == FMOE_F32) { if (vec) kern<float, true><<<blocks, 256, 0, stream>>>(p); else kern<float, false><<<blocks, 256, 0, stream>>>(p); } \
-        else { if (vec) kern<uint16_t, true><<<blocks, 256, 0, stream>>>(p); else kern<uint16_t, false><<<blocks, 256, 0, stream>>>(p); }           \
+        if (dtype == FMOE_F32) { if (whole) kern<float, true><<<blocks, 256, 0, stream>>>(p); else kern<float, false><<<blocks, 256, 0, stream>>>(p); } \
+        else { if (whole) kern<uint16_t, true><<<blocks, 256, 0, stream>>>(p); else kern<uint16_t, false><<<blocks, 256, 0, stream>>>(p); }           \
     } while (0)
     if (write) FMOE_CKPT(swiglu_checkpoint_kernel);
     else FMOE_CKPT(swiglu_checkpoint_read_kernel);
@@ -246,17 +247,19 @@ extern "C" int fmoe_swiglu_checkpoint_bwd(const int8_t* q, const uint8_t* e, con
     FMOE_REQUIRE(rows == 1 || (d_stride_row >= cols && dg_stride_row >= cols && (!h || h_stride_row >= cols)), "%s: rows overlap", name);
     const CkptBwd p{q, e, rows, (int32_t)cols, (int32_t)fmoe_swiglu_checkpoint_cols(cols), d, d_stride_row, weight, weight_dtype == FMOE_F32, dg, du, h,
                     dg_stride_row, h_stride_row, dots};
-    const bool vec = cols % 8 == 0 && whole_rows(d, d_stride_row, dtype) && whole_rows(dg, dg_stride_row, dtype) && whole_rows(du, dg_stride_row, dtype) &&
-                     (!h || whole_rows(h, h_stride_row, dtype));
-    const int64_t n = (rows + 3) / 4;
-    const unsigned blocks = (unsigned)(n < 256 * 8 ? n : 256 * 8);
-    hipStream_t stream = (hipStream_t)stream_;
-    if (dtype == FMOE_F32) {
-        if (vec) swiglu_checkpoint_bwd_kernel<float, true><<<blocks, 256, 0, stream>>>(p);
-        else swiglu_checkpoint_bwd_kernel<float, false><<<blocks, 256, 0, stream>>>(p);
-    } else {
-        if (vec) swiglu_checkpoint_bwd_kernel<uint16_t, true><<<blocks, 256, 0, stream>>>(p);
-        else swiglu_checkpoint_bwd_kernel<uint16_t, false><<<blocks, 256, 0, stream>>>(p);
-    }
+    const bool whole = cols % 8 == 0;
+    const int lanes = cols > 256 ? 64 : cols > 64 ? 32 : cols > 16 ? 8 : 2;
+    const int64_t per = 4 * (kWave / lanes), n = (rows + per - 1) / per;
+    auto go = [&](auto kern) { kern<<<(unsigned)(n < 256 * 8 ? n : 256 * 8), 256, 0, (hipStream_t)stream_>>>(p); };
+    auto of = [&](auto value, auto w) {
+        using E = decltype(value);
+        constexpr bool WHOLE = decltype(w)::value;
+        if (lanes == 64) go(swiglu_checkpoint_bwd_kernel<E, WHOLE, 64>);
+        else if (lanes == 32) go(swiglu_checkpoint_bwd_kernel<E, WHOLE, 32>);
+        else if (lanes == 8) go(swiglu_checkpoint_bwd_kernel<E, WHOLE, 8>);
+        else go(swiglu_checkpoint_bwd_kernel<E, WHOLE, 2>);
+    };
+    if (dtype == FMOE_F32) whole ? of(float(), std::true_type()) : of(float(), std::false_type());
+    else whole ? of(uint16_t(), std::true_type()) : of(uint16_t(), std::false_type());
     return check_launch(name);
 }

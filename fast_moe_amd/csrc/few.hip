@@ -34,23 +34,29 @@ struct FewParams {
     float* partial;
 };
 
-enum { kWF32 = 0, kWBF16 = 1, kWE4M3 = 2 };
+enum { kWF32 = 0, kWBF16 = 1, kWE4M3 = 2, kWE4M3Half = 3 };       // Half: rows of e4m3 that are whole chunks of 8 bytes only
 
-// Elements of a 16-byte chunk, bytes of an element, and chunks of x that go with one of weights
+// Elements of a lane's chunk (16 bytes, 8 for Half), bytes of an element, and 16-byte chunks of x that go with one of weights
 template <int WT> struct Wt;
 template <> struct Wt<kWF32> { static constexpr int CE = 4, ES = 4, XES = 4, XC = 1; };
 template <> struct Wt<kWBF16> { static constexpr int CE = 8, ES = 2, XES = 2, XC = 1; };
 template <> struct Wt<kWE4M3> { static constexpr int CE = 16, ES = 1, XES = 2, XC = 2; };
+template <> struct Wt<kWE4M3Half> { static constexpr int CE = 8, ES = 1, XES = 2, XC = 1; };
 
-// 16 bytes of a row of n elements of ES bytes from element k on, zeros behind its end.  VEC: rows are whole chunks at 16-byte boundaries.
-template <int ES, bool VEC>
+// A chunk (BYTES: 16 or 8) of a row of n elements of ES bytes from element k on, zeros behind its end.  VEC: rows are whole chunks at its boundaries.
+template <int ES, bool VEC, int BYTES = 16>
 __device__ __forceinline__ u32x4 chunk(const uint8_t* row, int k, int n) {
     u32x4 v = {0, 0, 0, 0};
-    if constexpr (VEC) {
+    if constexpr (VEC && BYTES == 8) {
+        if (k < n) {
+            const u32x2 h = *reinterpret_cast<const u32x2*>(row + (int64_t)k * ES);
+            v = u32x4{h[0], h[1], 0, 0};
+        }
+    } else if constexpr (VEC) {
         if (k < n) v = *reinterpret_cast<const u32x4*>(row + (int64_t)k * ES);
     } else {
 #pragma unroll
-        for (int i = 0; i < 16 / ES; ++i) {
+        for (int i = 0; i < BYTES / ES; ++i) {
             if (k + i >= n) continue;
             const uint8_t* p = row + (int64_t)(k + i) * ES;
             if constexpr (ES == 4) v[i] = *reinterpret_cast<const uint32_t*>(p);
@@ -62,7 +68,7 @@ __device__ __forceinline__ u32x4 chunk(const uint8_t* row, int k, int n) {
 }
 // Rows behind a base address that is the same in all lanes, each at a byte offset of its own (below 2^31: few_check).  Whole chunks come through a
 // buffer descriptor: an offset beyond its range reads as zeros, which makes the end of a row one select in the place of a branch around every load.
-template <int ES, bool VEC>
+template <int ES, bool VEC, int BYTES = 16>
 struct Rows {
     const uint8_t* base;
     __amdgpu_buffer_rsrc_t buffer;
@@ -71,8 +77,14 @@ struct Rows {
         if constexpr (VEC) buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0x7ffffff0, 0x00027000);
     }
     __device__ __forceinline__ u32x4 chunk(uint32_t row, int k, int n) const {
-        if constexpr (VEC) return __builtin_amdgcn_raw_buffer_load_b128(buffer, k < n ? (int)(row + (uint32_t)k * ES) : -1, 0, 0);
-        else return fmoe::chunk<ES, false>(base + row, k, n);
+        if constexpr (VEC && BYTES == 8) {
+            const u32x2 h = __builtin_amdgcn_raw_buffer_load_b64(buffer, k < n ? (int)(row + (uint32_t)k * ES) : -1, 0, 0);
+            return u32x4{h[0], h[1], 0, 0};
+        } else if constexpr (VEC) {
+            return __builtin_amdgcn_raw_buffer_load_b128(buffer, k < n ? (int)(row + (uint32_t)k * ES) : -1, 0, 0);
+        } else {
+            return fmoe::chunk<ES, false, BYTES>(base + row, k, n);
+        }
     }
 };
 
@@ -97,6 +109,8 @@ __device__ __forceinline__ void mma(f32x4& acc, const u32x4& w, const u32x4* x) 
             acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[j]), __uint_as_float(x[0][j]), acc, 0, 0, 0);
     } else if constexpr (WT == kWBF16) {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x[0]), acc, 0, 0, 0);
+    } else if constexpr (WT == kWE4M3Half) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3_to_bf16(w[0], w[1]), __builtin_bit_cast(bf16x8, x[0]), acc, 0, 0, 0);
     } else {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3_to_bf16(w[0], w[1]), __builtin_bit_cast(bf16x8, x[0]), acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3_to_bf16(w[2], w[3]), __builtin_bit_cast(bf16x8, x[1]), acc, 0, 0, 0);
@@ -384,7 +398,7 @@ __device__ __forceinline__ void build_lists(const fmoe_few_desc& d, const FewLis
 
 template <int WT, bool VEC, int NT, bool GATED>
 __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int share_bits) {
-    constexpr bool F32 = WT == kWF32;
+    constexpr bool F32 = WT == kWF32, E4M3 = WT == kWE4M3 || WT == kWE4M3Half;
     constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, MATS = GATED ? 2 : 1;
     constexpr int AHEAD = !VEC || NT * XC * MATS > 2 ? 2 : 3;    // batches of loads in flight
     constexpr int ROUND = NT == 1 ? MATS : 1;           // matrices whose sums are in LDS at a time
@@ -440,7 +454,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
     Item loading = {(start + group) / tiles, (start + group) % tiles}, adding = loading;
     const int total = entries * tiles, rounds = start < total ? (total - start + stride - 1) / stride : 0;
     // What is loaded runs AHEAD batches before what is multiplied, over the ends of items.
-    Rows<ES, VEC> w[MATS];
+    Rows<ES, VEC, CE * ES> w[MATS];
     Rows<XES, VEC> x;
     x.at(d.x);
     uint32_t wrow = 0, xrow[NT];
@@ -514,7 +528,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
                 const void* const b = m ? d.bias_p : d.bias;
                 const int col = min(col0 + i, d.H - 1);
                 bias[m][i] = any && b ? element<F32>(b, (int64_t)at.e * d.bias_stride_e + col) : 0.0f;
-                if constexpr (WT == kWE4M3) div[m][i] = any ? (m ? d.wp_scale : d.w_scale)[(int64_t)at.e * d.H + col] : 1.0f;
+                if constexpr (E4M3) div[m][i] = any ? (m ? d.wp_scale : d.w_scale)[(int64_t)at.e * d.H + col] : 1.0f;
             }
         f32x4 sum[MATS][NT];
 #pragma unroll
@@ -556,11 +570,11 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float a = sum[0][f][i];
-                if constexpr (WT == kWE4M3) a /= div[0][i];
+                if constexpr (E4M3) a /= div[0][i];
                 v[i] = silu_f32(a + bias[0][i]);
                 if constexpr (GATED) {
                     float u = sum[1][f][i];
-                    if constexpr (WT == kWE4M3) u /= div[1][i];
+                    if constexpr (E4M3) u /= div[1][i];
                     v[i] *= u + bias[1][i];
                 }
                 v[i] *= g;
@@ -607,7 +621,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 // gridDim.y > 1: so many blocks share a tile's contraction; their sums go through memory, and the one that arrives last adds them in block order.
 template <int WT, bool VEC, int NT, int PARTS>
 __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
-    constexpr bool F32 = WT == kWF32, ONE = PARTS == 1;
+    constexpr bool F32 = WT == kWF32, E4M3 = WT == kWE4M3 || WT == kWE4M3Half, ONE = PARTS == 1;
     constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, COLS = 16 / PARTS;
     constexpr int AHEAD = !VEC ? 1 : NT * XC == 1 ? 4 : NT * XC == 2 ? 3 : 2;      // pieces whose loads are in flight
     extern __shared__ uint8_t lds[];
@@ -628,7 +642,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
     Entry next = {0, 0, 0}, cur = {0, 0, 0};            // whose loads are on their way, and whose products add up
     int next_index = -1, cur_index = -1, of[AHEAD];
     const uint8_t *wrow = nullptr, *xrow[NT] = {};
-    Rows<ES, VEC> w;
+    Rows<ES, VEC, CE * ES> w;
     Rows<XES, VEC> x;
     uint32_t xoff[NT] = {};
     w.at(d.wo);
@@ -656,7 +670,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             if constexpr (ONE) wb[s] = w.chunk(woff, k + s * STEP, any ? d.H : 0);
-            else wb[s] = chunk<ES, VEC>(wrow, k + s * STEP, any ? d.H : 0);
+            else wb[s] = chunk<ES, VEC, CE * ES>(wrow, k + s * STEP, any ? d.H : 0);
         }
 #pragma unroll
         for (int f = 0; f < NT; ++f)
@@ -688,7 +702,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
                     f32x4* const to = reinterpret_cast<f32x4*>(sums + ((size_t)wave * d.T + l.slots[cur.first + c] / d.k) * 16 + 4 * quarter);
                     f32x4 v = *to;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] += WT == kWE4M3 ? acc[f][i] / inv[i] : acc[f][i];
+                    for (int i = 0; i < 4; ++i) v[i] += E4M3 ? acc[f][i] / inv[i] : acc[f][i];
                     *to = v;
                 }
             }
@@ -706,7 +720,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
                 if (of[i] >= 0) {
                     cur = few_entry<ONE>(l, of[i]);
                     cur_index = of[i];
-                    if constexpr (WT == kWE4M3)
+                    if constexpr (E4M3)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) inv[j] = d.wo_scale[(int64_t)cur.e * d.O + min(n0 + (4 * quarter + j) % COLS, d.O - 1)];
                 }
@@ -831,11 +845,14 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
                       (int32_t*)((uint8_t*)workspace + few_arrivals_at(d)),
                       (float*)((uint8_t*)workspace + few_arrivals_at(d) + (((size_t)plan.tiles * 4 + 255) & ~(size_t)255))};
     const int es = d.dtype == FMOE_F32 ? 4 : 2, wes = d.weight_dtype == FMOE_E4M3 ? 1 : es;
-    // whole 16-byte chunks at 16-byte boundaries wherever rows are read
-    auto whole = [](const void* q, int64_t elements, int size) { return aligned16(q) && elements * size % 16 == 0; };
-    const bool vec = whole(d.x, d.D, es) && whole(d.x, d.x_stride_row, es) && whole(d.gate_weight, d.gate_stride_row, es) && whole(d.w, d.D, wes) &&
-                     whole(d.w, d.w_stride_n, wes) && whole(d.w, d.w_stride_e, wes) && whole(d.wp, d.D, wes) && whole(d.wo, d.H, wes) &&
-                     whole(d.wo, d.wo_stride_n, wes) && whole(d.wo, d.wo_stride_e, wes) && d.H * es % 16 == 0;
+    // whole chunks at their boundaries wherever rows are read: 16 bytes, 8 of e4m3 weights where it comes to that
+    auto whole = [](const void* q, int64_t elements, int size, int chunk) { return ((uintptr_t)q & (chunk - 1)) == 0 && elements * size % chunk == 0; };
+    auto weights = [&](int chunk) {
+        return whole(d.w, d.D, wes, chunk) && whole(d.w, d.w_stride_n, wes, chunk) && whole(d.w, d.w_stride_e, wes, chunk) && whole(d.wp, d.D, wes, chunk) &&
+               whole(d.wo, d.H, wes, chunk) && whole(d.wo, d.wo_stride_n, wes, chunk) && whole(d.wo, d.wo_stride_e, wes, chunk);
+    };
+    const bool rows = whole(d.x, d.D, es, 16) && whole(d.x, d.x_stride_row, es, 16) && whole(d.gate_weight, d.gate_stride_row, es, 16) && d.H * es % 16 == 0;
+    const bool vec = rows && weights(16), half = rows && wes == 1 && weights(8);
     const bool gated = d.wp != nullptr;
     const int most_active = d.T * d.k < d.E ? d.T * d.k : d.E;
     hipStream_t stream = (hipStream_t)stream_;
@@ -885,7 +902,7 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     } else if (d.weight_dtype == FMOE_BF16) {
         if (vec) FMOE_FEW(kWBF16, true); else FMOE_FEW(kWBF16, false);
     } else {
-        if (vec) FMOE_FEW(kWE4M3, true); else FMOE_FEW(kWE4M3, false);
+        if (vec) FMOE_FEW(kWE4M3, true); else if (half) FMOE_FEW(kWE4M3Half, true); else FMOE_FEW(kWE4M3, false);
     }
 #undef FMOE_FEW
 #undef FMOE_FEW_UP

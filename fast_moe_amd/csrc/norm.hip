@@ -34,37 +34,50 @@ __device__ __forceinline__ float to_f32(uint16_t v) { return bf16_bits_to_f32(v)
 __device__ __forceinline__ void from_f32(float* p, float v) { *p = v; }
 __device__ __forceinline__ void from_f32(uint16_t* p, float v) { *p = (uint16_t)f32_to_bf16_bits(v); }
 
-// Which columns a lane holds: VEC: chunks of V neighbours, 16 bytes; otherwise single ones, neighbours in neighbouring lanes.
-template <typename E, bool VEC, int CH>
+// 16 bytes at any address an element may have (the hardware takes them at every alignment)
+__device__ __forceinline__ u32x4 load16(const void* p) {
+    u32x4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+__device__ __forceinline__ void store16(void* p, const u32x4& v) { __builtin_memcpy(p, &v, 16); }
+
+// Which columns a lane holds: chunks of V neighbours, 16 bytes.  WHOLE: rows are whole chunks; otherwise bf16's last one is read and written by elements, and
+// fp32 goes by elements altogether, neighbours in neighbouring lanes (16 bytes at addresses between the chunks' are slower: 3063 x 1001, forward and
+// backward 64 us against 49; in bf16, where an element is 2 bytes, faster: 12975 x 1822 forward 74 us against 102).
+template <typename E, bool WHOLE, int CH>
 struct Row {
     static constexpr int V = NE<E>::V, N = V * CH;
-    // what has been loaded and not been looked at: the chunks, or the values
-    struct Raw {
-        u32x4 v[VEC ? CH : 1];
-        E e[VEC ? 1 : N];
+    static constexpr bool ELEMENTS = !WHOLE && V == 4;
+    struct Raw {            // what has been loaded and not been looked at
+        u32x4 v[CH];
     };
     int tid, threads, cols;
-    __device__ __forceinline__ int col(int i) const {
-        return VEC ? ((i / V) * threads + tid) * V + i % V : i * threads + tid;
-    }
-    __device__ __forceinline__ bool in(int i) const { return col(i) < cols; }       // (VEC: all of a chunk or none)
+    __device__ __forceinline__ int col(int i) const { return ELEMENTS ? i * threads + tid : ((i / V) * threads + tid) * V + i % V; }
+    __device__ __forceinline__ bool in(int i) const { return col(WHOLE ? i / V * V : i) < cols; }
+    __device__ __forceinline__ bool whole(int c) const { return WHOLE ? in(c * V) : !ELEMENTS && col(c * V) + V <= cols; }
     __device__ __forceinline__ void fetch(const E* p, Raw& r) const {
-        if constexpr (VEC) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                r.v[c] = u32x4{0, 0, 0, 0};
-                if (in(c * V)) r.v[c] = *reinterpret_cast<const u32x4*>(p + col(c * V));
+        for (int c = 0; c < CH; ++c) {
+            if constexpr (ELEMENTS) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) r.v[c][i] = in(c * V + i) ? __float_as_uint(p[col(c * V + i)]) : 0u;
+                continue;
             }
-        } else {
+            r.v[c] = u32x4{0, 0, 0, 0};
+            if (whole(c)) {
+                r.v[c] = load16(p + col(c * V));
+            } else if (!WHOLE && in(c * V)) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) r.e[i] = in(i) ? p[col(i)] : E(0);
+                for (int i = 0; i < V; ++i)
+                    if (in(c * V + i)) r.v[c][i / 2] |= (uint32_t)p[col(c * V + i)] << (16 * (i & 1));
+            }
         }
     }
     __device__ __forceinline__ void take(const Raw& r, float (&f)[N]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if constexpr (!VEC) f[i] = to_f32(r.e[i]);
-            else if constexpr (V == 4) f[i] = __uint_as_float(r.v[i / V][i % V]);
+            if constexpr (V == 4) f[i] = __uint_as_float(r.v[i / V][i % V]);
             else f[i] = i & 1 ? __uint_as_float(r.v[i / V][i % V / 2] & 0xffff0000u) : __uint_as_float(r.v[i / V][i % V / 2] << 16);
         }
     }
@@ -74,28 +87,22 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] = all[c * V + i];
     }
-    __device__ __forceinline__ void load(const E* p, float (&f)[N]) const {
-        Raw r;
-        fetch(p, r);
-        take(r, f);
-    }
     __device__ __forceinline__ void store(E* p, const float (&f)[N]) const {
-        if constexpr (VEC) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                if (!in(c * V)) continue;
+        for (int c = 0; c < CH; ++c) {
+            if (whole(c)) {
                 u32x4 v;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if constexpr (V == 4) v[i] = __float_as_uint(f[c * V + i]);
                     else v[i] = cvt_pk_bf16(f[c * V + 2 * i], f[c * V + 2 * i + 1]);
                 }
-                *reinterpret_cast<u32x4*>(p + col(c * V)) = v;
-            }
-        } else {
+                store16(p + col(c * V), v);
+            } else if (!WHOLE) {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (in(i)) from_f32(p + col(i), f[i]);
+                for (int i = 0; i < V; ++i)
+                    if (in(c * V + i)) from_f32(p + col(c * V + i), f[c * V + i]);
+            }
         }
     }
     // a parameter of the columns of chunk c, in fp32 or bf16 whatever the rows are
@@ -103,21 +110,16 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] = none;
         if (!p) return;
-        if constexpr (VEC) {
-            if (!in(c * V)) return;
+        if (whole(c)) {
+            if (dtype == FMOE_F32) {
+                __builtin_memcpy(f, (const float*)p + col(c * V), sizeof(f));
+            } else {
+                uint16_t h[V];
+                __builtin_memcpy(h, (const uint16_t*)p + col(c * V), sizeof(h));
 #pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                if (dtype == FMOE_F32) {
-                    const f32x4 v = *reinterpret_cast<const f32x4*>((const float*)p + col(c * V) + i);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) f[i + j] = v[j];
-                } else {
-                    const u32x2 v = *reinterpret_cast<const u32x2*>((const uint16_t*)p + col(c * V) + i);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) f[i + j] = j & 1 ? __uint_as_float(v[j / 2] & 0xffff0000u) : __uint_as_float(v[j / 2] << 16);
-                }
+                for (int i = 0; i < V; ++i) f[i] = bf16_bits_to_f32(h[i]);
             }
-        } else {
+        } else if (!WHOLE) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int at = col(c * V + i);
@@ -212,9 +214,9 @@ struct Param {
 };
 
 // y given, or none (only the next norm).
-template <typename E, bool VEC, int CH>
+template <typename E, bool WHOLE, int CH>
 __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_norm_desc d, int waves) {
-    using R = Row<E, VEC, CH>;
+    using R = Row<E, WHOLE, CH>;
     using P = Param<R, CH == 1>;
     constexpr int N = R::N, V = R::V;
     __shared__ float buf[2][kNormMostWaves][4];
@@ -298,9 +300,9 @@ struct MergeParams {
     void *out, *next, *y_out;
     float* stats;
 };
-template <typename E, bool VEC, int CH, bool LAYER, bool P32, int BATCH>
+template <typename E, bool WHOLE, int CH, bool LAYER, bool P32, int BATCH>
 __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(MergeParams p, int waves) {
-    using R = Row<E, VEC, CH>;
+    using R = Row<E, WHOLE, CH>;
     constexpr int V = R::V, N = R::N;
     __shared__ float buf[2][kNormMostWaves][4];
     const int per = waves == 1 ? blockDim.x / kWave : 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
@@ -408,9 +410,9 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(Merge
 enum { kDScale = 0, kDWeight, kDNextWeight, kDBias, kDNextBias, kSums };
 
 // The next row's loads are issued before this row's sums are exchanged.
-template <typename E, bool VEC, int CH, bool LAYER, bool ELEMENT, int THREADS>
+template <typename E, bool WHOLE, int CH, bool LAYER, bool ELEMENT, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d, int waves, float* partial) {
-    using R = Row<E, VEC, CH>;
+    using R = Row<E, WHOLE, CH>;
     using P = Param<R, CH == 1>;
     constexpr int N = R::N, V = R::V, SUMS = LAYER ? kSums : 3;       // rms norm: no biases
     __shared__ float buf[2][kNormMostWaves][4];
@@ -585,25 +587,21 @@ __global__ __launch_bounds__(kSumWaves* kWave) void norm_sums_kernel(fmoe_norm_d
 constexpr int kNormMostCols = 8192, kNormBwdWaves = 8;
 
 struct NormPlan {
-    bool vec;
+    bool whole;
     int chunks, waves, per, threads;
 };
 // Chunks of a lane and waves of a row: one chunk, the row spread over as many lanes as it has chunks, as far as 16 waves (8 in the backward pass, whose
 // sums over rows take registers) go.  A row per wave of four chunks each, with no barrier, was slower: 16384 x 2048 bf16 forward 97 us against 67 (the
 // parameters are asked for again for every row, and 245 registers leave two waves to a SIMD).
 NormPlan norm_plan(const fmoe_norm_desc& d, bool backward) {
-    const int v = d.dtype == FMOE_F32 ? 4 : 8, es = d.dtype == FMOE_F32 ? 4 : 2;
-    auto whole = [&](const void* p, int64_t stride) { return aligned16(p) && stride * es % 16 == 0; };
+    const int v = d.dtype == FMOE_F32 ? 4 : 8;
     NormPlan p;
-    p.vec = d.cols % v == 0 && whole(d.y, d.y_stride) && whole(d.residual, d.residual_stride) && whole(d.out, 0) && whole(d.next, 0) && whole(d.y_out, 0) &&
-            (d.gate_mode != FMOE_GATE_ELEMENT || whole(d.gate, d.gate_stride)) && whole(d.d_out, 0) && whole(d.d_next, 0) && whole(d.d_y, 0) &&
-            whole(d.d_residual, 0) && (d.gate_mode != FMOE_GATE_ELEMENT || whole(d.d_gate, 0)) && aligned16(d.scale) && aligned16(d.weight) &&
-            aligned16(d.bias) && aligned16(d.next_weight) && aligned16(d.next_bias);
+    p.whole = d.cols % v == 0;
     const int lanes = (d.cols + v - 1) / v;                      // one chunk each
     auto waves = [&](int chunks) { return (lanes + chunks * kWave - 1) / (chunks * kWave); };
     p.chunks = 1;
     if (backward) {
-        while (waves(p.chunks) > (p.vec ? kNormBwdWaves : kNormMostWaves)) p.chunks *= 2;
+        while (waves(p.chunks) > (p.whole ? kNormBwdWaves : kNormMostWaves)) p.chunks *= 2;
     } else if (waves(1) > kNormMostWaves) {
         p.chunks = 2;
     }
@@ -675,34 +673,34 @@ extern "C" int fmoe_norm_add(const fmoe_norm_desc* desc, fmoe_stream_t stream) {
                             d.gate_mode && d.gate_sigmoid, d.eps, d.scale_value, d.y, d.residual, d.gate, d.merge, d.scale, d.weight, d.bias, d.next_weight, d.next_bias,
                             d.reverse_index, d.merge_index, d.out, d.next, d.y_out, d.stats};
         auto run = [&](auto kern) { kern<<<(unsigned)(blocks < most ? blocks : most), p.threads, 0, (hipStream_t)stream>>>(m, p.waves); };
-        auto of = [&](auto value, auto vec, auto layer, auto p32) {
+        auto of = [&](auto value, auto whole, auto layer, auto p32) {
             using E = decltype(value);
-            constexpr bool VEC = decltype(vec)::value, LAYER = decltype(layer)::value, P32 = decltype(p32)::value;
+            constexpr bool WHOLE = decltype(whole)::value, LAYER = decltype(layer)::value, P32 = decltype(p32)::value;
             if constexpr (sizeof(E) == 4) {
-                if (p.chunks == 2) return run(norm_merge_kernel<E, VEC, 2, LAYER, P32, 2>);
+                if (p.chunks == 2) return run(norm_merge_kernel<E, WHOLE, 2, LAYER, P32, 2>);
             }
-            if constexpr (VEC) {
-                if (d.K <= 2) return run(norm_merge_kernel<E, VEC, 1, LAYER, P32, 2>);
-                if (d.K > 4) return run(norm_merge_kernel<E, VEC, 1, LAYER, P32, 8>);
+            if constexpr (WHOLE) {
+                if (d.K <= 2) return run(norm_merge_kernel<E, WHOLE, 1, LAYER, P32, 2>);
+                if (d.K > 4) return run(norm_merge_kernel<E, WHOLE, 1, LAYER, P32, 8>);
             }
             // (a row read element by element takes a register for every one)
-            run(norm_merge_kernel<E, VEC, 1, LAYER, P32, VEC || sizeof(E) == 4 ? 4 : 2>);
+            run(norm_merge_kernel<E, WHOLE, 1, LAYER, P32, WHOLE || sizeof(E) == 4 ? 4 : 2>);
         };
-        with_bool(p.vec, [&](auto vec) {
+        with_bool(p.whole, [&](auto whole) {
             with_bool(d.norm == FMOE_NORM_LAYER, [&](auto layer) {
                 with_bool(d.param_dtype == FMOE_F32, [&](auto p32) {
-                    if (d.dtype == FMOE_F32) of(float(), vec, layer, p32);
-                    else of(uint16_t(), vec, layer, p32);
+                    if (d.dtype == FMOE_F32) of(float(), whole, layer, p32);
+                    else of(uint16_t(), whole, layer, p32);
                 });
             });
         });
         return check_launch("fmoe_norm_add");
     }
-    with_bool(p.vec, [&](auto vec) {
-        constexpr bool VEC = decltype(vec)::value;
-        if (d.dtype == FMOE_BF16) go(norm_add_kernel<uint16_t, VEC, 1>);
-        else if (p.chunks == 1) go(norm_add_kernel<float, VEC, 1>);
-        else go(norm_add_kernel<float, VEC, 2>);
+    with_bool(p.whole, [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        if (d.dtype == FMOE_BF16) go(norm_add_kernel<uint16_t, WHOLE, 1>);
+        else if (p.chunks == 1) go(norm_add_kernel<float, WHOLE, 1>);
+        else go(norm_add_kernel<float, WHOLE, 2>);
     });
     return check_launch("fmoe_norm_add");
 }
@@ -725,19 +723,19 @@ extern "C" int fmoe_norm_add_bwd(const fmoe_norm_desc* desc, void* workspace, si
     float* const partial = need ? (float*)workspace : nullptr;
     const int blocks = (norm_groups(d, p) + p.per - 1) / p.per;
     auto go = [&](auto kern) { kern<<<blocks, p.threads, 0, (hipStream_t)stream>>>(d, p.waves, partial); };
-    with_bool(p.vec, [&](auto vec) {
+    with_bool(p.whole, [&](auto whole) {
         with_bool(d.norm == FMOE_NORM_LAYER || d.bias || d.next_bias, [&](auto layer) {
             with_bool(d.gate_mode == FMOE_GATE_ELEMENT, [&](auto element) {
-                constexpr bool VEC = decltype(vec)::value, LAYER = decltype(layer)::value, ELEMENT = decltype(element)::value;
-                constexpr int THREADS = VEC ? kNormBwdWaves * kWave : kNormMostWaves * kWave;
+                constexpr bool WHOLE = decltype(whole)::value, LAYER = decltype(layer)::value, ELEMENT = decltype(element)::value;
+                constexpr int THREADS = WHOLE ? kNormBwdWaves * kWave : kNormMostWaves * kWave;
                 if (d.dtype == FMOE_F32) {
-                    if (p.chunks == 1) go(norm_add_bwd_kernel<float, VEC, 1, LAYER, ELEMENT, THREADS>);
-                    else if (p.chunks == 2) go(norm_add_bwd_kernel<float, VEC, 2, LAYER, ELEMENT, THREADS>);
-                    else if constexpr (VEC) go(norm_add_bwd_kernel<float, VEC, 4, LAYER, ELEMENT, THREADS>);
+                    if (p.chunks == 1) go(norm_add_bwd_kernel<float, WHOLE, 1, LAYER, ELEMENT, THREADS>);
+                    else if (p.chunks == 2) go(norm_add_bwd_kernel<float, WHOLE, 2, LAYER, ELEMENT, THREADS>);
+                    else if constexpr (WHOLE) go(norm_add_bwd_kernel<float, WHOLE, 4, LAYER, ELEMENT, THREADS>);
                 } else {
-                    if (p.chunks == 1 && p.waves <= kNormBwdWaves) go(norm_add_bwd_kernel<uint16_t, VEC, 1, LAYER, ELEMENT, kNormBwdWaves * kWave>);
-                    else if (p.chunks == 1) go(norm_add_bwd_kernel<uint16_t, VEC, 1, LAYER, ELEMENT, THREADS>);
-                    else if constexpr (VEC) go(norm_add_bwd_kernel<uint16_t, VEC, 2, LAYER, ELEMENT, THREADS>);
+                    if (p.chunks == 1 && p.waves <= kNormBwdWaves) go(norm_add_bwd_kernel<uint16_t, WHOLE, 1, LAYER, ELEMENT, kNormBwdWaves * kWave>);
+                    else if (p.chunks == 1) go(norm_add_bwd_kernel<uint16_t, WHOLE, 1, LAYER, ELEMENT, THREADS>);
+                    else if constexpr (WHOLE) go(norm_add_bwd_kernel<uint16_t, WHOLE, 2, LAYER, ELEMENT, THREADS>);
                 }
             });
         });

@@ -169,7 +169,7 @@ int fmoe_gate_route_pays(int dtype, int64_t T, int D, int E, int K);
  * g * h is rounded to dtype in between (bf16: half a step of 2^-8).  A token whose token_mask byte is 0 reads no expert and gets a row of zeros.
  * dtype (tokens, gate, biases, output): FMOE_BF16 or FMOE_F32; weight_dtype: the same, or FMOE_E4M3 with bf16 tokens, which are not
  * quantised (products in bf16, divided by the multiplier scales).  k contiguous in every weight.  Rows of whole 16-byte chunks at 16-byte
- * boundaries are read 16 bytes at a time, others element by element (an order of magnitude slower).  The same inputs give the same bits.
+ * boundaries (8 bytes of e4m3) are read a chunk at a time, others element by element (an order of magnitude slower).  The same inputs give the same bits.
  */
 typedef struct fmoe_few_desc {
     int32_t T, E, k;            /* T <= 64, E <= 256, k <= 16                          */
