@@ -414,12 +414,14 @@ template <typename E, bool WHOLE, int CH, bool LAYER, bool ELEMENT, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d, int waves, float* partial) {
     using R = Row<E, WHOLE, CH>;
     using P = Param<R, CH == 1>;
-    constexpr int N = R::N, V = R::V, SUMS = LAYER ? kSums : 3;       // rms norm: no biases
+    constexpr int N = R::N, V = R::V, SUMS = LAYER ? kSums : 3;       // LAYER: a layer norm, or an rms norm with biases
     __shared__ float buf[2][kNormMostWaves][4];
     const int per = waves == 1 ? blockDim.x / kWave : 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const R row{waves == 1 ? (int)threadIdx.x % kWave : (int)threadIdx.x, waves * kWave, d.cols};
     Exchange x{buf, waves, wave, 0};
     const float inv = 1.0f / (float)d.cols;
+    const bool centred = d.norm == FMOE_NORM_LAYER;
+    auto mean_of = [&](float s) { return LAYER && centred ? s * inv : 0.0f; };
     const P scale(row, d.scale, d.param_dtype, d.scale_value), weight(row, d.weight, d.param_dtype, 1.0f), bias(row, LAYER ? d.bias : nullptr, d.param_dtype, 0.0f),
         next_weight(row, d.next_weight, d.param_dtype, 0.0f);
     float sums[SUMS][N];
@@ -498,7 +500,7 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
             }
             x.sum(s);
 #pragma unroll
-            for (int i = 0; i < N; ++i) dt[i] += r2 * (dn[i] - o[i] * (s[0] * inv) - (LAYER ? s[1] * inv : 0.0f));
+            for (int i = 0; i < N; ++i) dt[i] += r2 * (dn[i] - o[i] * (s[0] * inv) - mean_of(s[1]));
         }
         if (d.d_residual) row.store((E*)d.d_residual + t * d.cols, dt);
         if (d.y) {
@@ -535,7 +537,7 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
             if (d.d_y) {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (d.weight) dt[i] = r * (dt[i] - a[i] * (q[0] * inv) - (LAYER ? q[1] * inv : 0.0f));
+                    if (d.weight) dt[i] = r * (dt[i] - a[i] * (q[0] * inv) - mean_of(q[1]));
                 row.store((E*)d.d_y + t * d.cols, dt);
             }
         }

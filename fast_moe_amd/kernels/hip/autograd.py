@@ -26,6 +26,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from ._lib import EPI_NONE, EPI_SWIGLU
@@ -476,6 +477,7 @@ class NormAdd(torch.autograd.Function):
         return out, nxt
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out, d_next):
         index, merge_index, merge, y, merged, residual, weight, bias, gate, scale, next_weight, next_bias, stats = ctx.saved_tensors
         gate_sigmoid, value, eps, norm, K = ctx.rest
@@ -518,6 +520,7 @@ class SwigluBlockCheckpoint8(torch.autograd.Function):
         return ops.combine(value, reverse_index, gates, gates_index)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         offsets, index, jagged, weight, bias, weight_p, bias_p, weight_out, bias_out, gates, gates_index, q, e = ctx.saved_tensors
         kept = ops.SwigluCheckpoint(q, e, *ctx.kept)
@@ -538,8 +541,8 @@ class SwigluBlockCheckpoint8(torch.autograd.Function):
             d_wo = _WgradOperand(h, offsets, flat.numel()).weight_grad(dr, weight_out)
         if bias_out is not None and (need[8] or need_g):
             token = torch.div(flat, K, rounding_mode="floor")
-            lengths = (offsets[1:] - offsets[:-1]).clamp_min(0)
-            expert = torch.repeat_interleave(torch.arange(lengths.numel(), device=flat.device), lengths, output_size=flat.numel())
+            # (an expert in range for every row, whatever the offsets say)
+            expert = torch.searchsorted(offsets[1:], torch.arange(flat.numel(), device=flat.device), right=True).clamp_max(offsets.numel() - 2)
             d_value, d_flat = ops.combine_bwd(dy, bias_out[expert] if need_g else None, token, K, gates, gates_index, need_gate_grad=need_g)
             if need[8]:
                 d_bo = ops.segment_colsum(d_value, offsets)

@@ -348,3 +348,72 @@ def test_refusals():
         moe.mul_merge_k_norm_add(merge["index"][:7], merge["reverse"], p["y"], r)
     with pytest.raises(NotImplementedError, match="not available"):
         moe.block_norm(r, p["weight"], kernel=moe.KernelType.PYTORCH)
+
+
+@pytest.mark.parametrize("T,D", [(3, 7), (5, 64), (4, 2048), (3, 8192)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("gate", ["none", "token", "element"])
+def test_rms_norm_with_biases(T, D, dtype, gate):
+    p, _ = make(T, D, dtype, "layer", gate, seed=T + D + 1)         # (both biases, which "rms" takes as well)
+    for t in p.values():
+        t.requires_grad_(True)
+    out, nxt = call(p, None, "rms", False)
+    d_out, d_next = (torch.randn(T, D, device="cuda").to(dtype) for _ in range(2))
+    torch.autograd.backward((out, nxt), (d_out, d_next))
+    want = formula(p, None, "rms", False, d_out, d_next)
+    close("out", out, want["out"])
+    close("next", nxt, want["next"])
+    for n, t in p.items():
+        close("d_" + n, t.grad, want["d_" + n])
+
+
+def test_gradients_against_differences():
+    T, D, step = 3, 24, 2.0 ** -6
+    p, _ = make(T, D, F32, "layer", "element", seed=11)
+    g = torch.Generator().manual_seed(12)
+    d_out, d_next = (torch.randn(T, D, generator=g).cuda() for _ in range(2))
+    for t in p.values():
+        t.requires_grad_(True)
+    torch.autograd.backward(call(p, None, "layer", True), (d_out, d_next))
+    for n, t in p.items():
+        direction = torch.randn(t.shape, generator=g).cuda()
+
+        def loss(by):
+            out, nxt = call({m: (v + by * direction if m == n else v).detach() for m, v in p.items()}, None, "layer", True)
+            return ((out.double() * d_out).sum() + (nxt.double() * d_next).sum()).item()
+
+        slope = (8 * (loss(step) - loss(-step)) - (loss(2 * step) - loss(-2 * step))) / (12 * step)      # error of step^4 = 2^-24 of the fifth derivative
+        want = (t.grad.double() * direction).sum().item()
+        # values of a few units in fp32, 150 of them, differences over 2^-6: 2^-24 * 4 * 12 * 64 of noise; the fifth derivative of a norm or sigmoid of
+        # such rows is within a few hundred
+        assert abs(slope - want) <= 2e-3 * (1 + abs(want)), (n, slope, want)
+
+
+def test_no_rows_strided_operands_and_no_second_derivative():
+    p, _ = make(1, 64, F32, "layer", "token", seed=1)
+    p = {n: (t if t.ndim == 1 else t[:0]).detach().requires_grad_(True) for n, t in p.items()}
+    out, nxt = call(p, None, "layer", False)
+    torch.autograd.backward((out, nxt), (torch.ones_like(out), torch.ones_like(nxt)))
+    assert out.shape == nxt.shape == (0, 64) and all(t.grad.shape == t.shape and not t.grad.any() for t in p.values())
+
+    T, D, K = 5, 96, 2
+    p, merge = make(T, D, BF16, "layer", "element", K=K, seed=2)
+    wide = {n: torch.zeros(t.shape[0], t.shape[1] + 7, dtype=t.dtype, device="cuda") for n, t in p.items() if n in ("y", "residual", "gate")}
+    for n in wide:
+        wide[n][:, 3:-4] = p[n]
+    views = {n: wide[n][:, 3:-4] if n in wide else t for n, t in p.items()}
+    views["weight"] = torch.stack((p["weight"], p["weight"]), dim=1)[:, 0]
+    got, grads = [], []
+    for q in (p, views):
+        leaves = {n: t.detach().requires_grad_(True) for n, t in q.items()}
+        o = call(leaves, merge, "layer", True)
+        torch.autograd.backward(o, [torch.full_like(t, 0.5) for t in o])
+        got.append(o)
+        grads.append([t.grad for t in leaves.values()])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and all(torch.equal(a, b) for a, b in zip(*grads))
+
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    grad, = torch.autograd.grad(moe.block_norm(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):       # (never a gradient of a gradient that leaves a part of it out)
+        grad.sum().backward()
