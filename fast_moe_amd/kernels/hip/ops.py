@@ -824,7 +824,7 @@ def gate_l1_bwd(scores: torch.Tensor, topk_idx: torch.Tensor, d_gates: torch.Ten
 
 
 # ----------------------------------------------------- a whole layer, few tokens
-FEW_TOKENS, FEW_EXPERTS, FEW_K = 64, 256, 16       # limits of fmoe_few_tokens
+FEW_TOKENS, FEW_EXPERTS, FEW_K, FEW_STRIDE = 64, 256, 16, 1 << 20      # limits of fmoe_few_tokens
 
 
 def _is_current(t: torch.Tensor) -> bool:
@@ -874,9 +874,9 @@ def few_tokens(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias: Optional[t
         if t is not None and t.dtype != want:
             raise ValueError(f"{name}: {what} must be {want}, got {t.dtype}")
     for what, t in (("weight", weight), ("weight_p", weight_p), ("weight_out", weight_out)):
-        if t is not None and t.shape[1] > 1 and (t.stride(1) != 1 or (t.shape[2] > 1 and t.stride(2) < t.shape[1]) or t.stride(0) < 0):
+        if t is not None and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[2] > 1 and not t.shape[1] <= t.stride(2) <= FEW_STRIDE)):
             raise ValueError(f"{name}: {what} must be a view of storage with the contraction contiguous, as the layers keep it "
-                             f"([E, D_out, D_in].permute(0, 2, 1)); got strides {t.stride()}")
+                             f"([E, D_out, D_in].permute(0, 2, 1)), rows at most 2^20 apart; got strides {t.stride()}")
     if weight_p is not None and weight_p.stride() != weight.stride():
         raise ValueError(f"{name}: weight and weight_p must have the same strides, got {weight.stride()} and {weight_p.stride()}")
     for what, t, n in (("gate_bias", gate_bias, (E,)), ("bias", bias, (E, H)), ("bias_p", bias_p, (E, H)), ("bias_out", bias_out, (E, O))):
@@ -896,7 +896,8 @@ def few_tokens(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias: Optional[t
     out = torch.empty((T, O), dtype=x.dtype, device=dev)
     if T == 0:
         return out
-    x, gate_weight = _plain_rows(x), _plain_rows(gate_weight)
+    x, gate_weight = (t if t.shape[0] == 1 or t.stride(0) <= FEW_STRIDE else t.contiguous() for t in (_plain_rows(x), _plain_rows(gate_weight)))
+    step = lambda t, dim, n: t.stride(dim) if t.shape[dim] > 1 else n       # (the stride of a single row says nothing)
     gate_bias = None if gate_bias is None else gate_bias.contiguous()
     token_mask = None if token_mask is None else token_mask.contiguous()
     bias, bias_p, bias_out = (None if t is None else _plain_rows(t) for t in (bias, bias_p, bias_out))
@@ -905,11 +906,11 @@ def few_tokens(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias: Optional[t
     d = FewDesc()
     d.T, d.E, d.k, d.D, d.H, d.O = T, E, k, D, H, O
     d.dtype, d.weight_dtype, d.renorm = _DTYPE_CODE[x.dtype], FMOE_E4M3 if fp8 else _DTYPE_CODE[x.dtype], int(bool(renorm))
-    d.x, d.x_stride_row = x.data_ptr(), max(x.stride(0), D)
-    d.gate_weight, d.gate_stride_row, d.gate_bias = gate_weight.data_ptr(), max(gate_weight.stride(0), D), _ptr(gate_bias)
+    d.x, d.x_stride_row = x.data_ptr(), step(x, 0, D)
+    d.gate_weight, d.gate_stride_row, d.gate_bias = gate_weight.data_ptr(), step(gate_weight, 0, D), _ptr(gate_bias)
     d.token_mask = _ptr(token_mask)
-    d.w, d.wp, d.w_stride_e, d.w_stride_n = weight.data_ptr(), _ptr(weight_p), weight.stride(0), max(weight.stride(2), D)
-    d.wo, d.wo_stride_e, d.wo_stride_n = weight_out.data_ptr(), weight_out.stride(0), max(weight_out.stride(2), H)
+    d.w, d.wp, d.w_stride_e, d.w_stride_n = weight.data_ptr(), _ptr(weight_p), weight.stride(0), step(weight, 2, D)
+    d.wo, d.wo_stride_e, d.wo_stride_n = weight_out.data_ptr(), weight_out.stride(0), step(weight_out, 2, H)
     d.w_scale, d.wp_scale, d.wo_scale = (_ptr(t) for t in scales)
     d.bias, d.bias_p = _ptr(bias), _ptr(bias_p)
     d.bias_stride_e = bias.stride(0) if bias is not None else bias_p.stride(0) if bias_p is not None else 0

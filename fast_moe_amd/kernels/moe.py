@@ -263,7 +263,7 @@ def fused_moe_few_tokens(
     token_mask: Optional[torch.Tensor] = None,
     kernel: KernelType = KernelType.HIP,
 ) -> torch.Tensor:
-    """A whole MoE layer for up to 64 tokens (a decode step) in two launches, [T, D] -> [T, O]: router
+    """A whole MoE layer for up to 64 tokens (a decode step) in two or three launches, [T, D] -> [T, O]: router
     ``softmax(x gate_weight^T + gate_bias)``, the ``k`` largest of every token (``renorm``: divided by their sum), and
     ``sum_j g_j * (act(x W[e_j] + bias[e_j]) W_out[e_j] + bias_out[e_j])`` with ``act(a) = silu(a)``, or
     ``silu(a) * (x W_p[e_j] + bias_p[e_j])`` when ``weight_p`` is given.

@@ -159,7 +159,7 @@ int fmoe_gate_route_pays(int dtype, int64_t T, int D, int E, int K);
 /* ------------------------------------------------- a whole layer, few tokens */
 
 /*
- * A whole mixture-of-experts layer for up to 64 tokens (a decode step) in two launches: router, the k experts of every token, and
+ * A whole mixture-of-experts layer for up to 64 tokens (a decode step) in two launches (three where the gate is large): router, the k experts of every token, and
  * their weighted sum; no counterpart in the reference, which runs the operators one by one (modules/fast_moe_module.py:188-225).
  *   l[t]    = x[t] . gate_weight^T + gate_bias                     fp32, not rounded
  *   experts = the k largest of l[t] in descending order (equal ones: the lower id first; NaN counts as the largest),
@@ -168,7 +168,7 @@ int fmoe_gate_route_pays(int dtype, int64_t T, int D, int E, int K);
  *   out[t]  = sum_j g[t, j] * (h . wo[e]^T + bias_out[e])          fp32 sums, rounded once
  * g * h is rounded to dtype in between (bf16: half a step of 2^-8).  A token whose token_mask byte is 0 reads no expert and gets a row of zeros.
  * dtype (tokens, gate, biases, output): FMOE_BF16 or FMOE_F32; weight_dtype: the same, or FMOE_E4M3 with bf16 tokens, which are not
- * quantised (products in bf16, divided by the multiplier scales).  k contiguous in every weight.  Rows of whole 16-byte chunks at 16-byte
+ * quantised (products in bf16, divided by the multiplier scales).  k contiguous in every weight, rows at most 2^20 elements apart.  Rows of whole 16-byte chunks at 16-byte
  * boundaries (8 bytes of e4m3) are read a chunk at a time, others element by element (an order of magnitude slower).  The same inputs give the same bits.
  */
 typedef struct fmoe_few_desc {

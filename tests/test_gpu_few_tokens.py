@@ -215,3 +215,19 @@ def test_refusals():
     (q, s), (qo, so) = moe_fp8.quantize_expert_weights(p["weight"]), moe_fp8.quantize_expert_weights(p["weight_out"])
     with pytest.raises(ValueError, match="scales of weight "):
         ops.few_tokens(p["x"], p["gate_weight"], None, q, None, None, None, qo, None, 2, scales=(s[:, :4], None, so))
+
+
+def test_single_rows_of_any_stride_and_rows_far_apart():
+    p = make(1, 4, 64, 1, 1, BF16, seed=2)
+    want = moe.fused_moe_few_tokens(k=2, **p)
+    far = torch.zeros(2, (1 << 20) + 64, dtype=BF16, device="cuda")
+    far[0, :64] = p["x"][0]
+    q = dict(p, x=far[:1, :64], weight=p["weight"].contiguous(), weight_p=p["weight_p"].contiguous(), weight_out=p["weight_out"].contiguous())
+    assert torch.equal(moe.fused_moe_few_tokens(k=2, **q), want)
+    far[1, :64] = 2 * p["x"][0]
+    two = moe.fused_moe_few_tokens(k=2, **dict(p, x=far[:, :64]))
+    assert torch.equal(two, moe.fused_moe_few_tokens(k=2, **dict(p, x=far[:, :64].contiguous())))
+    p = make(2, 2, 1, 8, 4, BF16, seed=3)
+    same = p["weight"][:, :, :1].expand(2, 1, 8)                # every hidden column the same storage
+    with pytest.raises(ValueError, match="contraction contiguous"):
+        moe.fused_moe_few_tokens(k=1, **dict(p, weight=same, weight_p=None))
