@@ -190,9 +190,8 @@ __device__ __forceinline__ Entry few_entry(const FewLists& l, int i) {
     const int x = UNIFORM ? uniform((int)v.x) : (int)v.x, y = UNIFORM ? uniform((int)v.y) : (int)v.y;
     return Entry{x & 0xffff, x >> 16, y};
 }
-// Sums that meet: two buffers of the 16 waves' two accumulators, or 8 shares of the router
-constexpr int kRedFloats = kWaves * 2 * kWave * 4, kRedBytes = 2 * kRedFloats * 4;
-static_assert(kRedBytes >= kWaves / 2 * 16 * kRouterRow * 4, "the router's sums lie in the same buffers");
+// Sums that meet in few_up: two buffers of the 16 waves' accumulators, or 8 shares of the router
+__host__ __device__ constexpr int few_red_bytes(int nt, int mats) { return 2 * kWaves * nt * mats * kWave * 16 > kWaves / 2 * 16 * kRouterRow * 4 ? 2 * kWaves * nt * mats * kWave * 16 : kWaves / 2 * 16 * kRouterRow * 4; }
 
 // Logits of tokens t0 .. t0 + 15 into LDS [16][E], 64 experts at a time: the waves' halves have 32 each and share the contraction in pieces of
 // 128 bytes per row (whole cache lines); their sums are added in wave order.
@@ -401,13 +400,13 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
     constexpr bool F32 = WT == kWF32, E4M3 = WT == kWE4M3 || WT == kWE4M3Half;
     constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, MATS = GATED ? 2 : 1;
     constexpr int AHEAD = !VEC || NT * XC * MATS > 2 ? 2 : 3;    // batches of loads in flight
-    constexpr int ROUND = NT == 1 ? MATS : 1;           // matrices whose sums are in LDS at a time
+    constexpr int RED = few_red_bytes(NT, MATS) / 8;     // floats of the waves' sums, of which there are two buffers
     extern __shared__ uint8_t lds[];
     const fmoe_few_desc& d = p.d;
     const int lane = lane_id(), wave = uniform(threadIdx.x / kWave), r16 = lane & 15, quarter = lane >> 4;
     float* const red = (float*)lds;
-    float* const logits = (float*)(lds + kRedBytes);
-    uint8_t* const listed = lds + kRedBytes + (p.stretches ? 0 : few_align(16 * d.E * 4));
+    float* const logits = (float*)(lds + few_red_bytes(NT, MATS));
+    uint8_t* const listed = lds + few_red_bytes(NT, MATS) + (p.stretches ? 0 : few_align(16 * d.E * 4));
     const FewLists l = few_lists(listed, d.T, d.E, d.k);
     for (int e = threadIdx.x; e < d.E; e += kWaves * kWave) l.mask[e] = 0;
     if (p.stretches) {          // few_logits has run
@@ -508,86 +507,40 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
     for (int i = 0; i < AHEAD; ++i) load(wv[i], xv[i]);
     clear();
     int turn = 0, n = NT > 1 && adding.entry < entries ? few_entry<true>(l, adding.entry).n : 0;
-    // One wave of a group adds up, another one each time; the others go on to the next item at once (the buffers take turns, so that it has read one
-    // before that is written again: in between is a barrier that it has to reach).
+    // An item's sums: a wave adds one of a lane's four columns (of one of the NT halves of the tokens) over the group's waves, others of the group each
+    // time; the rest goes on to the next item at once (the buffers take turns, so that it has read one before that is written again: in between is a
+    // barrier that it has to reach).  So few instructions on purpose: they come from memory the first time, 64 bytes after one another.
     auto finish = [&](int round) {
-        bool mine[NT], any = false;
-#pragma unroll
-        for (int f = 0; f < NT; ++f) {
-            mine[f] = ((round * NT + f) & (shares - 1)) == share && adding.entry < entries;
-            any |= mine[f];
-        }
-        const Entry at = any ? few_entry<true>(l, adding.entry) : Entry{0, 0, 0};
-        const int h0 = 16 * adding.tile, col0 = h0 + 4 * quarter;
-        // (asked for before the barrier)
-        float bias[MATS][4], div[MATS][4];
+        float* const buf = red + turn * RED;
+        turn ^= 1;
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const void* const b = m ? d.bias_p : d.bias;
-                const int col = min(col0 + i, d.H - 1);
-                bias[m][i] = any && b ? element<F32>(b, (int64_t)at.e * d.bias_stride_e + col) : 0.0f;
-                if constexpr (E4M3) div[m][i] = any ? (m ? d.wp_scale : d.w_scale)[(int64_t)at.e * d.H + col] : 1.0f;
-            }
-        f32x4 sum[MATS][NT];
+            for (int f = 0; f < NT; ++f) *reinterpret_cast<f32x4*>(buf + (((wave * MATS + m) * NT + f) * kWave + lane) * 4) = acc[m][f];
+        __syncthreads();
+        if (adding.entry < entries) {
+            const Entry at = few_entry<true>(l, adding.entry);
+#pragma unroll 1
+            for (int j = (share - 4 * NT * round) & (shares - 1); j < 4 * NT; j += shares) {
+                const int c = 16 * (j / 4) + r16, col = 16 * adding.tile + 4 * quarter + j % 4;
+                if (c >= at.n || col >= d.H) continue;
+                const float* from = buf + ((group * shares * MATS * NT + j / 4) * kWave + lane) * 4 + j % 4;
+                float v[MATS] = {};
+#pragma unroll 4
+                for (int w = 0; w < shares; ++w, from += MATS * NT * kWave * 4)
 #pragma unroll
-        for (int m0 = 0; m0 < MATS; m0 += ROUND) {
-            f32x4* const buf = reinterpret_cast<f32x4*>(red + turn * kRedFloats);
-            turn ^= 1;
+                    for (int m = 0; m < MATS; ++m) v[m] += from[m * NT * kWave * 4];
+                const int slot = l.slots[at.first + c];
 #pragma unroll
-            for (int m = 0; m < ROUND; ++m)
-#pragma unroll
-                for (int f = 0; f < NT; ++f) buf[((wave * ROUND + m) * NT + f) * kWave + lane] = acc[m0 + m][f];
-            __syncthreads();
-#pragma unroll
-            for (int f = 0; f < NT; ++f)
-                if (mine[f])
-#pragma unroll
-                    for (int m = 0; m < ROUND; ++m) {
-                        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                        const auto add = [&](int from, int waves) {
-#pragma unroll
-                            for (int w = 0; w < waves; ++w) {
-                                const f32x4 part = buf[(((group * shares + from + w) * ROUND + m) * NT + f) * kWave + lane];
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) v[i] += part[i];
-                            }
-                        };
-                        if (shares >= 4)
-                            for (int w = 0; w < shares; w += 4) add(w, 4);
-                        else
-                            for (int w = 0; w < shares; ++w) add(w, 1);
-                        sum[m0 + m][f] = v;
-                    }
-        }
-#pragma unroll
-        for (int f = 0; f < NT; ++f) {
-            if (!mine[f] || 16 * f + r16 >= at.n) continue;
-            const int slot = l.slots[at.first + 16 * f + r16];
-            const float g = l.gate[slot];
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float a = sum[0][f][i];
-                if constexpr (E4M3) a /= div[0][i];
-                v[i] = silu_f32(a + bias[0][i]);
-                if constexpr (GATED) {
-                    float u = sum[1][f][i];
-                    if constexpr (E4M3) u /= div[1][i];
-                    v[i] *= u + bias[1][i];
+                for (int m = 0; m < MATS; ++m) {
+                    const void* const b = m ? d.bias_p : d.bias;
+                    if constexpr (E4M3) v[m] /= (m ? d.wp_scale : d.w_scale)[(int64_t)at.e * d.H + col];
+                    if (b) v[m] += element<F32>(b, (int64_t)at.e * d.bias_stride_e + col);
                 }
-                v[i] *= g;
-            }
-            // bf16: the one rounding between the two products, of the gated value (half a step of bf16, as of the layer's own hidden rows)
-            const int64_t to = (int64_t)slot * d.H + col0;
-            if (VEC && col0 + 4 <= d.H) {
-                if constexpr (F32) *reinterpret_cast<f32x4*>((float*)p.h + to) = f32x4{v[0], v[1], v[2], v[3]};
-                else *reinterpret_cast<u32x2*>((uint16_t*)p.h + to) = u32x2{cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (col0 + i < d.H) put_element<F32>(p.h, to + i, v[i]);
+                float h = silu_f32(v[0]);
+                if constexpr (GATED) h *= v[1];
+                // bf16: the one rounding between the two products, of the gated value (half a step of bf16, as of the layer's own hidden rows)
+                put_element<F32>(p.h, (int64_t)slot * d.H + col, h * l.gate[slot]);
             }
         }
         clear();
@@ -861,11 +814,11 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     // waves to an item: so that each has four steps, and no CU is without an item for want of blocks
     int share_bits = 0;
     while (share_bits < 4 && ((4 << share_bits) * step < d.D || (items << share_bits) < 256 * kWaves)) ++share_bits;
-    auto up = [&](auto kern, bool& reserved) {
-        const int bytes = kRedBytes + (p.stretches ? 0 : few_align(16 * d.E * 4)) + lists;
+    auto up = [&](auto kern, bool& reserved, int red) {
+        const int bytes = red + (p.stretches ? 0 : few_align(16 * d.E * 4)) + lists;
         if (!reserved) {        // (more than 64 KB; the most that any call of this kernel asks for)
             const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                       kRedBytes + few_align(16 * kFewMostExperts * 4) + few_lists_bytes(kFewMostTokens, kFewMostExperts, kFewMostK));
+                                                       red + few_align(16 * kFewMostExperts * 4) + few_lists_bytes(kFewMostTokens, kFewMostExperts, kFewMostK));
             if (err != hipSuccess) return fail(FMOE_ERR_LAUNCH, "fmoe_few_tokens: cannot reserve %d B of LDS: %s", bytes, hipGetErrorString(err));
             reserved = true;
         }
@@ -880,7 +833,7 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
 #define FMOE_FEW_UP(WT, VEC, NT, GATED)                                     \
     ([&] {                                                                  \
         static bool reserved = false;                                       \
-        return up(few_up_kernel<WT, VEC, NT, GATED>, reserved);             \
+        return up(few_up_kernel<WT, VEC, NT, GATED>, reserved, few_red_bytes(NT, GATED ? 2 : 1)); \
     })()
 #define FMOE_FEW(WT, VEC)                                                   \
     do {                                                                    \
