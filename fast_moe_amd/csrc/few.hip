@@ -573,7 +573,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 // contraction side by side, of whose products the diagonal blocks count: more, smaller tiles where 16 columns each would leave CUs without one.
 // gridDim.y > 1: so many blocks share a tile's contraction; their sums go through memory, and the one that arrives last adds them in block order.
 template <int WT, bool VEC, int NT, int PARTS>
-__global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
+__global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p, bool spread) {
     constexpr bool F32 = WT == kWF32, E4M3 = WT == kWE4M3 || WT == kWE4M3Half, ONE = PARTS == 1;
     constexpr int CE = Wt<WT>::CE, ES = Wt<WT>::ES, XES = Wt<WT>::XES, XC = Wt<WT>::XC, STEP = 4 * CE, COLS = 16 / PARTS;
     constexpr int AHEAD = !VEC ? 1 : NT * XC == 1 ? 4 : NT * XC == 2 ? 3 : 2;      // pieces whose loads are in flight
@@ -589,9 +589,11 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
     __syncthreads();
     const int part = ONE ? 0 : r16 / COLS, n0 = blockIdx.x * COLS, row = min(n0 + r16 % COLS, d.O - 1);
     const int steps = (d.H + STEP - 1) / STEP, pieces = (steps + 1) / 2, total = uniform(*l.entries) * pieces;
-    // every stretch (a wave's, or a part of its) takes as many pieces of two steps, experts after one another
-    const int stretches = waves * PARTS * gridDim.y, per = (total + stretches - 1) / stretches;
-    const int from = ((blockIdx.y * waves + wave) * PARTS + part) * per, until = min(total, from + per);
+    // Every stretch (a wave's, or a part of its) takes as many pieces of two steps, experts after one another: all of its in a row, or (spread) every
+    // stretches-th, so that all of them work on the same rows at a time and an expert with more tokens costs each as much.
+    const int stretches = waves * PARTS * gridDim.y, per = (total + stretches - 1) / stretches, unit = spread ? 1 : per;
+    const int from = ((blockIdx.y * waves + wave) * PARTS + part) * unit, until = spread ? total : min(total, from + per);
+    const int skip = spread ? stretches - 1 : 0, over = skip / pieces, rest = skip - over * pieces;
     Entry next = {0, 0, 0}, cur = {0, 0, 0};            // whose loads are on their way, and whose products add up
     int next_index = -1, cur_index = -1, of[AHEAD];
     const uint8_t *wrow = nullptr, *xrow[NT] = {};
@@ -635,9 +637,11 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p) {
                     if constexpr (ONE) xb[s][f][c] = x.chunk(xoff[f], at, any && xoff[f] != ~0u ? d.H : 0);
                     else xb[s][f][c] = chunk<XES, VEC>(xrow[f], at, any && xrow[f] ? d.H : 0);
                 }
-        ++q;
-        if (++piece == pieces) {
-            piece = 0;
+        q += 1 + skip;
+        index += over;
+        piece += 1 + rest;
+        if (piece >= pieces) {
+            piece -= pieces;
             ++index;
         }
     };
@@ -828,7 +832,11 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     };
     auto down = [&](auto kern) {
         const int waves = d.T > 32 ? kWaves / 2 : kWaves;        // (their sums for 64 tokens in 32 KB of LDS)
-        kern<<<dim3(plan.tiles, plan.blocks), waves * kWave, waves * d.T * 64 + lists, stream>>>(p);
+        // Spread where an expert has two pieces for every stretch: 37 tokens, 12 experts, 2600 x 1000 fp32 48.9 us in a row, 44.6 spread, 1 token, 14336 x
+        // 4096 bf16 47.0 and 44.1.  With fewer, a stretch changes experts at nearly every piece: 16 tokens, 128 experts, 1536 x 4096 bf16 150 and 155 us,
+        // 1 token, 1408 x 2048 13.2 and 14.3, 4 tokens, 1536 x 4096 e4m3 43 and 48.
+        const int down_step = half && !vec ? 32 : step, pieces = ((d.H + down_step - 1) / down_step + 1) / 2;
+        kern<<<dim3(plan.tiles, plan.blocks), waves * kWave, waves * d.T * 64 + lists, stream>>>(p, pieces >= 2 * waves * plan.parts * plan.blocks);
     };
 #define FMOE_FEW_UP(WT, VEC, NT, GATED)                                     \
     ([&] {                                                                  \
