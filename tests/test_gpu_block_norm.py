@@ -417,3 +417,20 @@ def test_no_rows_strided_operands_and_no_second_derivative():
     grad, = torch.autograd.grad(moe.block_norm(x, w).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):       # (never a gradient of a gradient that leaves a part of it out)
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("T,D,K", [(5, 1001, 3), (9, 2048, 8), (3, 4100, 2)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("norm,sigmoid", [("rms", True), ("layer", False)])
+def test_merged_rows_with_a_gate_for_each_element(T, D, K, dtype, norm, sigmoid):
+    p, merge = make(T, D, dtype, norm, "element", K=K, param_dtype=F32, seed=T + D)
+    for t in p.values():
+        t.requires_grad_(True)
+    out, nxt = call(p, merge, norm, sigmoid)
+    d_out, d_next = (torch.randn(T, D, device="cuda").to(dtype) for _ in range(2))
+    torch.autograd.backward((out, nxt), (d_out, d_next))
+    want = formula(p, merge, norm, sigmoid, d_out, d_next)
+    close("out", out, want["out"])
+    close("next", nxt, want["next"])
+    for n, t in p.items():      # (the merged rows and their gradients rounded to the rows' dtype)
+        close("d_" + n, t.grad, want["d_" + n], rounded=4 * HALF_STEP[dtype])
