@@ -77,7 +77,7 @@ struct CkptRows {
     uint8_t* e;                 // [rows][2][padded / 32]
 };
 
-// 16 values a lane, two lanes a block; the lanes of a grid go over (row, matrix, half block) in memory order.
+// 16 values a lane, two lanes a block; the lanes of a grid go over (row, matrix, half block) in memory order.  131072 x 1408 bf16: 233 us, 4.8 TB/s.
 template <typename E, bool WHOLE>
 __global__ __launch_bounds__(256) void swiglu_checkpoint_kernel(CkptRows p) {
     const int halves = p.padded / 16, per_row = 2 * halves;
@@ -118,6 +118,7 @@ __device__ __forceinline__ void decode(u32x2 q, float scale, float (&f)[8]) {
     for (int i = 0; i < 8; ++i) f[i] = (float)(int)(int8_t)(q[i / 4] >> (8 * (i & 3))) * scale;
 }
 
+// The same, 8 values a lane.  131072 x 1408 bf16: 200 us, 5.6 TB/s.
 template <typename E, bool WHOLE>
 __global__ __launch_bounds__(256) void swiglu_checkpoint_read_kernel(CkptRows p) {
     const int eighths = p.padded / 8, per_row = 2 * eighths;
@@ -146,7 +147,8 @@ struct CkptBwd {
     float* dots;
 };
 
-// Eight values a lane; LANES of a wave to a row (all of them, or as many as a shorter row has eighths, rounded up to a power of two).
+// Eight values a lane; LANES of a wave to a row (all of them, or as many as a shorter row has eighths, rounded up to 2, 8 or 32): 200000 x 40 bf16 17 us against
+// 85 with a wave to every row, 100000 x 200 36 against 47.  9189 x 2600 bf16: 44 us, 5.5 TB/s.
 template <typename E, bool WHOLE, int LANES>
 __global__ __launch_bounds__(256) void swiglu_checkpoint_bwd_kernel(CkptBwd p) {
     constexpr int ROWS = kWave / LANES;

@@ -1,4 +1,4 @@
-// fmoe_few_tokens: a whole mixture-of-experts layer for a few tokens (a decode step) in two launches.
+// fmoe_few_tokens: a whole mixture-of-experts layer for a few tokens (a decode step) in two launches, three where the gate is large.
 //
 //   l[t, :] = x[t] . G[e] + bg[e];   the k largest l of a token are its experts, g = softmax of l over them (or over all)
 //   h[t, j] = g[t, j] * silu(x[t] . W[e] + b[e]) (* (x[t] . Wp[e] + bp[e]))             e = the token's j-th expert
@@ -7,11 +7,15 @@
 // What bounds it are the bytes of the experts hit, each to be read once: 2 * T flops a byte leave the matrix cores idle.  So the
 // weights go from memory to the MFMAs' registers with nothing in between (no LDS, no other wave reads them), and everything else
 // is kept out of their way:
-//   few_up    every block computes the whole router for itself (the same sums in the same order, so the same selection everywhere:
-//             a launch of its own would cost more than the gate's few hundred KB from the L2), then takes (expert, 16 hidden columns)
-//             items; its waves share the contraction and meet in LDS.  An expert's tokens are gathered into the MFMAs' columns.
-//   few_down  a block owns 16 output columns for all tokens; its waves share the experts and their contraction.  The gate is folded into h, so
-//             the experts' products add up in one accumulator, no partial sum leaves the block and no atomics are needed.
+//   few_logits  the router's products, where the gate is more than what every CU reads for itself in the time of a launch
+//   few_up      every block selects for itself (the same logits, so the same experts everywhere), then takes (expert, 16 hidden columns)
+//               items; its waves share the contraction and meet in LDS.  An expert's tokens are gathered into the MFMAs' columns.
+//   few_down    a block owns 16 output columns for all tokens; its waves share the experts and their contraction.  The gate is folded into h, so
+//               the experts' products add up in one sum.  Where there are few output columns several blocks share them, and the last one
+//               to arrive adds their sums in block order: the same bits every time.
+// Measured, whole passes: 16 tokens (12 of them live), 128 experts of 4096 x 1536 bf16, 2.6 GB 438 us, 5.95 TB/s; 4 tokens, the same in e4m3, 0.55 GB 121 us,
+// 4.5 TB/s; 1 token, 64 experts of 2048 x 1408 bf16, 0.14 GB 40 us, 3.5 TB/s; 37 tokens, 12 experts of 1000 x 2600 fp32, 0.25 GB 90 us, 2.8 TB/s;
+// 1 token, 128 x 256, 14 us.  (A 1 GiB copy: 5.2 TB/s.)  Some 12 us of each are the launches, the selection, a first load's way to memory, twice, and the last sums.
 // Weights are the MFMAs' A operand (rows = output columns), tokens its B operand (16 columns).
 #include "common.h"
 
@@ -733,13 +737,17 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p, bo
 // The workspace: the lists as few_up's first block leaves them, and the hidden rows.
 size_t few_hidden_at(const fmoe_few_desc& d) { return ((size_t)few_lists_bytes(d.T, d.E, d.k) + 255) & ~(size_t)255; }
 size_t few_logits_at(const fmoe_few_desc& d) { return (few_hidden_at(d) + (size_t)d.T * d.k * d.H * (d.dtype == FMOE_F32 ? 4 : 2) + 255) & ~(size_t)255; }
-// Stretches of the router's own launch, 0 where few_up computes the router.
+// Stretches of the router's own launch, 0 where few_up computes the router: 256 CUs reading 256 KB of gate each take 9 us, a launch and its reading back 5.
+// Up to 16 tokens are one block per 16 experts and stretch (4 of them: 4.5 us for 128 experts of 4096); more have blocks of their own, and every stretch is
+// read back for every token: 32 tokens, 128 experts of 4096 11.2 us as one stretch, 7.0 as two, 5.3 as four, which cost the selection 3.
 int few_stretches(const fmoe_few_desc& d) {
     if ((int64_t)d.E * d.D * (d.dtype == FMOE_F32 ? 4 : 2) * ((d.T + 15) / 16) <= 32 * 1024) return 0;
-    return d.T <= 16 ? 4 : 1;
+    return d.T <= 16 ? 4 : 2;
 }
 size_t few_arrivals_at(const fmoe_few_desc& d) { return (few_logits_at(d) + (size_t)few_stretches(d) * d.T * d.E * 4 + 255) & ~(size_t)255; }
-// few_down's tiles: parts of an MFMA's rows (up to 16 / parts tokens) so that there are 256 of them, else blocks to a tile.
+// few_down's tiles: parts of an MFMA's rows (up to 16 / parts tokens) so that there are 256 of them, else blocks to a tile.  Parts against tiles of 16:
+// 1 token, 1408 x 2048 12.8 us and 18.7, 1408 x 512 7.9 and 13.5, 5 tokens, 256 x 128 5.4 and 8.5.  Blocks against one to a tile: 64 tokens, 64 experts of
+// 1408 x 1024 bf16 54 us and 147, 37 tokens, 2600 x 1000 fp32 45 and 110.
 struct DownPlan {
     int parts, tiles, blocks;
 };
@@ -815,7 +823,8 @@ extern "C" int fmoe_few_tokens(const fmoe_few_desc* desc, void* workspace, size_
     hipStream_t stream = (hipStream_t)stream_;
     const int lists = few_lists_bytes(d.T, d.E, d.k), step = wes == 1 ? 64 : 64 / wes;
     const int64_t items = (int64_t)most_active * ((d.H + 15) / 16) * (d.T > 32 ? 2 : 1);
-    // waves to an item: so that each has four steps, and no CU is without an item for want of blocks
+    // waves to an item: so that each has four steps, and no CU is without an item for want of blocks.  (16 to every item: 16 tokens, 128 experts of 512 x 1536
+    // bf16 76 us in place of 58, a wave's two steps at a time being more than its share.)
     int share_bits = 0;
     while (share_bits < 4 && ((4 << share_bits) * step < d.D || (items << share_bits) < 256 * kWaves)) ++share_bits;
     auto up = [&](auto kern, bool& reserved, int red) {

