@@ -997,8 +997,8 @@ PyObject* py_norm_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
                 stats = empty({c.d.rows, 4}, at::kFloat, r);
                 c.d.stats = stats.data_ptr<float>();
                 if (c.d.K) {
-                    merged = empty(r.sizes(), r.scalar_type(), r);
-                    c.d.y_out = merged.data_ptr();
+                    merged = empty(r.sizes(), at::kFloat, r);
+                    c.d.y_out = merged.data_ptr<float>();
                 }
             }
             return c_norm_add(&c.d, (void*)stream);
@@ -1008,20 +1008,41 @@ PyObject* py_norm_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// (Norm's, stats, d_out, d_next, need (bits in the order of Norm's tensors), stream) -> the gradients of Norm's tensors
+// (Norm's, stats, d_out, d_next, need (bits in the order of Norm's tensors, the merge weights behind them), stream, and of a merge, else None: the merged rows,
+// token_index, merge, merge_index) -> the gradients of Norm's tensors and of merge
 PyObject* py_norm_add_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != Norm::ARGS + 5) return none();
+    if (n != Norm::ARGS + 9) return none();
     Norm c;
-    at::Tensor stats, d_out, d_next, grad[Norm::TENSORS], workspace;
+    at::Tensor stats, d_out, d_next, grad[Norm::TENSORS + 1], workspace, merged, token_index, merge, merge_index;
     int64_t need, stream;
+    at::Tensor* const of_merge[] = {&merged, &token_index, &merge, &merge_index};
+    for (int i = 0; i < 4; ++i)
+        if (!optional_tensor(args[Norm::ARGS + 5 + i], of_merge[i])) return none();
     if (!c.parse(args) || !optional_tensor(args[Norm::ARGS], &stats) || !optional_tensor(args[Norm::ARGS + 1], &d_out) ||
         !optional_tensor(args[Norm::ARGS + 2], &d_next) || !as_int(args[Norm::ARGS + 3], &need) || !as_int(args[Norm::ARGS + 4], &stream))
         return none();
     const at::Tensor& r = c.t[Norm::RESIDUAL];
     const int status = run(
         [&] {
-            if (!c.ok(0) || !stats.defined() || !d_next.defined()) return false;
+            int64_t K = 0;
+            if (merged.defined()) {
+                if (!float_matrix(r) || r.size(0) < 1 || !token_index.defined() || token_index.numel() < r.size(0) || token_index.numel() % r.size(0)) return false;
+                K = token_index.numel() / r.size(0);
+                const int64_t R = r.size(0) * K;
+                if (K > 64 || merged.scalar_type() != at::kFloat || merged.sizes() != r.sizes() || !merged.is_contiguous() || !i64_list(token_index, R) ||
+                    !same_device(r, merged) || !same_device(r, token_index) || !same_device(r, merge) || !same_device(r, merge_index))
+                    return false;
+                if (merge.defined() && (!merge.is_contiguous() || merge.numel() != R || (merge.scalar_type() != at::kFloat && merge.scalar_type() != at::kBFloat16) ||
+                                        (merge_index.defined() && !i64_list(merge_index, R))))
+                    return false;
+                if ((need >> Norm::TENSORS & 1) && !merge.defined()) return false;
+            } else if (need >> Norm::TENSORS & 1) {
+                return false;
+            }
+            if (!c.ok(K) || !stats.defined() || !d_next.defined()) return false;
+            c.d.K = (int32_t)K;
+            c.d.value_rows = c.d.rows * K;
             for (const at::Tensor* v : {&d_out, &d_next})
                 if (v->defined() && (v->scalar_type() != r.scalar_type() || v->sizes() != r.sizes() || !v->is_contiguous() || !same_device(r, *v))) return false;
             if (stats.scalar_type() != at::kFloat || !stats.is_contiguous() || stats.numel() != 4 * c.d.rows || !same_device(r, stats)) return false;
@@ -1033,9 +1054,22 @@ PyObject* py_norm_add_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
             void** const to[Norm::TENSORS] = {&c.d.d_y, &c.d.d_residual, &c.d.d_weight, &c.d.d_bias, &c.d.d_gate, &c.d.d_scale, &c.d.d_next_weight, &c.d.d_next_bias};
             for (int i = 0; i < Norm::TENSORS; ++i)
                 if (need >> i & 1) {
-                    grad[i] = empty(i == Norm::Y ? r.sizes() : c.t[i].sizes(), c.t[i].scalar_type(), r);
+                    grad[i] = i == Norm::Y && c.d.K ? empty_rows(c.d.value_rows, r.size(1), r.scalar_type(), r) : empty(c.t[i].sizes(), c.t[i].scalar_type(), r);
                     *to[i] = grad[i].data_ptr();
                 }
+            if (c.d.K) {
+                c.d.y_out = merged.data_ptr<float>();
+                c.d.token_index = token_index.data_ptr<int64_t>();
+                if (merge.defined()) {
+                    c.d.merge = merge.data_ptr();
+                    c.d.merge_dtype = dtype_code(merge.scalar_type());
+                    c.d.merge_index = merge_index.defined() ? merge_index.data_ptr<int64_t>() : nullptr;
+                }
+                if (need >> Norm::TENSORS & 1) {
+                    grad[Norm::TENSORS] = at::zeros({c.d.value_rows}, at::TensorOptions(r.device()).dtype(at::kFloat));
+                    c.d.d_merge = grad[Norm::TENSORS].data_ptr<float>();
+                }
+            }
             c.d.stats = stats.data_ptr<float>();
             c.d.d_out = d_out.defined() ? d_out.data_ptr() : nullptr;
             c.d.d_next = d_next.data_ptr();
@@ -1045,9 +1079,9 @@ PyObject* py_norm_add_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
         });
     if (raised(status, "fmoe_norm_add_bwd")) return nullptr;
     if (status != FMOE_OK) return none();
-    PyObject* out = PyTuple_New(Norm::TENSORS);
+    PyObject* out = PyTuple_New(Norm::TENSORS + 1);
     if (!out) return nullptr;
-    for (int i = 0; i < Norm::TENSORS; ++i) PyTuple_SET_ITEM(out, i, wrap_or_none(grad[i]));
+    for (int i = 0; i <= Norm::TENSORS; ++i) PyTuple_SET_ITEM(out, i, wrap_or_none(grad[i]));
     return out;
     END_HANDLE_TH_ERRORS
 }

@@ -127,10 +127,46 @@ struct Row {
             }
         }
     }
+    // rows of fp32 at the same columns, whatever E is
+    struct Raw32 {
+        u32x4 v[N / 4];
+    };
+    __device__ __forceinline__ void fetch_f32(const float* p, Raw32& r) const {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int q = 0; q < V / 4; ++q) {
+                u32x4& v = r.v[c * (V / 4) + q];
+                v = u32x4{0, 0, 0, 0};
+                if (whole(c)) {
+                    v = load16(p + col(c * V) + 4 * q);
+                } else if (!WHOLE) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = in(c * V + 4 * q + i) ? __float_as_uint(p[col(c * V + 4 * q + i)]) : 0u;
+                }
+            }
+    }
+    __device__ __forceinline__ void take_f32(const Raw32& r, float (&f)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = __uint_as_float(r.v[i / 4][i % 4]);
+    }
     __device__ __forceinline__ void store_f32(float* p, const float (&f)[N]) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (in(i)) p[col(i)] = f[i];
+        for (int c = 0; c < CH; ++c) {
+            if (whole(c)) {
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) {
+                    u32x4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(f[c * V + 4 * q + i]);
+                    store16(p + col(c * V) + 4 * q, v);
+                }
+            } else if (!WHOLE) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (in(c * V + i)) p[col(c * V + i)] = f[c * V + i];
+            }
+        }
     }
 };
 
@@ -298,8 +334,8 @@ struct MergeParams {
     float eps, scale_value;
     const void *y, *residual, *gate, *merge, *scale, *weight, *bias, *next_weight, *next_bias;
     const int64_t *reverse_index, *merge_index;
-    void *out, *next, *y_out;
-    float* stats;
+    void *out, *next;
+    float *y_out, *stats;
 };
 template <typename E, bool WHOLE, int CH, bool LAYER, bool P32, int BATCH, bool ELEMENT>
 __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(MergeParams p, int waves) {
@@ -366,7 +402,7 @@ __global__ __launch_bounds__(kNormMostWaves* kWave) void norm_merge_kernel(Merge
         float token = p.gate_mode && !ELEMENT ? to_f32(token_gate) : 1.0f;
         if (p.gate_sigmoid && !ELEMENT) token = sigmoid_f32(token);
         fetch(t + step);
-        if (p.y_out) row.store((E*)p.y_out + t * p.cols, y);
+        if (p.y_out) row.store_f32(p.y_out + t * p.cols, y);
         if (p.weight) row_stats(row, y, LAYER, p.eps, x, mean, rstd);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -411,7 +447,8 @@ enum { kDScale = 0, kDWeight, kDNextWeight, kDBias, kDNextBias, kSums };
 
 // The next row's loads are issued before this row's sums are exchanged.  16384 x 2048 bf16 90 us, 4.5 TB/s, and 5 us for the sums; 3063 x 1001 fp32 layer norms
 // with a gate for each element 26 us, 3.8 TB/s, and 6.
-template <typename E, bool WHOLE, int CH, bool LAYER, bool ELEMENT, int THREADS>
+// MERGED: y is the merged rows in fp32, and so is d_y (a sum of expert rows against its gradient takes what two roundings would leave out).
+template <typename E, bool WHOLE, int CH, bool LAYER, bool ELEMENT, bool MERGED, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d, int waves, float* partial) {
     using R = Row<E, WHOLE, CH>;
     using P = Param<R, CH == 1>;
@@ -433,13 +470,15 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
     const int first = blockIdx.x * per + (waves == 1 ? wave : 0);
     const int64_t step = (int64_t)gridDim.x * per;
     typename R::Raw ry, ro, rn, rt, rg;
+    typename R::Raw32 rm;
     f32x4 st;
     E token_gate = E(0);
     auto fetch = [&](int64_t t) {
         if (t >= d.rows) return;
         st = *reinterpret_cast<const f32x4*>(d.stats + 4 * t);
         row.fetch((const E*)d.residual + t * d.residual_stride, ro);
-        if (d.y) row.fetch((const E*)d.y + t * d.y_stride, ry);
+        if constexpr (MERGED) row.fetch_f32((const float*)d.y + t * d.cols, rm);
+        else if (d.y) row.fetch((const E*)d.y + t * d.y_stride, ry);
         if (d.d_next) row.fetch((const E*)d.d_next + t * d.cols, rn);
         if (d.d_out) row.fetch((const E*)d.d_out + t * d.cols, rt);
         if constexpr (ELEMENT) row.fetch((const E*)d.gate + t * d.gate_stride, rg);
@@ -450,7 +489,8 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
         const float m = st[0], r = st[1], m2 = st[2], r2 = st[3];
         float a[N], o[N], dn[N], dt[N], gates[ELEMENT ? N : 1];
         row.take(ro, o);
-        if (d.y) row.take(ry, a);
+        if constexpr (MERGED) row.take_f32(rm, a);
+        else if (d.y) row.take(ry, a);
         if (d.d_next) row.take(rn, dn);
         if (d.d_out) row.take(rt, dt);
         else
@@ -539,7 +579,8 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
 #pragma unroll
                 for (int i = 0; i < N; ++i)
                     if (d.weight) dt[i] = r * (dt[i] - a[i] * (q[0] * inv) - mean_of(q[1]));
-                row.store((E*)d.d_y + t * d.cols, dt);
+                if constexpr (MERGED) row.store_f32((float*)d.d_y + t * d.cols, dt);
+                else row.store((E*)d.d_y + t * d.cols, dt);
             }
         }
     }
@@ -549,6 +590,52 @@ __global__ __launch_bounds__(THREADS) void norm_add_bwd_kernel(fmoe_norm_desc d,
 #pragma unroll
         for (int s = 0; s < SUMS; ++s)
             if (want[s]) row.store_f32(at + (int64_t)s * d.cols, sums[s]);
+    }
+}
+
+// What d_y [rows, cols] of the merged rows (fp32) gives the routed rows, a wave to each: d_value[r] = w_r * d_y[token], and <value[r], d_y[token]> for its weight.
+struct MergeBwdParams {
+    const float* d_y;
+    const void* value;
+    int64_t rows, value_rows, value_stride;
+    const int64_t *token_index, *merge_index;
+    const void* merge;
+    int32_t cols, merge_f32;
+    void* d_value;
+    float* d_merge;
+};
+template <typename E, bool WHOLE>
+__global__ __launch_bounds__(256) void norm_merge_bwd_kernel(MergeBwdParams p) {
+    using R = Row<E, WHOLE, 1>;
+    constexpr int N = R::N, STEP = kWave * N;
+    const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (r >= p.value_rows) return;
+    const int64_t t = p.token_index[r], flat = p.merge_index ? p.merge_index[r] : r;
+    const bool named = (uint64_t)t < (uint64_t)p.rows, weighted = (uint64_t)flat < (uint64_t)p.value_rows;
+    float w = 1.0f, dot = 0.0f;
+    if (p.merge) w = !weighted ? 0.0f : p.merge_f32 ? reinterpret_cast<const float*>(p.merge)[flat] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p.merge)[flat]);
+    for (int c = 0; c < p.cols; c += STEP) {
+        const R row{lane_id(), kWave, p.cols - c};
+        typename R::Raw32 raw;
+        typename R::Raw rv;
+        float d[N], v[N];
+        if (p.d_merge) row.fetch((const E*)p.value + r * p.value_stride + c, rv);
+        row.fetch_f32(p.d_y + (named ? t : 0) * p.cols + c, raw);
+        row.take_f32(raw, d);
+        if (p.d_merge) {
+            row.take(rv, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) dot = __builtin_fmaf(v[i], d[i], dot);
+        }
+        if (p.d_value) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] = named ? w * d[i] : 0.0f;
+            row.store((E*)p.d_value + r * p.cols + c, d);
+        }
+    }
+    if (p.d_merge) {
+        dot = wave_sum(dot);
+        if (lane_id() == 0 && weighted) p.d_merge[flat] = named ? dot : 0.0f;
     }
 }
 
@@ -633,7 +720,7 @@ int norm_check(const fmoe_norm_desc* d, bool backward) {
     if (d->rows == 0) return FMOE_OK;
     FMOE_REQUIRE(d->residual && d->residual_stride >= 0, "%s: residual is missing", name);
     FMOE_REQUIRE(!d->gate_mode || (d->gate && d->y), "%s: a gate needs its tensor and y", name);
-    FMOE_REQUIRE(d->K >= 0 && d->K <= 64 && (!d->K || (d->y && d->reverse_index && d->value_rows == d->rows * d->K)),
+    FMOE_REQUIRE(d->K >= 0 && d->K <= 64 && (!d->K || (d->y && (backward || d->reverse_index) && d->value_rows == d->rows * d->K)),
                  "%s: a merge needs y [rows * K, cols] and reverse_index, K <= 64", name);
     FMOE_REQUIRE(!d->merge || d->merge_dtype == FMOE_F32 || d->merge_dtype == FMOE_BF16, "%s: merge weights must be bf16 or fp32", name);
     FMOE_REQUIRE(!d->stats || aligned16(d->stats), "%s: stats must be 16-byte aligned", name);
@@ -641,7 +728,8 @@ int norm_check(const fmoe_norm_desc* d, bool backward) {
         FMOE_REQUIRE(d->next ? d->next_weight != nullptr : d->out != nullptr, "%s: nothing to write", name);
         FMOE_REQUIRE(d->y || !d->out, "%s: out without y is the residual", name);
     } else {
-        FMOE_REQUIRE(!d->K, "%s: takes the merged y", name);
+        FMOE_REQUIRE(!d->K || (d->y_out && d->token_index), "%s: a merge needs the merged rows of the forward pass and token_index", name);
+        FMOE_REQUIRE((d->K && d->merge) || !d->d_merge, "%s: the gradient of an operand that is not there", name);
         FMOE_REQUIRE(d->stats && (d->d_next || d->d_out), "%s: needs the forward pass's stats and a gradient", name);
         FMOE_REQUIRE(!d->d_next || d->next_weight, "%s: d_next needs next_weight", name);
         FMOE_REQUIRE((d->y || !(d->d_y || d->d_gate || d->d_scale || d->d_weight || d->d_bias)) && (d->gate_mode || !d->d_gate) && (d->scale || !d->d_scale) &&
@@ -710,43 +798,66 @@ extern "C" int fmoe_norm_add(const fmoe_norm_desc* desc, fmoe_stream_t stream) {
     return check_launch("fmoe_norm_add");
 }
 
+// The workspace of the backward pass: the sums' partial ones, and d_y of the merged rows.
+static size_t norm_partial_bytes(const fmoe_norm_desc& d) {
+    if (!norm_wants_sums(d)) return 0;
+    const NormPlan p = norm_plan(d, true);
+    const int64_t groups = norm_groups(d, p), all = (groups + p.per - 1) / p.per * p.per;
+    return ((size_t)all * kSums * d.cols * sizeof(float) + 255) & ~(size_t)255;
+}
+
 extern "C" size_t fmoe_norm_add_bwd_workspace_bytes(const fmoe_norm_desc* desc) {
-    if (norm_check(desc, true) != FMOE_OK || desc->rows == 0 || !norm_wants_sums(*desc)) return 0;
-    const NormPlan p = norm_plan(*desc, true);
-    const int64_t groups = norm_groups(*desc, p), all = (groups + p.per - 1) / p.per * p.per;
-    return (size_t)all * kSums * desc->cols * sizeof(float);
+    if (norm_check(desc, true) != FMOE_OK || desc->rows == 0) return 0;
+    return norm_partial_bytes(*desc) + (desc->K && (desc->d_y || desc->d_merge) ? (size_t)desc->rows * desc->cols * sizeof(float) : 0);
 }
 
 extern "C" int fmoe_norm_add_bwd(const fmoe_norm_desc* desc, void* workspace, size_t workspace_bytes, fmoe_stream_t stream) {
     const int rc = norm_check(desc, true);
     if (rc != FMOE_OK || desc->rows == 0) return rc;
-    const fmoe_norm_desc& d = *desc;
-    const NormPlan p = norm_plan(d, true);
-    const size_t need = fmoe_norm_add_bwd_workspace_bytes(desc);
+    const size_t need = fmoe_norm_add_bwd_workspace_bytes(desc), sums = norm_partial_bytes(*desc);
     if (need && (!workspace || workspace_bytes < need))
         return fail(FMOE_ERR_WORKSPACE, "fmoe_norm_add_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    float* const partial = need ? (float*)workspace : nullptr;
+    FMOE_REQUIRE(!need || aligned16(workspace), "fmoe_norm_add_bwd: the workspace must be 16-byte aligned");
+    fmoe_norm_desc d = *desc;
+    const NormPlan p = norm_plan(d, true);
+    float* const partial = sums ? (float*)workspace : nullptr;
+    if (d.K) {
+        d.y = d.y_out;
+        d.d_y = d.d_y || d.d_merge ? (uint8_t*)workspace + sums : nullptr;
+    }
     const int blocks = (norm_groups(d, p) + p.per - 1) / p.per;
     auto go = [&](auto kern) { kern<<<blocks, p.threads, 0, (hipStream_t)stream>>>(d, p.waves, partial); };
     with_bool(p.whole, [&](auto whole) {
         with_bool(d.norm == FMOE_NORM_LAYER || d.bias || d.next_bias, [&](auto layer) {
             with_bool(d.gate_mode == FMOE_GATE_ELEMENT, [&](auto element) {
-                constexpr bool WHOLE = decltype(whole)::value, LAYER = decltype(layer)::value, ELEMENT = decltype(element)::value;
-                constexpr int THREADS = WHOLE ? kNormBwdWaves * kWave : kNormMostWaves * kWave;
-                if (d.dtype == FMOE_F32) {
-                    if (p.chunks == 1) go(norm_add_bwd_kernel<float, WHOLE, 1, LAYER, ELEMENT, THREADS>);
-                    else if (p.chunks == 2) go(norm_add_bwd_kernel<float, WHOLE, 2, LAYER, ELEMENT, THREADS>);
-                    else if constexpr (WHOLE) go(norm_add_bwd_kernel<float, WHOLE, 4, LAYER, ELEMENT, THREADS>);
-                } else {
-                    if (p.chunks == 1 && p.waves <= kNormBwdWaves) go(norm_add_bwd_kernel<uint16_t, WHOLE, 1, LAYER, ELEMENT, kNormBwdWaves * kWave>);
-                    else if (p.chunks == 1) go(norm_add_bwd_kernel<uint16_t, WHOLE, 1, LAYER, ELEMENT, THREADS>);
-                    else if constexpr (WHOLE) go(norm_add_bwd_kernel<uint16_t, WHOLE, 2, LAYER, ELEMENT, THREADS>);
-                }
+                with_bool(d.K > 0, [&](auto merged) {
+                    constexpr bool WHOLE = decltype(whole)::value, LAYER = decltype(layer)::value, ELEMENT = decltype(element)::value, MERGED = decltype(merged)::value;
+                    constexpr int THREADS = WHOLE ? kNormBwdWaves * kWave : kNormMostWaves * kWave;
+                    if (d.dtype == FMOE_F32) {
+                        if (p.chunks == 1) go(norm_add_bwd_kernel<float, WHOLE, 1, LAYER, ELEMENT, MERGED, THREADS>);
+                        else if (p.chunks == 2) go(norm_add_bwd_kernel<float, WHOLE, 2, LAYER, ELEMENT, MERGED, THREADS>);
+                        else if constexpr (WHOLE) go(norm_add_bwd_kernel<float, WHOLE, 4, LAYER, ELEMENT, MERGED, THREADS>);
+                    } else {
+                        if (p.chunks == 1 && p.waves <= kNormBwdWaves) go(norm_add_bwd_kernel<uint16_t, WHOLE, 1, LAYER, ELEMENT, MERGED, kNormBwdWaves * kWave>);
+                        else if (p.chunks == 1) go(norm_add_bwd_kernel<uint16_t, WHOLE, 1, LAYER, ELEMENT, MERGED, THREADS>);
+                        else if constexpr (WHOLE) go(norm_add_bwd_kernel<uint16_t, WHOLE, 2, LAYER, ELEMENT, MERGED, THREADS>);
+                    }
+                });
             });
         });
     });
-    const int launched = check_launch("fmoe_norm_add_bwd");
-    if (launched != FMOE_OK || !need) return launched;
+    int launched = check_launch("fmoe_norm_add_bwd");
+    if (launched == FMOE_OK && d.K && d.d_y) {
+        const MergeBwdParams m{(const float*)d.d_y, desc->y, d.rows, d.value_rows, d.y_stride, d.token_index, d.merge_index, d.merge, d.cols, d.merge_dtype == FMOE_F32,
+                               desc->d_y, d.d_merge};
+        const unsigned rows = (unsigned)((d.value_rows + 3) / 4);
+        with_bool(p.whole, [&](auto whole) {
+            if (d.dtype == FMOE_F32) norm_merge_bwd_kernel<float, decltype(whole)::value><<<rows, 256, 0, (hipStream_t)stream>>>(m);
+            else norm_merge_bwd_kernel<uint16_t, decltype(whole)::value><<<rows, 256, 0, (hipStream_t)stream>>>(m);
+        });
+        launched = check_launch("fmoe_norm_add_bwd");
+    }
+    if (launched != FMOE_OK || !partial) return launched;
     norm_sums_kernel<<<dim3((d.cols + kSumCols - 1) / kSumCols, kSums), kSumWaves * kWave, 0, (hipStream_t)stream>>>(d, partial, blocks * p.per);
     return check_launch("fmoe_norm_add_bwd");
 }

@@ -87,9 +87,9 @@ class NormDesc(ctypes.Structure):
         ("reverse_index", c_void_p), ("merge", c_void_p), ("merge_index", c_void_p),
         ("residual", c_void_p), ("residual_stride", c_int64), ("gate", c_void_p), ("gate_stride", c_int64),
         ("scale", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("next_weight", c_void_p), ("next_bias", c_void_p),
-        ("out", c_void_p), ("next", c_void_p), ("y_out", c_void_p), ("stats", c_void_p),
+        ("out", c_void_p), ("next", c_void_p), ("y_out", c_void_p), ("stats", c_void_p), ("token_index", c_void_p),
         ("d_out", c_void_p), ("d_next", c_void_p), ("d_y", c_void_p), ("d_residual", c_void_p), ("d_gate", c_void_p),
-        ("d_scale", c_void_p), ("d_weight", c_void_p), ("d_bias", c_void_p), ("d_next_weight", c_void_p), ("d_next_bias", c_void_p),
+        ("d_scale", c_void_p), ("d_weight", c_void_p), ("d_bias", c_void_p), ("d_next_weight", c_void_p), ("d_next_bias", c_void_p), ("d_merge", c_void_p),
     ]
 
 

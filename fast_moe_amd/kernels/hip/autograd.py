@@ -486,15 +486,11 @@ class NormAdd(torch.autograd.Function):
         args = ops.NormArgs(weight, bias, gate, gate_sigmoid, value if scale is None else scale, next_weight, next_bias, eps, norm)
         names = ("merge", "y", "residual", "weight", "bias", "gate", "scale", "next_weight", "next_bias")
         need = dict(zip(names, ctx.needs_input_grad[3:12]))
-        rows = need["y"], need["merge"]
-        need["y"] = need["y"] or need["merge"]
-        grads = ops.norm_add_bwd(merged if K else y, residual, args, stats, d_out, d_next, need)
-        d_merge, d_y = None, grads["y"]
-        if K and d_y is not None:
-            d_y, d_gate = ops.combine_bwd(d_y, y, index, K, merge, merge_index, need_gate_grad=rows[1])
-            if rows[1]:
-                d_merge = d_gate.view(merge.shape).to(merge.dtype)
-        return (None, None, None, d_merge, d_y if rows[0] else None, *(grads[n] for n in names[2:]), None, None, None)
+        grads = ops.norm_add_bwd(y, residual, args, stats, d_out, d_next, need, merged, *((index, merge, merge_index) if K else ()))
+        d_merge = grads["merge"]
+        if d_merge is not None:
+            d_merge = d_merge.view(merge.shape).to(merge.dtype)
+        return (None, None, None, d_merge, *(grads[n] for n in names[1:]), None, None, None)
 
 
 class SwigluBlockCheckpoint8(torch.autograd.Function):

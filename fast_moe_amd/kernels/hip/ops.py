@@ -1011,7 +1011,7 @@ def _norm_desc(name: str, y: Optional[torch.Tensor], residual: torch.Tensor, a: 
 
 def norm_add(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, reverse_index: Optional[torch.Tensor] = None,
              merge: Optional[torch.Tensor] = None, merge_index: Optional[torch.Tensor] = None, for_backward: bool = False):
-    """-> (out, next, y, stats), see fmoe_norm_add; ``y`` is the merged one and it and ``stats`` are None unless ``for_backward``."""
+    """-> (out, next, y, stats), see fmoe_norm_add; ``y`` is the merged one, in fp32; it and ``stats`` are None unless ``for_backward``."""
     name = "norm_add"
     if _is_current(residual):
         parts = _lib.host().norm_add(y, residual, *_norm_operands(a), reverse_index, merge, merge_index, int(for_backward), _stream(residual))
@@ -1043,7 +1043,7 @@ def norm_add(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, rev
                     raise ValueError(f"{name}: merge_index must have {T * K} entries")
                 d.merge_index = merge_index.data_ptr()
     if for_backward:
-        merged = new() if K else None
+        merged = torch.empty(residual.shape, dtype=torch.float32, device=residual.device) if K else None
         stats = torch.empty((T, 4), dtype=torch.float32, device=residual.device)
     d.out, d.next, d.y_out, d.stats = _ptr(out), _ptr(nxt), _ptr(merged), _ptr(stats)
     if T:
@@ -1054,24 +1054,38 @@ def norm_add(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, rev
 
 
 def norm_add_bwd(y: Optional[torch.Tensor], residual: torch.Tensor, a: NormArgs, stats: torch.Tensor, d_out: Optional[torch.Tensor],
-                 d_next: Optional[torch.Tensor], need: Dict[str, bool]) -> Dict[str, Optional[torch.Tensor]]:
-    """Gradients of norm_add by operand name (those ``need`` asks for), see fmoe_norm_add_bwd."""
+                 d_next: Optional[torch.Tensor], need: Dict[str, bool], merged: Optional[torch.Tensor] = None,
+                 token_index: Optional[torch.Tensor] = None, merge: Optional[torch.Tensor] = None,
+                 merge_index: Optional[torch.Tensor] = None) -> Dict[str, Optional[torch.Tensor]]:
+    """Gradients of norm_add by operand name (those ``need`` asks for), see fmoe_norm_add_bwd; with ``merged``, what the forward call kept,
+    y and its gradient are the routed rows and ``merge`` (flat, fp32) is among them."""
     rows = lambda t: None if t is None else t.to(residual.dtype).contiguous()
     d_out, d_next = rows(d_out), rows(d_next)
     if _is_current(residual):
-        names = ("y", "residual", "weight", "bias", "gate", "scale", "next_weight", "next_bias")
+        names = ("y", "residual", "weight", "bias", "gate", "scale", "next_weight", "next_bias", "merge")
         parts = _lib.host().norm_add_bwd(y, residual, *_norm_operands(a), stats, d_out, d_next, sum(1 << i for i, n in enumerate(names) if need.get(n)),
-                                         _stream(residual))
+                                         _stream(residual), merged, token_index, merge, merge_index)
         if parts is not None:
             return dict(zip(names, parts))
-    d, keep = _norm_desc("norm_add_bwd", y, residual, a, residual.shape[0])
     T, D = residual.shape
+    K = token_index.numel() // T if merged is not None and T else 0
+    d, keep = _norm_desc("norm_add_bwd", y, residual, a, T * K if K else T)
     d.stats, d.d_out, d.d_next = stats.data_ptr(), _ptr(d_out), _ptr(d_next)
     grads = {}
-    like = {"y": residual, "residual": residual, "gate": a.gate, "scale": a.scale, "weight": a.weight, "bias": a.bias,
+    like = {"y": y, "residual": residual, "gate": a.gate, "scale": a.scale, "weight": a.weight, "bias": a.bias,
             "next_weight": a.next_weight, "next_bias": a.next_bias}
+    grads["merge"] = torch.zeros((T * K,), dtype=torch.float32, device=residual.device) if need.get("merge") else None
+    if K:
+        token_index = _i64("token_index", token_index)
+        d.K, d.value_rows, d.y_out, d.token_index, d.d_merge = K, T * K, merged.data_ptr(), token_index.data_ptr(), _ptr(grads["merge"])
+        if merge is not None:
+            merge = merge.contiguous()
+            merge_index = None if merge_index is None else _i64("merge_index", merge_index)
+            d.merge, d.merge_dtype, d.merge_index = merge.data_ptr(), _DTYPE_CODE[merge.dtype], _ptr(merge_index)
     for n, t in like.items():
-        grads[n] = torch.empty(t.shape, dtype=t.dtype, device=residual.device) if need.get(n) else None
+        grads[n] = None
+        if need.get(n):
+            grads[n] = empty_rows(*t.shape, t.dtype, t.device) if n == "y" and K else torch.empty(t.shape, dtype=t.dtype, device=t.device)
         if n.startswith("next") and need.get(n) and d_next is None:
             grads[n].zero_()
             continue

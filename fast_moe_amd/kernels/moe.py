@@ -317,7 +317,7 @@ def mul_merge_k_norm_add(index: torch.Tensor, reverse_index: torch.Tensor, value
                          norm: str = "rms", kernel: KernelType = KernelType.HIP) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``block_norm_add`` of the merge of an expert block's rows, without the merged rows' round trip: y is
     ``mul_merge_k_add(index, reverse_index, value, weight=merge_weight, weight_index=weight_index)`` (index: the token of every row),
-    summed in fp32 and not rounded.  For the backward pass the merged rows are kept in value's dtype."""
+    summed in fp32 and not rounded.  For the backward pass the merged rows are kept in fp32."""
     require_hip_kernel(kernel, "mul_merge_k_norm_add")
     N = index.shape[0]
     L, K = reverse_index.shape

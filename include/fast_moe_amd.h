@@ -564,12 +564,13 @@ int fmoe_combine_bwd(const void* dy, const void* value, int value_dtype, int64_t
  *          row r: merge[merge_index ? merge_index[r] : r], 1 if merge is NULL; indices outside [0, rows * K) are left out), in fp32
  *   gate:  one per row (FMOE_GATE_TOKEN, gate[row * gate_stride]) or per element, raw or behind a sigmoid
  *   scale: [cols], or scale_value where it is NULL
- *   y_out [rows, cols]: receives the merged y;  stats [rows, 4] fp32: the rows' means and reciprocals, what the backward pass wants
+ *   y_out [rows, cols] fp32: receives the merged y;  stats [rows, 4] fp32: the rows' means and reciprocals, what the backward pass wants
  * dtype: FMOE_BF16 or FMOE_F32 for y, residual, gate, outputs and their gradients; param_dtype: either, for scale, weights and biases.
  * Outputs, y_out, gradients and merge are contiguous; up to 8192 columns.
- * Backward (y merged already, K = 0): d_out and d_next (either may be NULL) -> every gradient whose pointer is set: d_y, d_residual [rows,
+ * Backward: d_out and d_next (either may be NULL) -> every gradient whose pointer is set: d_y, d_residual [rows,
  * cols], d_gate (per row contiguous, or [rows, cols]), d_scale, d_weight, d_bias, d_next_weight, d_next_bias [cols] in param_dtype, which take
- * a workspace: their sums over rows are added in a fixed order.
+ * a workspace: their sums over rows are added in a fixed order.  K > 0 (a workspace too): y_out is the forward pass's, token_index [rows * K] the
+ * token of every routed row, d_y [rows * K, cols] their gradients, d_merge [rows * K] fp32 those of merge (in its order), made from a d_y in fp32.
  */
 enum fmoe_norm_kind { FMOE_NORM_RMS = 0, FMOE_NORM_LAYER = 1 };
 enum fmoe_gate_mode { FMOE_GATE_NONE = 0, FMOE_GATE_TOKEN = 1, FMOE_GATE_ELEMENT = 2 };
@@ -589,10 +590,12 @@ typedef struct fmoe_norm_desc {
     const void* gate;
     int64_t gate_stride;
     const void *scale, *weight, *bias, *next_weight, *next_bias;
-    void *out, *next, *y_out;
-    float* stats;
+    void *out, *next;
+    float *y_out, *stats;
+    const int64_t* token_index;
     const void *d_out, *d_next;
     void *d_y, *d_residual, *d_gate, *d_scale, *d_weight, *d_bias, *d_next_weight, *d_next_bias;
+    float* d_merge;
 } fmoe_norm_desc;
 int fmoe_norm_add(const fmoe_norm_desc* desc /* host pointer */, fmoe_stream_t stream);
 size_t fmoe_norm_add_bwd_workspace_bytes(const fmoe_norm_desc* desc /* host pointer */);

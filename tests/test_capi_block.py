@@ -109,7 +109,7 @@ def test_norms_refuse_without_a_gpu(lib):
     assert forward(norm(rows=0, residual=None)) == 0
     given = dict(stats=ANY, d_out=ANY, d_y=ANY)
     backward = lambda d: lib.fmoe_norm_add_bwd(ctypes.byref(d), None, 0, None)
-    for bad, message in ((dict(stats=None), "stats and a gradient"), (dict(d_out=None), "stats and a gradient"), (dict(K=1, reverse_index=ANY, value_rows=4), "merged y"),
+    for bad, message in ((dict(stats=None), "stats and a gradient"), (dict(d_out=None), "stats and a gradient"), (dict(K=1, value_rows=4), "merged rows"), (dict(d_merge=ANY), "not there"),
                          (dict(next_weight=None, d_next=ANY), "d_next needs"), (dict(d_scale=ANY), "not there"), (dict(d_gate=ANY), "not there"),
                          (dict(d_bias=ANY), "not there"), (dict(y=None), "not there")):
         d = norm(**dict(given, **bad))

@@ -434,3 +434,17 @@ def test_merged_rows_with_a_gate_for_each_element(T, D, K, dtype, norm, sigmoid)
     close("next", nxt, want["next"])
     for n, t in p.items():      # (the merged rows and their gradients rounded to the rows' dtype)
         close("d_" + n, t.grad, want["d_" + n], rounded=4 * HALF_STEP[dtype])
+
+
+@pytest.mark.parametrize("T,D,K", [(17, 256, 2), (5, 1001, 3), (40, 2048, 8), (3, 6000, 2)])
+@pytest.mark.parametrize("norm,gate", [("rms", "none"), ("layer", "element")])
+def test_nothing_is_rounded_between_the_merge_and_its_gradients(T, D, K, norm, gate):
+    # the merge weights' gradients are sums that cancel (the gradient of a normed row is at right angles to it): bf16 rounds them once, at the end
+    p, merge = make(T, D, BF16, norm, gate, K=K, seed=T + D)
+    for t in p.values():
+        t.requires_grad_(True)
+    d_out, d_next = (torch.randn(T, D, device="cuda").to(BF16) for _ in range(2))
+    torch.autograd.backward(call(p, merge, norm, True), (d_out, d_next))
+    want = formula(p, merge, norm, True, d_out, d_next)
+    for n, t in p.items():
+        close("d_" + n, t.grad, want["d_" + n])
