@@ -30,7 +30,7 @@ constexpr int kRouterRow = 64 + 4;      // floats of a token's sums over 64 expe
 struct FewParams {
     fmoe_few_desc d;
     void* lists;            // who goes where (FewLists)
-    void* h;                // hidden rows [T * k][H]
+    void* h;                // hidden rows [T * k][H]; of bf16 two planes of them, whose sum they are
     const float* logits;    // [stretches][T][E]
     int stretches;          // of the router's own launch, 0: the router is few_up's
     int tiles;              // of few_down that several blocks share, or 0
@@ -194,6 +194,9 @@ __device__ __forceinline__ Entry few_entry(const FewLists& l, int i) {
     const int x = UNIFORM ? uniform((int)v.x) : (int)v.x, y = UNIFORM ? uniform((int)v.y) : (int)v.y;
     return Entry{x & 0xffff, x >> 16, y};
 }
+// Elements of a plane of hidden rows
+__host__ __device__ inline int64_t few_plane(const fmoe_few_desc& d) { return (int64_t)d.T * d.k * d.H; }
+
 // Sums that meet in few_up: two buffers of the 16 waves' accumulators, or 8 shares of the router
 __host__ __device__ constexpr int few_red_bytes(int nt, int mats) { return 2 * kWaves * nt * mats * kWave * 16 > kWaves / 2 * 16 * kRouterRow * 4 ? 2 * kWaves * nt * mats * kWave * 16 : kWaves / 2 * 16 * kRouterRow * 4; }
 
@@ -543,8 +546,13 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
                 }
                 float h = silu_f32(v[0]);
                 if constexpr (GATED) h *= v[1];
-                // bf16: the one rounding between the two products, of the gated value (half a step of bf16, as of the layer's own hidden rows)
-                put_element<F32>(p.h, (int64_t)slot * d.H + col, h * l.gate[slot]);
+                h *= l.gate[slot];
+                const int64_t to = (int64_t)slot * d.H + col;
+                put_element<F32>(p.h, to, h);
+                if constexpr (!F32) {       // what the rounding leaves
+                    const float hi = bf16_bits_to_f32(f32_to_bf16_bits(h));
+                    put_element<false>(p.h, few_plane(d) + to, __builtin_isinf(hi) ? 0.0f : h - hi);
+                }
             }
         }
         clear();
@@ -575,6 +583,9 @@ __global__ __launch_bounds__(kWaves* kWave) void few_up_kernel(FewParams p, int 
 
 // PARTS: a tile has 16 / PARTS output columns, and the MFMAs' rows (and columns: up to 16 / PARTS tokens) hold that many stretches of the
 // contraction side by side, of whose products the diagonal blocks count: more, smaller tiles where 16 columns each would leave CUs without one.
+// bf16: a hidden row is the sum of two, its rounding to bf16 and what that leaves.  The second ones take columns that an expert's tokens leave free, at no more
+// loads or products; an expert with more than half as many tokens as a tile has columns does without them (half a step of bf16 for each hidden value, which
+// makes the output's error 1.4 times that of its own rounding; columns of their own for all of them took 10 to 30 % of this kernel's time).
 // gridDim.y > 1: so many blocks share a tile's contraction; their sums go through memory, and the one that arrives last adds them in block order.
 template <int WT, bool VEC, int NT, int PARTS>
 __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p, bool spread) {
@@ -606,6 +617,8 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p, bo
     uint32_t xoff[NT] = {};
     w.at(d.wo);
     x.at(p.h);
+    const uint32_t second = F32 ? 0u : (uint32_t)(few_plane(d) * XES);      // of a row's two (the workspace is shorter than 2^31 bytes)
+    auto both = [&](const Entry& at) { return !F32 && 2 * at.n <= COLS; };
     const uint32_t woff = (uint32_t)((row - n0) * (int)d.wo_stride_n * ES);
     u32x4 wv[AHEAD][2], xv[AHEAD][2][NT][XC];
     int q = from, index = total ? from / pieces : 0, piece = from - index * pieces;
@@ -619,8 +632,13 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p, bo
             else wrow = (const uint8_t*)d.wo + ((int64_t)next.e * d.wo_stride_e + (int64_t)row * d.wo_stride_n) * ES;
 #pragma unroll
             for (int f = 0; f < NT; ++f) {
-                const int c = 16 * f + r16 % COLS;
-                const uint32_t at = c < next.n ? (uint32_t)(l.slots[next.first + c] * d.H * XES) : ~0u;
+                int c = 16 * f + r16 % COLS;
+                uint32_t at = 0;
+                if (f == 0 && both(next) && c >= COLS / 2) {
+                    c -= COLS / 2;
+                    at = second;
+                }
+                at = c < next.n ? at + (uint32_t)(l.slots[next.first + c] * d.H * XES) : ~0u;
                 if constexpr (ONE) xoff[f] = at;
                 else xrow[f] = at != ~0u ? (const uint8_t*)p.h + at : nullptr;
             }
@@ -659,11 +677,16 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p, bo
 #pragma unroll
             for (int f = 0; f < NT; ++f) {
                 const int c = 16 * f + r16 % COLS;
+                f32x4 own = acc[f];
+                if (f == 0 && both(cur)) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) own[i] += __shfl_xor(acc[0][i], COLS / 2, kWave);
+                }
                 if (c < cur.n && (ONE || quarter * 4 / COLS == part)) {
                     f32x4* const to = reinterpret_cast<f32x4*>(sums + ((size_t)wave * d.T + l.slots[cur.first + c] / d.k) * 16 + 4 * quarter);
                     f32x4 v = *to;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] += E4M3 ? acc[f][i] / inv[i] : acc[f][i];
+                    for (int i = 0; i < 4; ++i) v[i] += E4M3 ? own[i] / inv[i] : own[i];
                     *to = v;
                 }
             }
@@ -736,7 +759,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_down_kernel(FewParams p, bo
 
 // The workspace: the lists as few_up's first block leaves them, and the hidden rows.
 size_t few_hidden_at(const fmoe_few_desc& d) { return ((size_t)few_lists_bytes(d.T, d.E, d.k) + 255) & ~(size_t)255; }
-size_t few_logits_at(const fmoe_few_desc& d) { return (few_hidden_at(d) + (size_t)d.T * d.k * d.H * (d.dtype == FMOE_F32 ? 4 : 2) + 255) & ~(size_t)255; }
+size_t few_logits_at(const fmoe_few_desc& d) { return (few_hidden_at(d) + (size_t)few_plane(d) * 4 + 255) & ~(size_t)255; }
 // Stretches of the router's own launch, 0 where few_up computes the router: 256 CUs reading 256 KB of gate each take 9 us, a launch and its reading back 5.
 // Up to 16 tokens are one block per 16 experts and stretch (4 of them: 4.5 us for 128 experts of 4096); more have blocks of their own, and every stretch is
 // read back for every token: 32 tokens, 128 experts of 4096 11.2 us as one stretch, 7.0 as two, 5.3 as four, which cost the selection 3.

@@ -166,7 +166,8 @@ int fmoe_gate_route_pays(int dtype, int64_t T, int D, int E, int K);
  *   g[t, j] = exp(l_j) / sum over the selected (renorm != 0: the L1-normalised softmax) or over all experts
  *   a       = x[t] . w[e]^T + bias[e],   h = silu(a), or silu(a) * (x[t] . wp[e]^T + bias_p[e]) with wp
  *   out[t]  = sum_j g[t, j] * (h . wo[e]^T + bias_out[e])          fp32 sums, rounded once
- * g * h is rounded to dtype in between (bf16: half a step of 2^-8).  A token whose token_mask byte is 0 reads no expert and gets a row of zeros.
+ * In between g * h is kept in dtype: bf16 as the sum of two (16 bits) where the expert has up to 8 tokens (4 or 2 where there are few output columns),
+ * else rounded (half a step of 2^-8).  A token whose token_mask byte is 0 reads no expert and gets a row of zeros.
  * dtype (tokens, gate, biases, output): FMOE_BF16 or FMOE_F32; weight_dtype: the same, or FMOE_E4M3 with bf16 tokens, which are not
  * quantised (products in bf16, divided by the multiplier scales).  k contiguous in every weight, rows at most 2^20 elements apart.  Rows of whole 16-byte chunks at 16-byte
  * boundaries (8 bytes of e4m3) are read a chunk at a time, others element by element (an order of magnitude slower).  The same inputs give the same bits.

@@ -231,3 +231,27 @@ def test_single_rows_of_any_stride_and_rows_far_apart():
     same = p["weight"][:, :, :1].expand(2, 1, 8)                # every hidden column the same storage
     with pytest.raises(ValueError, match="contraction contiguous"):
         moe.fused_moe_few_tokens(k=1, **dict(p, weight=same, weight_p=None))
+
+
+@pytest.mark.parametrize("T,E,k,D,H,O", [(1, 8, 2, 128, 256, 128), (4, 16, 4, 256, 176, 256), (16, 8, 2, 512, 96, 80), (33, 8, 2, 96, 80, 64), (9, 9, 3, 33, 17, 31)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_bf16_rounds_the_output_and_hardly_anything_else(T, E, k, D, H, O, fp8):
+    p = make(T, E, D, H, O, BF16, True, False, seed=T + 17)
+    plain, pairs = dict(p), {}
+    if fp8:
+        for n in ("weight", "weight_p", "weight_out"):
+            pairs[n] = moe_fp8.quantize_expert_weights(p[n])
+            plain[n] = pairs[n][0].float().double() / pairs[n][1].double()[:, None, :]
+        got = moe_fp8.fused_moe_few_tokens(p["x"], p["gate_weight"], None, pairs["weight"], None, pairs["weight_p"], None, pairs["weight_out"], None, k)
+    else:
+        got = moe.fused_moe_few_tokens(k=k, **p)
+    want, slack = reference(plain, k)
+    # Hidden rows of 16 bits (2^-17 of the value, 2^-16 with room), fp32 sums of up to 512 products and the router's: 2^-14 of the sum of magnitudes holds
+    # them all; then the output's own rounding.  A hidden row's second half has a column that its expert's tokens leave free: an expert with more tokens than
+    # half of them has its hidden rows rounded to bf16, 2^-8 of the value.  Columns: 16, of which narrow outputs of few tokens use a half or a quarter.
+    columns = 16 if T > 8 or O >= 4096 else 8 if T > 4 or O >= 2048 else 4
+    logits = (plain["x"].double().cpu()[:, None, :] * plain["gate_weight"].double().cpu()).sum(dim=2)
+    chosen = torch.zeros(T, E).scatter_(1, torch.sort(logits, descending=True, stable=True, dim=1).indices[:, :k], 1.0)
+    crowded = (chosen * (2 * chosen.sum(dim=0) > columns)).amax(dim=1, keepdim=True).double()
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -14 + 2.0 ** -8 * crowded) * slack + 1e-30
+    assert ((got.double().cpu() - want).abs() <= bound).all()
