@@ -13,8 +13,8 @@
 //   few_down    a block owns 16 output columns for all tokens; its waves share the experts and their contraction.  The gate is folded into h, so
 //               the experts' products add up in one sum.  Where there are few output columns several blocks share them, and the last one
 //               to arrive adds their sums in block order: the same bits every time.
-// Measured, whole passes: 16 tokens (12 of them live), 128 experts of 4096 x 1536 bf16, 2.6 GB 432 us, 6.0 TB/s; 4 tokens, the same in e4m3, 0.55 GB 119 us,
-// 4.6 TB/s; 1 token, 64 experts of 2048 x 1408 bf16, 0.14 GB 40 us, 3.5 TB/s; 37 tokens, 12 experts of 1000 x 2600 fp32, 0.25 GB 89 us, 2.8 TB/s;
+// Measured, whole passes: 16 tokens (12 of them live), 128 experts of 4096 x 1536 bf16, 2.6 GB 437 us, 6.0 TB/s; 4 tokens, the same in e4m3, 0.55 GB 117 us,
+// 4.7 TB/s; 1 token, 64 experts of 2048 x 1408 bf16, 0.14 GB 40 us, 3.5 TB/s; 37 tokens, 12 experts of 1000 x 2600 fp32, 0.25 GB 89 us, 2.8 TB/s;
 // 1 token, 128 x 256, 14 us.  (A 1 GiB copy: 5.2 TB/s.)  Some 12 us of each are the launches, the selection, a first load's way to memory, twice, and the last sums.
 // Weights are the MFMAs' A operand (rows = output columns), tokens its B operand (16 columns).
 #include "common.h"
