@@ -213,7 +213,7 @@ static int ckpt_both(bool write, const char* name, void* g, void* u, int dtype, 
     const CkptRows p{g, u, g_stride, u_stride, rows, (int32_t)cols, (int32_t)fmoe_swiglu_checkpoint_cols(cols), q, e};
     const bool whole = cols % 8 == 0;
     const int64_t n = (rows * (2 * p.padded / (write ? 16 : 8)) + 255) / 256;
-    FMOE_REQUIRE(n < ((int64_t)1 << 31), "%s: too many values for one call", name);
+    FMOE_REQUIRE(n < ((int64_t)1 << 24), "%s: too many values for one call", name);      // (2^32 lanes are a grid)
     const unsigned blocks = (unsigned)n;
     hipStream_t stream = (hipStream_t)stream_;
 #define FMOE_CKPT(kern)                                                                                                    \

@@ -521,6 +521,9 @@ class SwigluBlockCheckpoint8(torch.autograd.Function):
         offsets, index, jagged, weight, bias, weight_p, bias_p, weight_out, bias_out, gates, gates_index, q, e = ctx.saved_tensors
         kept = ops.SwigluCheckpoint(q, e, *ctx.kept)
         K, need = index.shape[1], ctx.needs_input_grad
+        if index.numel() == 0:
+            operands = (None, None, jagged, weight, bias, weight_p, bias_p, weight_out, bias_out, gates, None, None)
+            return tuple(torch.zeros_like(t) if t is not None and n else None for t, n in zip(operands, need))
         dy = dy.to(kept.dtype).contiguous()
         flat = index.reshape(-1)
         need_g = gates is not None and need[9]

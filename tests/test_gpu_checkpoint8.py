@@ -262,3 +262,16 @@ def test_refusals():
     r, p = block(8, 4, 2, 64, 64, BF16, False)
     with pytest.raises(ValueError, match="None or 8"):
         moe.fused_jagged_bmm_swiglu_combine(r["offsets"], r["index"], p["x"], p["w"], None, p["wp"], None, p["wo"], None, 2, checkpoint_bits=4)
+
+
+def test_block_without_tokens():
+    D, H, E, K = 64, 96, 4, 2
+    rnd = lambda *s: torch.randn(*s, device="cuda").to(BF16)
+    p = {"x": rnd(0, D), "w": rnd(E, H, D).permute(0, 2, 1), "b": None, "wp": rnd(E, H, D).permute(0, 2, 1), "bp": None, "wo": rnd(E, D, H).permute(0, 2, 1),
+         "bo": rnd(E, D), "gates": rnd(0, K)}
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    r = {"offsets": torch.zeros(E + 1, dtype=torch.int64, device="cuda"), "index": none.view(0, K), "gate_index": none}
+    y, grads = run_block(r, p, K, 8, rnd(0, D))
+    assert y.shape == (0, D) and len(grads) == 6
+    for n, g in grads.items():
+        assert g.shape == p[n].shape and not g.any()
